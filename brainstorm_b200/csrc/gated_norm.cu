@@ -1,0 +1,410 @@
+// Norms before and after a block, fused with the block's gate and residual scale.
+//
+//   n  = y * r_post * w_post          r_post = (mean(y^2) + eps)^(-1/2)      the norm after the block
+//   x' = x + scale * act(gate) * n                                           gate, residual scale, residual
+//   h  = x' * r_pre * w_pre           r_pre = (mean(x'^2) + eps)^(-1/2)      the norm before the next block
+//
+// One pass over the data in each direction: a row lives in the registers of its threads between the
+// loads and the stores, both means are taken there, and nothing is read twice.  Backward, with
+// x^ = x' r_pre, y^ = y r_post, e = dh w_pre, a = act(gate):
+//
+//   G  = dx' + r_pre (e - x^ mean(e x^))       dx = G          dw_pre = sum_rows dh x^
+//   dgate = G scale n act'                                     dscale = sum_rows G a n
+//   f  = G scale a w_post;  dy = r_post (f - y^ mean(f y^))    dw_post = sum_rows G scale a y^
+//
+// The column sums are kept per block in shared memory (a thread owns its columns, so there is nothing
+// to synchronise), leave one row of partials per block, and are added in a fixed order by a second
+// kernel: no atomics, the same bits every time.
+//
+// Bound: HBM.  Forward moves 5 arrays, backward 8.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace b200 {
+
+constexpr int GN_MAX_WIDTH = 16384;
+
+struct GatedNorm {
+  const float *x, *y, *gate, *w_post, *scale, *w_pre;
+  float *x_out, *h_out, *r_post, *r_pre;
+  int64_t rows, ld_x, ld_y, ld_gate, ld_x_out, ld_h_out;
+  int width, act;
+  float eps;
+};
+struct GatedNormGrad {
+  const float *x_out, *y, *gate, *w_post, *scale, *w_pre, *r_post, *r_pre, *dx_out, *dh;
+  float *dx, *dy, *dgate, *partials;       // partials: one row of 3 * width sums (dw_post, dscale, dw_pre) per block
+  int64_t rows, ld_x_out, ld_y, ld_gate, ld_dx_out, ld_dh, ld_dx, ld_dy, ld_dgate;
+  int width, act, accumulate;
+};
+
+// The activations of the handler (0 sigmoid, 1 tanh, 2 rel, 3 el, 4 linear) and their derivatives as
+// functions of the output.
+__device__ __forceinline__ float gn_act(int act, float x) {
+  switch (act) {
+    case 0: return 1.f / (1.f + expf(-x));
+    case 1: return tanhf(x);
+    case 2: return x > 0.f ? x : (x == x ? 0.f : x);
+    case 3: return x > 0.f ? x : expm1f(x);
+    default: return x;
+  }
+}
+__device__ __forceinline__ float gn_act_deriv(int act, float a) {
+  switch (act) {
+    case 0: return a * (1.f - a);
+    case 1: return 1.f - a * a;
+    case 2: return a > 0.f ? 1.f : 0.f;
+    case 3: return a > 0.f ? 1.f : a + 1.f;
+    default: return 1.f;
+  }
+}
+
+// A row is held by G threads (a power of two, 32 .. 1024), E floats each: VEC = 4: float4 number
+// i * G + t of the row, VEC = 1: float number i * G + t.
+template <int E, int VEC>
+__device__ __forceinline__ void gn_load(float (&v)[E], const float* row, int width, int G, int t) {
+#pragma unroll
+  for (int i = 0; i < E / VEC; ++i) {
+    const int c = (i * G + t) * VEC;
+    if (VEC == 4) {
+      const float4 q = c < width ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    } else {
+      v[i] = c < width ? row[c] : 0.f;
+    }
+  }
+}
+template <int E, int VEC>
+__device__ __forceinline__ void gn_store(const float (&v)[E], float* row, int width, int G, int t) {
+#pragma unroll
+  for (int i = 0; i < E / VEC; ++i) {
+    const int c = (i * G + t) * VEC;
+    if (c < width) {
+      if (VEC == 4) *reinterpret_cast<float4*>(row + c) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      else row[c] = v[i];
+    }
+  }
+}
+template <int E, int VEC>
+__device__ __forceinline__ void gn_add(float (&v)[E], const float* row, int width, int G, int t) {
+#pragma unroll
+  for (int i = 0; i < E / VEC; ++i) {
+    const int c = (i * G + t) * VEC;
+    if (c < width)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[VEC * i + j] = row[c + j] + v[VEC * i + j];
+  }
+}
+// The weight of column slot (i, j) of this thread; 1 where there is no weight vector.
+template <int VEC>
+__device__ __forceinline__ float gn_weight(const float* w, int width, int G, int t, int e) {
+  if (!w) return 1.f;
+  const int c = ((e / VEC) * G + t) * VEC + e % VEC;
+  return c < width ? __ldg(w + c) : 0.f;
+}
+
+// Sum over the G threads of a row, in a fixed order; valid in all of them.  All threads of the block
+// call it together.
+__device__ __forceinline__ float gn_row_sum(float v, int G, float* smem) {
+  v = warp_sum(v);
+  if (G == 32) return v;
+  const int warp = threadIdx.x >> 5, wpr = G >> 5;      // warps per row
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) smem[warp] = v;
+  __syncthreads();
+  const int first = warp - warp % wpr;
+  float s = 0.f;
+  for (int w = 0; w < wpr; ++w) s += smem[first + w];
+  return s;
+}
+
+template <int E, int VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_forward_kernel(GatedNorm p, int G) {
+  __shared__ float red[32];
+  const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
+  const float inv_width = 1.f / (float)p.width;
+  for (int64_t row0 = (int64_t)blockIdx.x * per_block; row0 < p.rows; row0 += (int64_t)gridDim.x * per_block) {
+    const int64_t row = row0 + threadIdx.x / G;
+    const bool live = row < p.rows;
+    float x[E], y[E], g[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = y[e] = g[e] = 0.f;
+    if (live) {
+      gn_load<E, VEC>(x, p.x + row * p.ld_x, p.width, G, t);
+      if (p.y) {
+        gn_load<E, VEC>(y, p.y + row * p.ld_y, p.width, G, t);
+        if (p.gate) gn_load<E, VEC>(g, p.gate + row * p.ld_gate, p.width, G, t);
+      }
+    }
+    if (p.y) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += y[e] * y[e];
+      const float r = 1.f / sqrtf(gn_row_sum(s, G, red) * inv_width + p.eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float a = p.gate ? gn_act(p.act, g[e]) : 1.f;
+        x[e] += gn_weight<VEC>(p.scale, p.width, G, t, e) * a * (y[e] * r * gn_weight<VEC>(p.w_post, p.width, G, t, e));
+      }
+      if (live) {
+        gn_store<E, VEC>(x, p.x_out + row * p.ld_x_out, p.width, G, t);
+        if (t == 0 && p.r_post) p.r_post[row] = r;
+      }
+    }
+    if (p.h_out) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += x[e] * x[e];
+      const float r = 1.f / sqrtf(gn_row_sum(s, G, red) * inv_width + p.eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = x[e] * r * gn_weight<VEC>(p.w_pre, p.width, G, t, e);
+      if (live) {
+        gn_store<E, VEC>(x, p.h_out + row * p.ld_h_out, p.width, G, t);
+        if (t == 0 && p.r_pre) p.r_pre[row] = r;
+      }
+    }
+  }
+}
+
+// Shared memory: three rows of column sums for each group of G threads, E * blockDim.x floats each
+// (slot e of thread t at e * blockDim.x + threadIdx.x: conflict-free, and no thread touches another's).
+template <int E, int VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_backward_kernel(GatedNormGrad p, int G) {
+  extern __shared__ float sums[];
+  __shared__ float red[32];
+  const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
+  float* s_post = sums + threadIdx.x;
+  float* s_scale = s_post + E * blockDim.x;
+  float* s_pre = s_scale + E * blockDim.x;
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_post[e * blockDim.x] = s_scale[e * blockDim.x] = s_pre[e * blockDim.x] = 0.f;
+  const float inv_width = 1.f / (float)p.width;
+  for (int64_t row0 = (int64_t)blockIdx.x * per_block; row0 < p.rows; row0 += (int64_t)gridDim.x * per_block) {
+    const int64_t row = row0 + threadIdx.x / G;
+    const bool live = row < p.rows;
+    float x[E], y[E], g[E], d[E], h[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = y[e] = g[e] = d[e] = h[e] = 0.f;
+    float r_pre = 0.f, r_post = 0.f;
+    if (live) {
+      if (p.dh) {
+        gn_load<E, VEC>(h, p.dh + row * p.ld_dh, p.width, G, t);
+        gn_load<E, VEC>(x, p.x_out + row * p.ld_x_out, p.width, G, t);
+        r_pre = p.r_pre[row];
+      }
+      if (p.dx_out) gn_load<E, VEC>(d, p.dx_out + row * p.ld_dx_out, p.width, G, t);
+      if (p.y) {
+        gn_load<E, VEC>(y, p.y + row * p.ld_y, p.width, G, t);
+        if (p.gate) gn_load<E, VEC>(g, p.gate + row * p.ld_gate, p.width, G, t);
+        r_post = p.r_post[row];
+      }
+    }
+    if (p.dh) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        x[e] *= r_pre;
+        s_pre[e * blockDim.x] += h[e] * x[e];
+        h[e] *= gn_weight<VEC>(p.w_pre, p.width, G, t, e);
+        s += h[e] * x[e];
+      }
+      const float m = gn_row_sum(s, G, red) * inv_width;
+#pragma unroll
+      for (int e = 0; e < E; ++e) d[e] += r_pre * (h[e] - x[e] * m);
+    }
+    if (live) {
+      if (p.accumulate) {
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = d[e];
+        gn_add<E, VEC>(o, p.dx + row * p.ld_dx, p.width, G, t);
+        gn_store<E, VEC>(o, p.dx + row * p.ld_dx, p.width, G, t);
+      } else {
+        gn_store<E, VEC>(d, p.dx + row * p.ld_dx, p.width, G, t);
+      }
+    }
+    if (p.y) {
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float w = gn_weight<VEC>(p.w_post, p.width, G, t, e), sc = gn_weight<VEC>(p.scale, p.width, G, t, e);
+        const float a = p.gate ? gn_act(p.act, g[e]) : 1.f;
+        y[e] *= r_post;
+        s_scale[e * blockDim.x] += d[e] * a * (y[e] * w);
+        const float ds = d[e] * sc;
+        if (p.gate) g[e] = ds * (y[e] * w) * gn_act_deriv(p.act, a);
+        s_post[e * blockDim.x] += ds * a * y[e];
+        d[e] = ds * a * w;
+        s += d[e] * y[e];
+      }
+      const float m = gn_row_sum(s, G, red) * inv_width;
+#pragma unroll
+      for (int e = 0; e < E; ++e) d[e] = r_post * (d[e] - y[e] * m);
+      if (live) {
+        if (p.accumulate) gn_add<E, VEC>(d, p.dy + row * p.ld_dy, p.width, G, t);
+        gn_store<E, VEC>(d, p.dy + row * p.ld_dy, p.width, G, t);
+        if (p.gate) {
+          if (p.accumulate) gn_add<E, VEC>(g, p.dgate + row * p.ld_dgate, p.width, G, t);
+          gn_store<E, VEC>(g, p.dgate + row * p.ld_dgate, p.width, G, t);
+        }
+      }
+    }
+  }
+  if (!p.partials) return;
+  __syncthreads();
+  if (threadIdx.x < G) {      // the groups of the block, in order
+    float* out = p.partials + (int64_t)blockIdx.x * 3 * p.width;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = ((e / VEC) * G + t) * VEC + e % VEC;
+      if (c >= p.width) continue;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const float* col = sums + (int64_t)(k * E + e) * blockDim.x + t;
+        float s = 0.f;
+        for (int q = 0; q < per_block; ++q) s += col[q * G];
+        out[(int64_t)k * p.width + c] = s;
+      }
+    }
+  }
+}
+
+// out[c] (+)= sum over the partial rows of column c, for the three vectors laid side by side.  32
+// columns x 8 slices of rows per block; the slices are added in order.
+__global__ void __launch_bounds__(256) gated_norm_sums_kernel(const float* partials, int blocks, int width, float* dw_post, float* dscale,
+                                                              float* dw_pre, int accumulate) {
+  __shared__ float part[8][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t cols = 3 * (int64_t)width;
+  float s = 0.f;
+  if (c < cols)
+#pragma unroll 4
+    for (int b = slice; b < blocks; b += 8) s += partials[(int64_t)b * cols + c];
+  part[slice][lane] = s;
+  __syncthreads();
+  if (slice || c >= cols) return;
+  s = part[0][lane];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += part[k][lane];
+  const int which = (int)(c / width);
+  float* out = which == 0 ? dw_post : which == 1 ? dscale : dw_pre;
+  if (!out) return;
+  out += c - (int64_t)which * width;
+  *out = accumulate ? *out + s : s;
+}
+
+// Threads per row and floats per thread for a width: the fewest threads (a warp at least) that hold
+// the row in 16 floats each.
+static void gn_shape(int width, int* G, int* E) {
+  int e = width <= 128 ? 4 : width <= 256 ? 8 : 16, g = 32;
+  while (g * e < width) g *= 2;
+  *G = g;
+  *E = e;
+}
+static int gn_backward_blocks(int64_t rows, int width) {
+  int G, E;
+  gn_shape(width, &G, &E);
+  const int threads = std::max(G, 256);
+  const int64_t want = ceil_div(rows, threads / G);
+  return (int)std::min<int64_t>(want, (int64_t)state().sm_count * (threads > 256 ? 1 : 2));
+}
+static bool gn_vec(int width, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
+  if (width % 4) return false;
+  for (const void* p : ptrs) if (!aligned16(p)) return false;
+  for (int64_t l : lds) if (l % 4) return false;
+  return true;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+// Rows of up to 4096 values: blocks of 256 threads; wider ones: one row for a block of 512 or 1024.
+#define GN_KERNELS(KERNEL)                                                                                                \
+  (threads == 1024 ? (vec ? KERNEL<16, 4, 1024> : KERNEL<16, 1, 1024>)                                                     \
+   : threads == 512 ? (vec ? KERNEL<16, 4, 512> : KERNEL<16, 1, 512>)                                                      \
+   : E == 4 ? (vec ? KERNEL<4, 4, 256> : KERNEL<4, 1, 256>)                                                                \
+   : E == 8 ? (vec ? KERNEL<8, 4, 256> : KERNEL<8, 1, 256>)                                                                \
+            : (vec ? KERNEL<16, 4, 256> : KERNEL<16, 1, 256>))
+
+B200_API int b200_gated_norm_forward(const float* x, const float* y, const float* gate, const float* w_post, const float* scale,
+                                     const float* w_pre, float* x_out, float* h_out, float* r_post, float* r_pre, int64_t rows,
+                                     int64_t width, int64_t ld_x, int64_t ld_y, int64_t ld_gate, int64_t ld_x_out, int64_t ld_h_out,
+                                     float eps, int act) {
+  if (int rc = require_ready()) return rc;
+  B200_REQUIRE(rows >= 0 && width >= 0, "negative extent");
+  B200_REQUIRE(width <= GN_MAX_WIDTH, "gated norm: rows of more than %d values are not supported", GN_MAX_WIDTH);
+  B200_REQUIRE(act >= 0 && act <= 4, "unknown activation %d", act);
+  B200_REQUIRE(eps >= 0.f, "gated norm: epsilon must not be negative");
+  if (rows == 0 || width == 0) return B200_OK;
+  B200_REQUIRE(x && (y || h_out), "gated norm: nothing to compute");
+  B200_REQUIRE(!y || x_out, "gated norm: a block output needs x_out");
+  B200_REQUIRE(y || !gate, "gated norm: a gate needs a block output");
+  B200_REQUIRE(ld_x >= width && (!y || (ld_y >= width && ld_x_out >= width)) && (!gate || ld_gate >= width) && (!h_out || ld_h_out >= width),
+               "gated norm: leading dimension too small");
+  GatedNorm p = {x, y, gate, w_post, scale, w_pre, x_out, h_out, r_post, r_pre, rows, ld_x, ld_y, ld_gate, ld_x_out, ld_h_out,
+                 (int)width, act, eps};
+  int G, E;
+  gn_shape((int)width, &G, &E);
+  const bool vec = gn_vec((int)width, {x, y, gate, y ? x_out : nullptr, h_out}, {ld_x, y ? ld_y : 0, gate ? ld_gate : 0, y ? ld_x_out : 0, h_out ? ld_h_out : 0});
+  const int threads = std::max(G, 256);
+  const int blocks = (int)std::min<int64_t>(ceil_div(rows, threads / G), (int64_t)state().sm_count * (threads > 256 ? 1 : 3));
+  GN_KERNELS(gated_norm_forward_kernel)<<<blocks, threads, 0, state().stream>>>(p, G);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+B200_API int64_t b200_gated_norm_scratch_floats(int64_t rows, int64_t width) {
+  if (rows <= 0 || width <= 0 || width > GN_MAX_WIDTH) return 0;
+  return (int64_t)gn_backward_blocks(rows, (int)width) * 3 * width;
+}
+
+B200_API int b200_gated_norm_backward(const float* x_out, const float* y, const float* gate, const float* w_post, const float* scale,
+                                      const float* w_pre, const float* r_post, const float* r_pre, const float* dx_out, const float* dh,
+                                      float* dx, float* dy, float* dgate, float* dw_post, float* dscale, float* dw_pre, int64_t rows,
+                                      int64_t width, int64_t ld_x_out, int64_t ld_y, int64_t ld_gate, int64_t ld_dx_out, int64_t ld_dh,
+                                      int64_t ld_dx, int64_t ld_dy, int64_t ld_dgate, int act, int accumulate, float* scratch,
+                                      int64_t scratch_floats) {
+  if (int rc = require_ready()) return rc;
+  B200_REQUIRE(rows >= 0 && width >= 0, "negative extent");
+  B200_REQUIRE(width <= GN_MAX_WIDTH, "gated norm: rows of more than %d values are not supported", GN_MAX_WIDTH);
+  B200_REQUIRE(act >= 0 && act <= 4, "unknown activation %d", act);
+  const bool sums = dw_post || dscale || dw_pre;
+  if (width == 0) return B200_OK;
+  if (rows == 0) {   // empty sums
+    if (!accumulate)
+      for (float* v : {dw_post, dscale, dw_pre})
+        if (v) B200_CUDA(cudaMemsetAsync(v, 0, (size_t)width * sizeof(float), state().stream));
+    return B200_OK;
+  }
+  B200_REQUIRE(dx && (y || dh), "gated norm: nothing to compute");
+  B200_REQUIRE(!dh || (x_out && r_pre), "gated norm: dh needs x_out and r_pre");
+  B200_REQUIRE(!y || (r_post && dy), "gated norm: a block output needs r_post and dy");
+  B200_REQUIRE(!gate || (y && dgate), "gated norm: a gate needs a block output and dgate");
+  B200_REQUIRE(ld_dx >= width && (!dh || (ld_dh >= width && ld_x_out >= width)) && (!dx_out || ld_dx_out >= width) &&
+                   (!y || (ld_y >= width && ld_dy >= width)) && (!gate || (ld_gate >= width && ld_dgate >= width)),
+               "gated norm: leading dimension too small");
+  const int blocks = gn_backward_blocks(rows, (int)width);
+  B200_REQUIRE(!sums || (scratch && scratch_floats >= (int64_t)blocks * 3 * width), "gated norm: scratch too small");
+  GatedNormGrad p = {x_out, y, gate, w_post, scale, w_pre, r_post, r_pre, dx_out, dh, dx, dy, dgate, sums ? scratch : nullptr, rows,
+                     ld_x_out, ld_y, ld_gate, ld_dx_out, ld_dh, ld_dx, ld_dy, ld_dgate, (int)width, act, accumulate ? 1 : 0};
+  int G, E;
+  gn_shape((int)width, &G, &E);
+  const bool vec = gn_vec((int)width, {dh ? x_out : nullptr, y, gate, dx_out, dh, dx, y ? dy : nullptr, gate ? dgate : nullptr},
+                          {dh ? ld_x_out : 0, y ? ld_y : 0, gate ? ld_gate : 0, dx_out ? ld_dx_out : 0, dh ? ld_dh : 0, ld_dx, y ? ld_dy : 0, gate ? ld_dgate : 0});
+  const int threads = std::max(G, 256);
+  const size_t smem = (size_t)3 * E * threads * sizeof(float);
+  auto kernel = GN_KERNELS(gated_norm_backward_kernel);
+  // 48 KiB and more of dynamic shared memory has to be asked for (the static part counts too)
+  if (smem >= 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<blocks, threads, smem, state().stream>>>(p, G);
+  B200_LAUNCH_CHECK();
+  if (sums) {
+    gated_norm_sums_kernel<<<(unsigned)ceil_div(3 * width, 32), 256, 0, state().stream>>>(scratch, blocks, (int)width, dw_post, dscale, dw_pre,
+                                                                                          accumulate ? 1 : 0);
+    B200_LAUNCH_CHECK();
+  }
+  return B200_OK;
+}

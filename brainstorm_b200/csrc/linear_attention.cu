@@ -1,0 +1,252 @@
+// Decayed linear attention, recurrent form: the state of one (sequence, head) stays in the registers of
+// one block while the tokens pass by.  Serves single tokens (the step of a model that answers) and short
+// sequences.
+//
+// Bound for a single token: HBM, the state is read once and written once (8 dk dv bytes) and everything
+// else is small.  For several tokens: latency, two block barriers for each token.
+#include <algorithm>
+
+#include "linear_attention.cuh"
+
+namespace b200 {
+
+struct LaRuns {
+  LaRun run[3];
+};
+
+// Thread (warp w, lane): column group cg = lane % CG of four columns, rows rl + RL * r, r < R, where
+// rl = w * (32 / CG) + lane / CG and RL = warps * 32 / CG.  VEC: the four columns lie side by side
+// (128-bit accesses); else they are CG apart (coalesced 32-bit ones).
+template <int R, bool VEC>
+__global__ void __launch_bounds__(256) la_recurrent_kernel(LaCommon c, LaRuns runs, int CG) {
+  __shared__ float qkv[2][3 * LA_MAX_DIM];
+  __shared__ float part[8][LA_MAX_DIM];
+  const LaRun p = runs.run[blockIdx.y];
+  const int b = blockIdx.x / c.H, h = blockIdx.x % c.H;
+  const int n = la_length(c, b);
+  const float l = c.decay[h];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int cg = lane % CG, rpw = 32 / CG, RL = warps * rpw, rl = w * rpw + lane / CG;
+  const int dk = p.dk, dv = p.dv;
+  const float* q = p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h;
+  const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h;
+  const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h;
+  float* o = p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h;
+  auto col = [&](int j) { return VEC ? 4 * cg + j : cg + CG * j; };
+
+  float S[R][4];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) S[r][j] = 0.f;
+  if (p.s_in) {
+    const float* s = p.s_in + (int64_t)blockIdx.x * dk * dv;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = rl + RL * r;
+      if (i >= dk) continue;
+      if (VEC && !p.s_in_t) {
+        if (4 * cg < dv) {
+          const float4 x = *reinterpret_cast<const float4*>(s + (int64_t)i * dv + 4 * cg);
+          S[r][0] = x.x; S[r][1] = x.y; S[r][2] = x.z; S[r][3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col(j) < dv) S[r][j] = p.s_in_t ? s[(int64_t)col(j) * dk + i] : s[(int64_t)i * dv + col(j)];
+      }
+    }
+  }
+
+  auto fetch = [&](int step, float* dst) {
+    const int64_t t = p.reverse ? n - 1 - step : step;
+    for (int i = threadIdx.x; i < dk; i += blockDim.x) {
+      dst[i] = q[t * p.qs.t + i];
+      dst[LA_MAX_DIM + i] = k[t * p.ks.t + i] * p.k_scale;
+    }
+    for (int i = threadIdx.x; i < dv; i += blockDim.x) dst[2 * LA_MAX_DIM + i] = v[t * p.vs.t + i];
+  };
+  if (n > 0) fetch(0, qkv[0]);
+  for (int step = 0; step < n; ++step) {
+    __syncthreads();      // this step's token is in place, and the sums of the step before are read
+    const float* now = qkv[step & 1];
+    if (step + 1 < n) fetch(step + 1, qkv[(step + 1) & 1]);
+    const float f = (p.reverse && step == 0) ? 1.f : l;
+    float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = col(j) < dv ? now[2 * LA_MAX_DIM + col(j)] : 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = rl + RL * r;
+      if (i >= dk) continue;
+      const float kk = now[LA_MAX_DIM + i], qq = now[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        S[r][j] = f * S[r][j] + kk * vv[j];
+        acc[j] += qq * S[r][j];
+      }
+    }
+    for (int m = CG; m < 32; m <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], m);
+    if (lane < CG)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col(j) < dv) part[w][col(j)] = acc[j];
+    __syncthreads();
+    const int64_t t = p.reverse ? n - 1 - step : step;
+    for (int i = threadIdx.x; i < dv; i += blockDim.x) {
+      float s = 0.f;
+      for (int u = 0; u < warps; ++u) s += part[u][i];
+      float* dst = o + t * p.os.t + i;
+      *dst = p.accumulate ? *dst + p.o_scale * s : p.o_scale * s;
+    }
+  }
+  if (!p.accumulate)       // tokens behind the end of the sequence
+    for (int64_t t = n; t < c.T; ++t)
+      for (int i = threadIdx.x; i < dv; i += blockDim.x) o[t * p.os.t + i] = 0.f;
+  if (p.s_out) {
+    float* s = p.s_out + (int64_t)blockIdx.x * dk * dv;
+    const float f = (p.reverse && n > 0) ? l : 1.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = rl + RL * r;
+      if (i >= dk) continue;
+      if (VEC) {
+        if (4 * cg < dv)
+          *reinterpret_cast<float4*>(s + (int64_t)i * dv + 4 * cg) = make_float4(f * S[r][0], f * S[r][1], f * S[r][2], f * S[r][3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col(j) < dv) s[(int64_t)i * dv + col(j)] = f * S[r][j];
+      }
+    }
+  }
+}
+
+// One launch for up to three runs over the same sequences (the extents of the widest decide the block).
+int la_recurrent(const LaCommon& c, const LaRun* runs, int count) {
+  LaRuns all = {};
+  int dk = 0, dv = 0;
+  bool vec = true;
+  for (int i = 0; i < count; ++i) {
+    all.run[i] = runs[i];
+    dk = std::max(dk, runs[i].dk);
+    dv = std::max(dv, runs[i].dv);
+    vec = vec && runs[i].dv % 4 == 0 && aligned16(runs[i].s_in) && aligned16(runs[i].s_out);
+  }
+  const int cg = dv <= 32 ? 8 : dv <= 64 ? 16 : 32, rpw = 32 / cg;
+  const int warps = (int)std::min<int64_t>(8, ceil_div(dk, rpw * 4));
+  const int rows = (int)ceil_div(dk, warps * rpw);      // per thread
+  const dim3 grid((unsigned)((int64_t)c.B * c.H), (unsigned)count);
+  const cudaStream_t st = state().stream;
+  if (rows <= 4 && vec) la_recurrent_kernel<4, true><<<grid, warps * 32, 0, st>>>(c, all, cg);
+  else if (rows <= 4) la_recurrent_kernel<4, false><<<grid, warps * 32, 0, st>>>(c, all, cg);
+  else if (rows <= 8 && vec) la_recurrent_kernel<8, true><<<grid, warps * 32, 0, st>>>(c, all, cg);
+  else if (rows <= 8) la_recurrent_kernel<8, false><<<grid, warps * 32, 0, st>>>(c, all, cg);
+  else if (vec) la_recurrent_kernel<16, true><<<grid, warps * 32, 0, st>>>(c, all, cg);
+  else la_recurrent_kernel<16, false><<<grid, warps * 32, 0, st>>>(c, all, cg);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+// dst (T, B, heads, d) (+)= the sum over the `group` operator heads that share a head, in order; src is
+// (T, B, heads * group, d), contiguous.
+__global__ void __launch_bounds__(256) la_share_kernel(const float* src, float* dst, LaStrides ds, int64_t rows, int B, int heads, int group,
+                                                       int d, int accumulate) {
+  const int64_t total = rows * heads * d;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int e = (int)(i % d);
+    const int64_t rh = i / d;
+    const int h = (int)(rh % heads);
+    const int64_t row = rh / heads, t = row / B, b = row % B;
+    const float* s = src + ((row * heads + h) * group) * d + e;
+    float sum = s[0];
+    for (int g = 1; g < group; ++g) sum += s[(int64_t)g * d];
+    float* o = dst + t * ds.t + b * ds.b + h * ds.h + e;
+    *o = accumulate ? *o + sum : sum;
+  }
+}
+
+static int la_run(const LaCommon& c, const LaRun* runs, int count) { return la_recurrent(c, runs, count); }
+
+static int la_check(const char* what, int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv) {
+  B200_REQUIRE(T >= 0 && B >= 0 && H >= 0 && kv_heads >= 0 && dk >= 0 && dv >= 0, "%s: negative extent", what);
+  B200_REQUIRE(B * H == 0 || (dk > 0 && dv > 0), "%s: heads without values", what);
+  B200_REQUIRE(dk <= LA_MAX_DIM && dv <= LA_MAX_DIM, "%s: heads of more than %d values are not supported", what, LA_MAX_DIM);
+  B200_REQUIRE(T < (1ll << 31) && B * H < (1ll << 31), "%s: extent exceeds 2^31", what);
+  B200_REQUIRE(H == 0 || (kv_heads > 0 && H % kv_heads == 0), "%s: %lld heads cannot share %lld key/value heads", what, (long long)H,
+               (long long)kv_heads);
+  return B200_OK;
+}
+// strides: t, b, h of q, k, v and the outputs, in that order
+static LaStrides la_strides(const int64_t* s, int i, int64_t div) { return LaStrides{s[3 * i], s[3 * i + 1], s[3 * i + 2], (int)div}; }
+
+}  // namespace b200
+
+using namespace b200;
+
+B200_API int64_t b200_linear_attention_forward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t dk, int64_t dv) { return 0; }
+
+B200_API int b200_linear_attention_forward(const float* q, const float* k, const float* v, const float* decay, float* out, const float* state,
+                                           float* state_out, const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads,
+                                           int64_t dk, int64_t dv, const int64_t* strides, float scale, float* scratch, int64_t scratch_floats) {
+  if (int rc = require_ready()) return rc;
+  if (int rc = la_check("linear attention", T, B, H, kv_heads, dk, dv)) return rc;
+  if (B * H == 0) return B200_OK;
+  B200_REQUIRE(scratch_floats >= b200_linear_attention_forward_scratch_floats(T, B, H, dk, dv), "linear attention: scratch too small");
+  B200_REQUIRE(decay && (T == 0 || (q && k && v && out && strides)), "linear attention: NULL operand");
+  const int64_t g = H / kv_heads;
+  const int64_t none[12] = {0};
+  const int64_t* s = strides ? strides : none;
+  LaCommon c = {decay, lengths, (int)T, (int)B, (int)H};
+  LaRun r = {q, k, v, out, la_strides(s, 0, 1), la_strides(s, 1, g), la_strides(s, 2, g), la_strides(s, 3, 1), state, state_out, 0, 0,
+             0, (int)dk, (int)dv, 1.f, scale};
+  return la_run(c, &r, 1);
+}
+
+B200_API int64_t b200_linear_attention_backward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv) {
+  return kv_heads < H ? T * B * H * (dk + dv) : 0;
+}
+
+B200_API int b200_linear_attention_backward(const float* q, const float* k, const float* v, const float* decay, const float* dout, float* dq,
+                                            float* dk_out, float* dv_out, const float* state, const float* dstate_out, float* dstate,
+                                            const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv,
+                                            const int64_t* strides, float scale, int accumulate, float* scratch, int64_t scratch_floats) {
+  if (int rc = require_ready()) return rc;
+  if (int rc = la_check("linear attention", T, B, H, kv_heads, dk, dv)) return rc;
+  if (B * H == 0) return B200_OK;
+  B200_REQUIRE(decay && (T == 0 || (q && k && v && dout && dq && dk_out && dv_out && strides)), "linear attention: NULL operand");
+  B200_REQUIRE(scratch_floats >= b200_linear_attention_backward_scratch_floats(T, B, H, kv_heads, dk, dv), "linear attention: scratch too small");
+  const int64_t g = H / kv_heads;
+  const int64_t none[21] = {0};
+  const int64_t* s = strides ? strides : none;
+  const int acc = accumulate ? 1 : 0;
+  LaCommon c = {decay, lengths, (int)T, (int)B, (int)H};
+  const LaStrides qs = la_strides(s, 0, 1), ks = la_strides(s, 1, g), vs = la_strides(s, 2, g), dos = la_strides(s, 3, 1), dqs = la_strides(s, 4, 1);
+  LaStrides dks = la_strides(s, 5, 1), dvs = la_strides(s, 6, 1);
+  float *dk_w = dk_out, *dv_w = dv_out;
+  if (g > 1) {     // one gradient for each head of q first, then the sum over the heads that share
+    dk_w = scratch;
+    dv_w = scratch + T * B * H * dk;
+    dks = LaStrides{B * H * dk, H * dk, dk, 1};
+    dvs = LaStrides{B * H * dv, H * dv, dv, 1};
+  }
+  LaRun runs[3] = {
+      {dout, v, k, dq, dos, vs, ks, dqs, state, nullptr, 1, 0, acc, (int)dv, (int)dk, 1.f, scale},
+      {v, dout, q, dk_w, vs, dos, qs, dks, dstate_out, nullptr, 1, 1, g > 1 ? 0 : acc, (int)dv, (int)dk, scale, 1.f},
+      {k, q, dout, dv_w, ks, qs, dos, dvs, dstate_out, dstate, 0, 1, g > 1 ? 0 : acc, (int)dk, (int)dv, scale, 1.f},
+  };
+  if (int rc = la_run(c, runs, 3)) return rc;
+  if (g > 1 && T > 0) {
+    for (int i = 0; i < 2; ++i) {
+      const int d = (int)(i ? dv : dk);
+      const int64_t total = T * B * kv_heads * d;
+      const int64_t blocks = std::min<int64_t>(ceil_div(total, 256), (int64_t)b200::state().sm_count * 16);
+      la_share_kernel<<<(unsigned)blocks, 256, 0, b200::state().stream>>>(i ? dv_w : dk_w, i ? dv_out : dk_out, la_strides(s, i ? 6 : 5, 1), T * B,
+                                                                          (int)B, (int)kv_heads, (int)g, d, acc);
+      B200_LAUNCH_CHECK();
+    }
+  }
+  return B200_OK;
+}

@@ -1,0 +1,51 @@
+// Decayed linear attention: what its kernels share.
+//
+// For each sequence b and head h, with the head's decay l:
+//
+//   S_t = l S_{t-1} + k_t (x) v_t        o_t = scale * q_t S_t          t = 0 .. n_b - 1
+//
+// Forward and all three gradients are ONE operator with other roles and directions, a `LaRun`:
+//
+//   out:  Q = q,  K = k, V = v,   first token first, S starts from state       (o_scale = scale)
+//   dq:   Q = do, K = v, V = k,   first token first, S starts from state^T     (o_scale = scale)
+//   dk:   Q = v,  K = do, V = q,  last token first,  S starts from dstate_out^T  (k_scale = scale)
+//   dv:   Q = k,  K = q, V = do,  last token first,  S starts from dstate_out   (k_scale = scale), ends as dstate
+//
+// because S_t and its gradient M_t = sum_{s >= t} l^{s-t} scale q_s (x) do_s + l^{n-1-t} dstate_out obey the
+// same recurrence in opposite directions.  Going backwards the incoming state counts undecayed at the
+// first token visited, and the outgoing one is decayed once more (state enters S_0 with a factor l).
+#pragma once
+#include "common.cuh"
+
+namespace b200 {
+
+constexpr int LA_MAX_DIM = 128;
+
+struct LaStrides {      // of a (T, B, heads, d) array with contiguous d; `div`: heads of the operator per head of the array
+  int64_t t, b, h;
+  int div;
+};
+struct LaRun {
+  const float *q, *k, *v;
+  float* o;
+  LaStrides qs, ks, vs, os;
+  const float* s_in;     // (B, H, dk, dv), or (B, H, dv, dk) with s_in_t; NULL = zeros
+  float* s_out;          // (B, H, dk, dv) or NULL
+  int s_in_t, reverse, accumulate;
+  int dk, dv;
+  float k_scale, o_scale;
+};
+struct LaCommon {
+  const float *decay, *lengths;   // (H), (B) or NULL = all T
+  int T, B, H;
+};
+
+// Tokens of sequence b: its length truncated like a label and held to [0, T]; a NaN counts as 0.
+__device__ __forceinline__ int la_length(const LaCommon& c, int b) {
+  if (!c.lengths) return c.T;
+  const float f = c.lengths[b];
+  return !(f >= 1.f) ? 0 : f >= (float)c.T ? c.T : (int)f;
+}
+
+int la_recurrent(const LaCommon& c, const LaRun* runs, int count);
+}  // namespace b200

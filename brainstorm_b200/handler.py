@@ -22,6 +22,7 @@ import numpy as np
 from ._lib import lib, check, B200Error  # noqa: F401
 from .array import B200Array
 from .handler_api import Handler, new_random_state
+from .sequence_ops import SequenceOps
 
 _f32 = np.float32
 _byref = ctypes.byref
@@ -72,7 +73,7 @@ def _matrix(a):
     return rows, cols, a.strides[0] if rows > 1 else cols
 
 
-class B200Handler(Handler):
+class B200Handler(SequenceOps, Handler):
     """Handler backend for one B200 GPU (one process per GPU).
 
     Args:

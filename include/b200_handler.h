@@ -382,6 +382,66 @@ int b200_bn_backward_vectors(const float* sums, float inv_m, const float* gamma,
 int b200_bn_backward_deltas(const float* dout, const float* x_hat, const float* vec, float* in_deltas, int64_t rows, int64_t cols);
 int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int64_t ld, int act);
 
+/* ---- sequence blocks.  The reference has no such operators (its recurrent layers are
+ *      brainstorm/layers/lstm_layer.py:21 and recurrent_layer.py, its gate and norm layers
+ *      highway_layer.py:21 and batch_normalization_layer.py:23, its steppers
+ *      training/steppers.py:46-145); these stand beside them.
+ *
+ *      Decayed linear attention: S_t = decay[h] S_{t-1} + k_t (x) v_t, out_t = scale q_t S_t
+ *      for the first lengths[b] tokens of sequence b (fp32 values truncated like labels and
+ *      held to [0, T]; NULL: all T); out is zero behind them and the state keeps what it was
+ *      at the end.  Arrays are (T, B, heads, d) with contiguous d; `strides` (host memory)
+ *      gives the t, b and head strides in floats of q, k, v, out (forward) and of q, k, v,
+ *      dout, dq, dk, dv (backward).  q, out have H heads, k and v kv_heads, H a multiple of
+ *      kv_heads: head h reads key/value head h / (H / kv_heads).  dk, dv: 1 .. 128.  state,
+ *      state_out, dstate_out, dstate: contiguous (B, H, dk, dv), each may be NULL (zeros in,
+ *      not wanted out); state_out may be state, dstate may be dstate_out; no other output may
+ *      overlap an input or another output.  decay is a constant of the layer, any finite
+ *      values, not differentiated.  Backward: gradients of sum(out * dout) + sum(state_out *
+ *      dstate_out), ADDED to dq, dk, dv (not to dstate) when accumulate is set; they are
+ *      zero behind the end of a sequence.  Sums run in a fixed order, no atomics.
+ *
+ *      Gated norm: with y: r_post = (mean(y^2) + eps)^-1/2, x_out = x + scale * act(gate) *
+ *      (y * r_post * w_post); without y x_out is x.  With h_out: r_pre = (mean(x_out^2) +
+ *      eps)^-1/2, h_out = x_out * r_pre * w_pre.  w_post, scale, w_pre are vectors of `width`
+ *      values or NULL (ones); gate NULL: no gate; act as in b200_bias_act.  Row pitches ld_*;
+ *      width up to 16384.  x_out may be x, h_out may be y.  Backward takes the gradients
+ *      dx_out (NULL: zero) and dh (NULL: no h_out was taken) and gives dx, dy, dgate and the
+ *      vectors dw_post, dscale, dw_pre (each may be NULL); accumulate: all are ADDED to.  dx
+ *      may be dx_out.  scratch of b200_gated_norm_scratch_floats(rows, width) floats for the
+ *      vectors' partial sums.
+ *
+ *      muon_update, for `batch` contiguous (rows, cols) matrices: momentum = beta momentum +
+ *      grad; u = grad + beta momentum if nesterov, else momentum; X = u / (|u|_F + 1e-7);
+ *      `steps` times X = a X + (b A + c A A) X with A = X X^T and (a, b, c) = (3.4445,
+ *      -4.7750, 2.0315); update = X; param = (1 - learning_rate * weight_decay) param -
+ *      learning_rate * X.  16-byte aligned scratch of b200_muon_scratch_floats floats.  The
+ *      four arrays must not overlap. ---------------------------------------------------- */
+int b200_linear_attention_forward(const float* q, const float* k, const float* v, const float* decay, float* out, const float* state,
+                                  float* state_out, const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads,
+                                  int64_t dk, int64_t dv, const int64_t* strides, float scale, float* scratch, int64_t scratch_floats);
+int64_t b200_linear_attention_forward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t dk, int64_t dv);
+int64_t b200_linear_attention_backward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv);
+int b200_linear_attention_backward(const float* q, const float* k, const float* v, const float* decay, const float* dout, float* dq,
+                                   float* dk_out, float* dv_out, const float* state, const float* dstate_out, float* dstate,
+                                   const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv,
+                                   const int64_t* strides, float scale, int accumulate, float* scratch, int64_t scratch_floats);
+int b200_gated_norm_forward(const float* x, const float* y, const float* gate, const float* w_post, const float* scale,
+                            const float* w_pre, float* x_out, float* h_out, float* r_post, float* r_pre, int64_t rows,
+                            int64_t width, int64_t ld_x, int64_t ld_y, int64_t ld_gate, int64_t ld_x_out, int64_t ld_h_out,
+                            float eps, int act);
+int64_t b200_gated_norm_scratch_floats(int64_t rows, int64_t width);
+int b200_gated_norm_backward(const float* x_out, const float* y, const float* gate, const float* w_post, const float* scale,
+                             const float* w_pre, const float* r_post, const float* r_pre, const float* dx_out, const float* dh,
+                             float* dx, float* dy, float* dgate, float* dw_post, float* dscale, float* dw_pre, int64_t rows,
+                             int64_t width, int64_t ld_x_out, int64_t ld_y, int64_t ld_gate, int64_t ld_dx_out, int64_t ld_dh,
+                             int64_t ld_dx, int64_t ld_dy, int64_t ld_dgate, int act, int accumulate, float* scratch,
+                             int64_t scratch_floats);
+int64_t b200_muon_scratch_floats(int64_t batch, int64_t rows, int64_t cols);
+int b200_muon_update(float* param, const float* grad, float* momentum, float* update, int64_t batch, int64_t rows, int64_t cols,
+                     float learning_rate, float beta, int nesterov, float weight_decay, int steps, float* scratch,
+                     int64_t scratch_floats);
+
 /* ---- random: generate_probability_mask :507, fill_gaussian :494;
  *      numpy_handler.py:199,193.  Device-side Philox4x32-10 streams addressed by
  *      (seed, offset); the host-RNG parity mode of the Python handler does not
