@@ -168,7 +168,11 @@ __global__ void __launch_bounds__(256) la_share_kernel(const float* src, float* 
   }
 }
 
-static int la_run(const LaCommon& c, const LaRun* runs, int count) { return la_recurrent(c, runs, count); }
+constexpr int LA_RECURRENT_TOKENS = 8;      // sequences of up to this many tokens take the recurrent form
+
+static int la_run(const LaCommon& c, const LaRun* runs, int count, float* work) {
+  return c.T <= LA_RECURRENT_TOKENS ? la_recurrent(c, runs, count) : la_chunked(c, runs, count, work);
+}
 
 static int la_check(const char* what, int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv) {
   B200_REQUIRE(T >= 0 && B >= 0 && H >= 0 && kv_heads >= 0 && dk >= 0 && dv >= 0, "%s: negative extent", what);
@@ -186,7 +190,10 @@ static LaStrides la_strides(const int64_t* s, int i, int64_t div) { return LaStr
 
 using namespace b200;
 
-B200_API int64_t b200_linear_attention_forward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t dk, int64_t dv) { return 0; }
+B200_API int64_t b200_linear_attention_forward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t dk, int64_t dv) {
+  if (T <= LA_RECURRENT_TOKENS || B * H <= 0 || dk <= 0 || dv <= 0 || dk > LA_MAX_DIM || dv > LA_MAX_DIM) return 0;
+  return la_chunked_work(T, B * H, (int)dk, (int)dv, false);
+}
 
 B200_API int b200_linear_attention_forward(const float* q, const float* k, const float* v, const float* decay, float* out, const float* state,
                                            float* state_out, const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads,
@@ -202,11 +209,12 @@ B200_API int b200_linear_attention_forward(const float* q, const float* k, const
   LaCommon c = {decay, lengths, (int)T, (int)B, (int)H};
   LaRun r = {q, k, v, out, la_strides(s, 0, 1), la_strides(s, 1, g), la_strides(s, 2, g), la_strides(s, 3, 1), state, state_out, 0, 0,
              0, (int)dk, (int)dv, 1.f, scale};
-  return la_run(c, &r, 1);
+  return la_run(c, &r, 1, scratch);
 }
 
 B200_API int64_t b200_linear_attention_backward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv) {
-  return kv_heads < H ? T * B * H * (dk + dv) : 0;
+  if (T <= 0 || B * H <= 0 || dk <= 0 || dv <= 0 || dk > LA_MAX_DIM || dv > LA_MAX_DIM) return 0;
+  return (kv_heads < H ? T * B * H * (dk + dv) : 0) + (T <= LA_RECURRENT_TOKENS ? 0 : la_chunked_work(T, B * H, (int)dk, (int)dv, true));
 }
 
 B200_API int b200_linear_attention_backward(const float* q, const float* k, const float* v, const float* decay, const float* dout, float* dq,
@@ -218,6 +226,7 @@ B200_API int b200_linear_attention_backward(const float* q, const float* k, cons
   if (B * H == 0) return B200_OK;
   B200_REQUIRE(decay && (T == 0 || (q && k && v && dout && dq && dk_out && dv_out && strides)), "linear attention: NULL operand");
   B200_REQUIRE(scratch_floats >= b200_linear_attention_backward_scratch_floats(T, B, H, kv_heads, dk, dv), "linear attention: scratch too small");
+  B200_REQUIRE(!dstate || dstate != dstate_out, "linear attention: dstate overlaps dstate_out");   // two gradients read it
   const int64_t g = H / kv_heads;
   const int64_t none[21] = {0};
   const int64_t* s = strides ? strides : none;
@@ -237,7 +246,7 @@ B200_API int b200_linear_attention_backward(const float* q, const float* k, cons
       {v, dout, q, dk_w, vs, dos, qs, dks, dstate_out, nullptr, 1, 1, g > 1 ? 0 : acc, (int)dv, (int)dk, scale, 1.f},
       {k, q, dout, dv_w, ks, qs, dos, dvs, dstate_out, dstate, 0, 1, g > 1 ? 0 : acc, (int)dk, (int)dv, scale, 1.f},
   };
-  if (int rc = la_run(c, runs, 3)) return rc;
+  if (int rc = la_run(c, runs, 3, scratch + (g > 1 ? T * B * H * (dk + dv) : 0))) return rc;
   if (g > 1 && T > 0) {
     for (int i = 0; i < 2; ++i) {
       const int d = (int)(i ? dv : dk);

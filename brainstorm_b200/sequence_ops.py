@@ -79,12 +79,22 @@ def _expect(a, shape, what):
 
 def _span(a):
     """[first, last) address of a view."""
+    if a._contig:
+        return a.ptr, a.ptr + 4 * a.size
     return a.ptr, a.ptr + 4 * (sum((n - 1) * s for n, s in zip(a.shape, a.strides)) + 1)
 
 
 def _apart(outputs, inputs, allowed=()):
     """Refuse an output that starts where another operand starts, and contiguous ones that overlap at all
     (two row-pitched views may interleave in one buffer, as the columns of a hub do)."""
+    spans = sorted([_span(a) for _, a in outputs if a is not None and a.size] + [_span(a) for _, a in inputs if a is not None and a.size])
+    end = 0
+    for lo, hi in spans:
+        if lo < end:
+            break
+        end = hi
+    else:
+        return              # no two operands meet anywhere
     seen = [(n, a) for n, a in inputs if a is not None and a.size]
     for name, a in outputs:
         if a is None or not a.size:
@@ -132,15 +142,14 @@ class SequenceOps(object):
                                   accumulate=True):
         """Gradients of ``linear_attention_forward``: adds to ``dq``, ``dk``, ``dv`` (overwrites them without
         ``accumulate``) and writes ``dstate``, the gradient of ``state``.  ``dstate_out`` is the gradient of
-        ``state_out`` (None: zero); ``dstate`` may be ``dstate_out``.  Gradients are zero behind the end of a
+        ``state_out`` (None: zero).  Gradients are zero behind the end of a
         sequence; ``dout`` is not read there."""
         T, B, H, K, d_k, d_v = self._attention_shapes(q, k, v, 4)
         for a, shape, what in ((dout, (T, B, H, d_v), 'dout'), (dq, q.shape, 'dq'), (dk, k.shape, 'dk'), (dv, v.shape, 'dv')):
             _expect(a, shape, what)
         arrays = (('q', q), ('k', k), ('v', v), ('dout', dout), ('dq', dq), ('dk', dk), ('dv', dv))
         strides = (ctypes.c_int64 * 21)(*[s for what, a in arrays for s in _heads(a, 4, what)])
-        _apart(arrays[4:] + (('dstate', dstate),), arrays[:4] + (('decay', decay), ('state', state), ('dstate_out', dstate_out), ('lengths', lengths)),
-               (('dstate', 'dstate_out'),))
+        _apart(arrays[4:] + (('dstate', dstate),), arrays[:4] + (('decay', decay), ('state', state), ('dstate_out', dstate_out), ('lengths', lengths)))
         states = (B, H, d_k, d_v)
         work, need = self._attention_work(lib.b200_linear_attention_backward_scratch_floats(T, B, H, K, d_k, d_v))
         check(lib.b200_linear_attention_backward(

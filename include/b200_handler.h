@@ -395,11 +395,13 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      dout, dq, dk, dv (backward).  q, out have H heads, k and v kv_heads, H a multiple of
  *      kv_heads: head h reads key/value head h / (H / kv_heads).  dk, dv: 1 .. 128.  state,
  *      state_out, dstate_out, dstate: contiguous (B, H, dk, dv), each may be NULL (zeros in,
- *      not wanted out); state_out may be state, dstate may be dstate_out; no other output may
- *      overlap an input or another output.  decay is a constant of the layer, any finite
+ *      not wanted out); state_out may be state; no other output may overlap
+ *      an input or another output.  decay is a constant of the layer, any finite
  *      values, not differentiated.  Backward: gradients of sum(out * dout) + sum(state_out *
  *      dstate_out), ADDED to dq, dk, dv (not to dstate) when accumulate is set; they are
  *      zero behind the end of a sequence.  Sums run in a fixed order, no atomics.
+ *      16-byte aligned scratch of the given number of floats (0: NULL will do; it depends on the
+ *      extents and on the number of SMs).
  *
  *      Gated norm: with y: r_post = (mean(y^2) + eps)^-1/2, x_out = x + scale * act(gate) *
  *      (y * r_post * w_post); without y x_out is x.  With h_out: r_pre = (mean(x_out^2) +

@@ -201,10 +201,6 @@ def test_state_in_place(handler, T):
     h.linear_attention_forward(p['q'], p['k'], p['v'], p['decay'], out, state=p['state'], state_out=p['state'])
     assert np.array_equal(h.get_numpy_copy(p['state']), apart['state_out'])
     assert np.array_equal(h.get_numpy_copy(out), apart['out'])
-    g = [h.zeros(d[n].shape) for n in 'qkv']
-    p['state'] = h.create_from_numpy(d['state'])
-    h.linear_attention_backward(p['q'], p['k'], p['v'], p['decay'], p['dout'], *g, state=p['state'], dstate_out=p['dstate_out'], dstate=p['dstate_out'])
-    assert np.array_equal(h.get_numpy_copy(p['dstate_out']), apart['dstate'])
 
 
 @pytest.mark.gpu
@@ -397,6 +393,9 @@ def test_refusals_of_overlaps_and_strides():
         _calls().linear_attention_backward(q, k, v, decay, out, out, s(5, 4, 2, 2, 8), s(6, 4, 2, 2, 8))
     with pytest.raises(ValueError, match='dv overlaps dk'):
         _calls().linear_attention_backward(q, k, v, decay, out, s(5, 4, 2, 4, 8), s(6, 4, 2, 2, 8), s(6, 4, 2, 2, 8))
+    state = s(9, 2, 4, 8, 8)
+    with pytest.raises(ValueError, match='dstate overlaps dstate_out'):
+        _calls().linear_attention_backward(q, k, v, decay, out, s(5, 4, 2, 4, 8), s(6, 4, 2, 2, 8), s(7, 4, 2, 2, 8), dstate_out=state, dstate=state)
     with pytest.raises(ValueError, match='3 dimensions'):
         _calls().linear_attention_step(q, k, v, decay, s(5, 2, 4, 8, 8), out)
 
