@@ -43,7 +43,7 @@ struct GatedNormGrad {
 // functions of the output.
 __device__ __forceinline__ float gn_act(int act, float x) {
   switch (act) {
-    case 0: return 1.f / (1.f + expf(-x));
+    case 0: return __fdividef(1.f, 1.f + expf(-x));      // two units in the last place; 0 for x < -87
     case 1: return tanhf(x);
     case 2: return x > 0.f ? x : (x == x ? 0.f : x);
     case 3: return x > 0.f ? x : expm1f(x);
@@ -96,12 +96,42 @@ __device__ __forceinline__ void gn_add(float (&v)[E], const float* row, int widt
       for (int j = 0; j < VEC; ++j) v[VEC * i + j] = row[c + j] + v[VEC * i + j];
   }
 }
-// The weight of column slot (i, j) of this thread; 1 where there is no weight vector.
-template <int VEC>
-__device__ __forceinline__ float gn_weight(const float* w, int width, int G, int t, int e) {
-  if (!w) return 1.f;
-  const int c = ((e / VEC) * G + t) * VEC + e % VEC;
-  return c < width ? __ldg(w + c) : 0.f;
+// The weights of this thread's columns; ones where there is no vector.
+template <int E, int VEC>
+__device__ __forceinline__ void gn_weights(float (&v)[E], const float* w, int width, int G, int t) {
+  if (w) {
+    gn_load<E, VEC>(v, w, width, G, t);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 1.f;
+  }
+}
+// v[e] = act(v[e]) with the choice outside the loop
+template <int E>
+__device__ __forceinline__ void gn_act_all(int act, float (&v)[E]) {
+  if (act == 0) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = gn_act(0, v[e]);
+  } else if (act == 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = gn_act(1, v[e]);
+  } else if (act == 2) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = gn_act(2, v[e]);
+  } else if (act == 3) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = gn_act(3, v[e]);
+  }
+}
+// Column sums in shared memory: float4 number i of thread t at i * threads + t.
+template <int E>
+__device__ __forceinline__ void gn_sum_into(float4* s, const float (&v)[E]) {
+#pragma unroll
+  for (int i = 0; i < E / 4; ++i) {
+    float4 q = s[i * blockDim.x];
+    q.x += v[4 * i]; q.y += v[4 * i + 1]; q.z += v[4 * i + 2]; q.w += v[4 * i + 3];
+    s[i * blockDim.x] = q;
+  }
 }
 
 // Sum over the G threads of a row, in a fixed order; valid in all of them.  All threads of the block
@@ -142,23 +172,33 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_fo
 #pragma unroll
       for (int e = 0; e < E; ++e) s += y[e] * y[e];
       const float r = 1.f / sqrtf(gn_row_sum(s, G, red) * inv_width + p.eps);
+      if (p.gate) {
+        gn_act_all<E>(p.act, g);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float a = p.gate ? gn_act(p.act, g[e]) : 1.f;
-        x[e] += gn_weight<VEC>(p.scale, p.width, G, t, e) * a * (y[e] * r * gn_weight<VEC>(p.w_post, p.width, G, t, e));
+        for (int e = 0; e < E; ++e) y[e] = y[e] * r * g[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] *= r;
       }
+      gn_weights<E, VEC>(g, p.w_post, p.width, G, t);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] *= g[e];
+      gn_weights<E, VEC>(g, p.scale, p.width, G, t);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] += y[e] * g[e];
       if (live) {
         gn_store<E, VEC>(x, p.x_out + row * p.ld_x_out, p.width, G, t);
         if (t == 0 && p.r_post) p.r_post[row] = r;
       }
     }
     if (p.h_out) {
+      gn_weights<E, VEC>(g, p.w_pre, p.width, G, t);
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) s += x[e] * x[e];
       const float r = 1.f / sqrtf(gn_row_sum(s, G, red) * inv_width + p.eps);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = x[e] * r * gn_weight<VEC>(p.w_pre, p.width, G, t, e);
+      for (int e = 0; e < E; ++e) x[e] = x[e] * r * g[e];
       if (live) {
         gn_store<E, VEC>(x, p.h_out + row * p.ld_h_out, p.width, G, t);
         if (t == 0 && p.r_pre) p.r_pre[row] = r;
@@ -167,18 +207,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_fo
   }
 }
 
-// Shared memory: three rows of column sums for each group of G threads, E * blockDim.x floats each
-// (slot e of thread t at e * blockDim.x + threadIdx.x: conflict-free, and no thread touches another's).
+// Shared memory: three vectors of column sums for each group of G threads (gn_sum_into).
 template <int E, int VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_backward_kernel(GatedNormGrad p, int G) {
-  extern __shared__ float sums[];
+  extern __shared__ float4 sums[];
   __shared__ float red[32];
   const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
-  float* s_post = sums + threadIdx.x;
-  float* s_scale = s_post + E * blockDim.x;
-  float* s_pre = s_scale + E * blockDim.x;
+  float4* s_post = sums + threadIdx.x;
+  float4* s_scale = s_post + E / 4 * blockDim.x;
+  float4* s_pre = s_scale + E / 4 * blockDim.x;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s_post[e * blockDim.x] = s_scale[e * blockDim.x] = s_pre[e * blockDim.x] = 0.f;
+  for (int i = 0; i < E / 4; ++i) s_post[i * blockDim.x] = s_scale[i * blockDim.x] = s_pre[i * blockDim.x] = make_float4(0.f, 0.f, 0.f, 0.f);
   const float inv_width = 1.f / (float)p.width;
   for (int64_t row0 = (int64_t)blockIdx.x * per_block; row0 < p.rows; row0 += (int64_t)gridDim.x * per_block) {
     const int64_t row = row0 + threadIdx.x / G;
@@ -201,12 +240,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
       }
     }
     if (p.dh) {
-      float s = 0.f;
+      float s = 0.f, w[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         x[e] *= r_pre;
-        s_pre[e * blockDim.x] += h[e] * x[e];
-        h[e] *= gn_weight<VEC>(p.w_pre, p.width, G, t, e);
+        w[e] = h[e] * x[e];
+      }
+      gn_sum_into<E>(s_pre, w);
+      gn_weights<E, VEC>(w, p.w_pre, p.width, G, t);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        h[e] *= w[e];
         s += h[e] * x[e];
       }
       const float m = gn_row_sum(s, G, red) * inv_width;
@@ -225,19 +269,39 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
       }
     }
     if (p.y) {
-      float s = 0.f;
+      // x and h are free: x = act(gate), h = n = y^ w_post, w the weights
+      float s = 0.f, w[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = p.gate ? g[e] : 1.f;
+      if (p.gate) gn_act_all<E>(p.act, x);
+      gn_weights<E, VEC>(w, p.w_post, p.width, G, t);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float w = gn_weight<VEC>(p.w_post, p.width, G, t, e), sc = gn_weight<VEC>(p.scale, p.width, G, t, e);
-        const float a = p.gate ? gn_act(p.act, g[e]) : 1.f;
         y[e] *= r_post;
-        s_scale[e * blockDim.x] += d[e] * a * (y[e] * w);
-        const float ds = d[e] * sc;
-        if (p.gate) g[e] = ds * (y[e] * w) * gn_act_deriv(p.act, a);
-        s_post[e * blockDim.x] += ds * a * y[e];
-        d[e] = ds * a * w;
+        h[e] = y[e] * w[e];
+        g[e] = d[e] * x[e] * h[e];
+      }
+      gn_sum_into<E>(s_scale, g);
+      gn_weights<E, VEC>(g, p.scale, p.width, G, t);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        d[e] *= g[e];                                             // G scale
+        g[e] = d[e] * h[e];                                       // without act'
+        d[e] *= x[e];
+        h[e] = d[e] * y[e];
+        d[e] *= w[e];
         s += d[e] * y[e];
       }
+      if (p.gate) {
+        if (p.act == 0) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) g[e] *= gn_act_deriv(0, x[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) g[e] *= gn_act_deriv(p.act, x[e]);
+        }
+      }
+      gn_sum_into<E>(s_post, h);
       const float m = gn_row_sum(s, G, red) * inv_width;
 #pragma unroll
       for (int e = 0; e < E; ++e) d[e] = r_post * (d[e] - y[e] * m);
@@ -261,9 +325,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
       if (c >= p.width) continue;
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        const float* col = sums + (int64_t)(k * E + e) * blockDim.x + t;
+        const float* col = reinterpret_cast<const float*>(sums + (int64_t)(k * (E / 4) + e / 4) * blockDim.x + t) + e % 4;
         float s = 0.f;
-        for (int q = 0; q < per_block; ++q) s += col[q * G];
+        for (int q = 0; q < per_block; ++q) s += col[4 * q * G];
         out[(int64_t)k * p.width + c] = s;
       }
     }
@@ -295,20 +359,16 @@ __global__ void __launch_bounds__(256) gated_norm_sums_kernel(const float* parti
   *out = accumulate ? *out + s : s;
 }
 
-// Threads per row and floats per thread for a width: the fewest threads (a warp at least) that hold
-// the row in 16 floats each.
-static void gn_shape(int width, int* G, int* E) {
-  int e = width <= 128 ? 4 : width <= 256 ? 8 : 16, g = 32;
+// Threads per row and floats per thread for a width: the fewest threads (a warp at least) that hold the row
+// in 16 floats each, 8 where single loads with their bounds need the registers.
+static void gn_shape(int width, bool vec, int* G, int* E) {
+  int e = width <= 128 ? 4 : (width <= 256 || (!vec && width <= 8192)) ? 8 : 16, g = 32;
   while (g * e < width) g *= 2;
   *G = g;
   *E = e;
 }
-static int gn_backward_blocks(int64_t rows, int width) {
-  int G, E;
-  gn_shape(width, &G, &E);
-  const int threads = std::max(G, 256);
-  const int64_t want = ceil_div(rows, threads / G);
-  return (int)std::min<int64_t>(want, (int64_t)state().sm_count * (threads > 256 ? 1 : 2));
+static int gn_blocks(int64_t rows, int G, int threads, int per_sm) {
+  return (int)std::min<int64_t>(ceil_div(rows, threads / G), (int64_t)state().sm_count * (threads > 256 ? 1 : per_sm));
 }
 static bool gn_vec(int width, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
   if (width % 4) return false;
@@ -323,8 +383,8 @@ using namespace b200;
 
 // Rows of up to 4096 values: blocks of 256 threads; wider ones: one row for a block of 512 or 1024.
 #define GN_KERNELS(KERNEL)                                                                                                \
-  (threads == 1024 ? (vec ? KERNEL<16, 4, 1024> : KERNEL<16, 1, 1024>)                                                     \
-   : threads == 512 ? (vec ? KERNEL<16, 4, 512> : KERNEL<16, 1, 512>)                                                      \
+  (threads == 1024 ? (vec ? KERNEL<16, 4, 1024> : E == 8 ? KERNEL<8, 1, 1024> : KERNEL<16, 1, 1024>)                       \
+   : threads == 512 ? (vec ? KERNEL<16, 4, 512> : E == 8 ? KERNEL<8, 1, 512> : KERNEL<16, 1, 512>)                         \
    : E == 4 ? (vec ? KERNEL<4, 4, 256> : KERNEL<4, 1, 256>)                                                                \
    : E == 8 ? (vec ? KERNEL<8, 4, 256> : KERNEL<8, 1, 256>)                                                                \
             : (vec ? KERNEL<16, 4, 256> : KERNEL<16, 1, 256>))
@@ -346,11 +406,11 @@ B200_API int b200_gated_norm_forward(const float* x, const float* y, const float
                "gated norm: leading dimension too small");
   GatedNorm p = {x, y, gate, w_post, scale, w_pre, x_out, h_out, r_post, r_pre, rows, ld_x, ld_y, ld_gate, ld_x_out, ld_h_out,
                  (int)width, act, eps};
+  const bool vec = gn_vec((int)width, {x, y, gate, y ? x_out : nullptr, h_out}, {ld_x, y ? ld_y : 0, gate ? ld_gate : 0, y ? ld_x_out : 0, h_out ? ld_h_out : 0}) &&
+                   aligned16(w_post) && aligned16(scale) && aligned16(w_pre);
   int G, E;
-  gn_shape((int)width, &G, &E);
-  const bool vec = gn_vec((int)width, {x, y, gate, y ? x_out : nullptr, h_out}, {ld_x, y ? ld_y : 0, gate ? ld_gate : 0, y ? ld_x_out : 0, h_out ? ld_h_out : 0});
-  const int threads = std::max(G, 256);
-  const int blocks = (int)std::min<int64_t>(ceil_div(rows, threads / G), (int64_t)state().sm_count * (threads > 256 ? 1 : 3));
+  gn_shape((int)width, vec, &G, &E);
+  const int threads = std::max(G, 256), blocks = gn_blocks(rows, G, threads, 3);
   GN_KERNELS(gated_norm_forward_kernel)<<<blocks, threads, 0, state().stream>>>(p, G);
   B200_LAUNCH_CHECK();
   return B200_OK;
@@ -358,7 +418,7 @@ B200_API int b200_gated_norm_forward(const float* x, const float* y, const float
 
 B200_API int64_t b200_gated_norm_scratch_floats(int64_t rows, int64_t width) {
   if (rows <= 0 || width <= 0 || width > GN_MAX_WIDTH) return 0;
-  return (int64_t)gn_backward_blocks(rows, (int)width) * 3 * width;
+  return std::min<int64_t>(rows, (int64_t)state().sm_count * 2) * 3 * width;      // a row of sums for each block, at most
 }
 
 B200_API int b200_gated_norm_backward(const float* x_out, const float* y, const float* gate, const float* w_post, const float* scale,
@@ -386,15 +446,15 @@ B200_API int b200_gated_norm_backward(const float* x_out, const float* y, const 
   B200_REQUIRE(ld_dx >= width && (!dh || (ld_dh >= width && ld_x_out >= width)) && (!dx_out || ld_dx_out >= width) &&
                    (!y || (ld_y >= width && ld_dy >= width)) && (!gate || (ld_gate >= width && ld_dgate >= width)),
                "gated norm: leading dimension too small");
-  const int blocks = gn_backward_blocks(rows, (int)width);
-  B200_REQUIRE(!sums || (scratch && scratch_floats >= (int64_t)blocks * 3 * width), "gated norm: scratch too small");
+  B200_REQUIRE(!sums || (scratch && scratch_floats >= b200_gated_norm_scratch_floats(rows, width)), "gated norm: scratch too small");
   GatedNormGrad p = {x_out, y, gate, w_post, scale, w_pre, r_post, r_pre, dx_out, dh, dx, dy, dgate, sums ? scratch : nullptr, rows,
                      ld_x_out, ld_y, ld_gate, ld_dx_out, ld_dh, ld_dx, ld_dy, ld_dgate, (int)width, act, accumulate ? 1 : 0};
-  int G, E;
-  gn_shape((int)width, &G, &E);
   const bool vec = gn_vec((int)width, {dh ? x_out : nullptr, y, gate, dx_out, dh, dx, y ? dy : nullptr, gate ? dgate : nullptr},
-                          {dh ? ld_x_out : 0, y ? ld_y : 0, gate ? ld_gate : 0, dx_out ? ld_dx_out : 0, dh ? ld_dh : 0, ld_dx, y ? ld_dy : 0, gate ? ld_dgate : 0});
-  const int threads = std::max(G, 256);
+                          {dh ? ld_x_out : 0, y ? ld_y : 0, gate ? ld_gate : 0, dx_out ? ld_dx_out : 0, dh ? ld_dh : 0, ld_dx, y ? ld_dy : 0, gate ? ld_dgate : 0}) &&
+                   aligned16(w_post) && aligned16(scale) && aligned16(w_pre);
+  int G, E;
+  gn_shape((int)width, vec, &G, &E);
+  const int threads = std::max(G, 256), blocks = gn_blocks(rows, G, threads, 2);
   const size_t smem = (size_t)3 * E * threads * sizeof(float);
   auto kernel = GN_KERNELS(gated_norm_backward_kernel);
   // 48 KiB and more of dynamic shared memory has to be asked for (the static part counts too)

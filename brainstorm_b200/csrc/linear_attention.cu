@@ -1,9 +1,10 @@
-// Decayed linear attention, recurrent form: the state of one (sequence, head) stays in the registers of
-// one block while the tokens pass by.  Serves single tokens (the step of a model that answers) and short
-// sequences.
+// Decayed linear attention, recurrent form: 32 columns of the state of one (sequence, head) stay in the
+// registers of one block while the tokens pass by.  Columns of the state never meet, so blocks are
+// independent.  Serves single tokens (the step of a model that answers) and short sequences.
 //
 // Bound for a single token: HBM, the state is read once and written once (8 dk dv bytes) and everything
-// else is small.  For several tokens: latency, two block barriers for each token.
+// else is small; the state, k, q and v are all asked for at once, and a block of 128 threads with up to 8
+// 128-bit loads each leaves room for many blocks on an SM.  For several tokens: latency, one barrier each.
 #include <algorithm>
 
 #include "linear_attention.cuh"
@@ -14,107 +15,96 @@ struct LaRuns {
   LaRun run[3];
 };
 
-// Thread (warp w, lane): column group cg = lane % CG of four columns, rows rl + RL * r, r < R, where
-// rl = w * (32 / CG) + lane / CG and RL = warps * 32 / CG.  VEC: the four columns lie side by side
-// (128-bit accesses); else they are CG apart (coalesced 32-bit ones).
+constexpr int LR_COLS = 32, LR_THREADS = 128;
+
+// Thread: four columns cg (of 8 groups), rows rl + 16 r, r < R.  VEC: the four columns lie side by side
+// (128-bit accesses); else they are 8 apart (coalesced 32-bit ones).
 template <int R, bool VEC>
-__global__ void __launch_bounds__(256) la_recurrent_kernel(LaCommon c, LaRuns runs, int CG) {
-  __shared__ float qkv[2][3 * LA_MAX_DIM];
-  __shared__ float part[8][LA_MAX_DIM];
-  const LaRun p = runs.run[blockIdx.y];
-  const int b = blockIdx.x / c.H, h = blockIdx.x % c.H;
+__global__ void __launch_bounds__(LR_THREADS, R == 8 ? 5 : 8) la_recurrent_kernel(LaCommon c, LaRuns runs, int max_slabs) {
+  __shared__ float part[2][4][LR_COLS];
+  const LaRun& p = runs.run[blockIdx.y];
+  const int bh = blockIdx.x / max_slabs, c0 = (blockIdx.x - bh * max_slabs) * LR_COLS;
+  const int dk = p.dk, dv = p.dv;
+  if (c0 >= dv) return;
+  const int b = bh / c.H, h = bh - b * c.H;
   const int n = la_length(c, b);
   const float l = c.decay[h];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int cg = lane % CG, rpw = 32 / CG, RL = warps * rpw, rl = w * rpw + lane / CG;
-  const int dk = p.dk, dv = p.dv;
-  const float* q = p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h;
-  const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h;
-  const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h;
+  const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t tok0 = p.reverse ? n - 1 : 0, dir = p.reverse ? -1 : 1;
+  const float* q = p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h + tok0 * p.qs.t;
+  const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h + tok0 * p.ks.t;
+  const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + tok0 * p.vs.t;
   float* o = p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h;
-  auto col = [&](int j) { return VEC ? 4 * cg + j : cg + CG * j; };
+  auto col = [&](int j) { return c0 + (VEC ? 4 * cg + j : cg + 8 * j); };
 
-  float S[R][4];
+  float S[R][4], kk[R], qq[R], vv[4];
+  const float* s_in = p.s_in ? p.s_in + (int64_t)bh * dk * dv : nullptr;
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; ++r) {
+    const int i = rl + 16 * r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) S[r][j] = 0.f;
-  if (p.s_in) {
-    const float* s = p.s_in + (int64_t)blockIdx.x * dk * dv;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int i = rl + RL * r;
-      if (i >= dk) continue;
-      if (VEC && !p.s_in_t) {
-        if (4 * cg < dv) {
-          const float4 x = *reinterpret_cast<const float4*>(s + (int64_t)i * dv + 4 * cg);
-          S[r][0] = x.x; S[r][1] = x.y; S[r][2] = x.z; S[r][3] = x.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col(j) < dv) S[r][j] = p.s_in_t ? s[(int64_t)col(j) * dk + i] : s[(int64_t)i * dv + col(j)];
+    if (!s_in || i >= dk) continue;
+    if (VEC && !p.s_in_t) {
+      if (col(0) < dv) {
+        const float4 x = *reinterpret_cast<const float4*>(s_in + (int64_t)i * dv + col(0));
+        S[r][0] = x.x; S[r][1] = x.y; S[r][2] = x.z; S[r][3] = x.w;
       }
-    }
-  }
-
-  auto fetch = [&](int step, float* dst) {
-    const int64_t t = p.reverse ? n - 1 - step : step;
-    for (int i = threadIdx.x; i < dk; i += blockDim.x) {
-      dst[i] = q[t * p.qs.t + i];
-      dst[LA_MAX_DIM + i] = k[t * p.ks.t + i] * p.k_scale;
-    }
-    for (int i = threadIdx.x; i < dv; i += blockDim.x) dst[2 * LA_MAX_DIM + i] = v[t * p.vs.t + i];
-  };
-  if (n > 0) fetch(0, qkv[0]);
-  for (int step = 0; step < n; ++step) {
-    __syncthreads();      // this step's token is in place, and the sums of the step before are read
-    const float* now = qkv[step & 1];
-    if (step + 1 < n) fetch(step + 1, qkv[(step + 1) & 1]);
-    const float f = (p.reverse && step == 0) ? 1.f : l;
-    float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) vv[j] = col(j) < dv ? now[2 * LA_MAX_DIM + col(j)] : 0.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int i = rl + RL * r;
-      if (i >= dk) continue;
-      const float kk = now[LA_MAX_DIM + i], qq = now[i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        S[r][j] = f * S[r][j] + kk * vv[j];
-        acc[j] += qq * S[r][j];
-      }
-    }
-    for (int m = CG; m < 32; m <<= 1)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], m);
-    if (lane < CG)
+    } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (col(j) < dv) part[w][col(j)] = acc[j];
-    __syncthreads();
-    const int64_t t = p.reverse ? n - 1 - step : step;
-    for (int i = threadIdx.x; i < dv; i += blockDim.x) {
-      float s = 0.f;
-      for (int u = 0; u < warps; ++u) s += part[u][i];
-      float* dst = o + t * p.os.t + i;
-      *dst = p.accumulate ? *dst + p.o_scale * s : p.o_scale * s;
+        if (col(j) < dv) S[r][j] = p.s_in_t ? s_in[(int64_t)col(j) * dk + i] : s_in[(int64_t)i * dv + col(j)];
     }
   }
-  if (!p.accumulate)       // tokens behind the end of the sequence
-    for (int64_t t = n; t < c.T; ++t)
-      for (int i = threadIdx.x; i < dv; i += blockDim.x) o[t * p.os.t + i] = 0.f;
+  auto fetch = [&](int step) {
+    const float *qt = q + dir * step * p.qs.t, *kt = k + dir * step * p.ks.t, *vt = v + dir * step * p.vs.t;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = rl + 16 * r;
+      qq[r] = i < dk ? qt[i] : 0.f;
+      kk[r] = i < dk ? kt[i] * p.k_scale : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = col(j) < dv ? vt[col(j)] : 0.f;
+  };
+  if (n > 0) fetch(0);
+  for (int step = 0; step < n; ++step) {
+    const float f = (p.reverse && step == 0) ? 1.f : l;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        S[r][j] = f * S[r][j] + kk[r] * vv[j];
+        acc[j] += qq[r] * S[r][j];
+      }
+    if (step + 1 < n) fetch(step + 1);
+#pragma unroll
+    for (int m = 8; m < 32; m <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], m);
+    if (lane < 8)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[step & 1][w][col(j) - c0] = acc[j];
+    __syncthreads();      // the sums of this step are in place; those of the step before have been read
+    if (threadIdx.x < LR_COLS && c0 + (int)threadIdx.x < dv) {
+      const float(*s)[LR_COLS] = part[step & 1];
+      const float x = p.o_scale * ((s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]));
+      float* dst = o + (tok0 + dir * step) * p.os.t + c0 + threadIdx.x;
+      *dst = p.accumulate ? *dst + x : x;
+    }
+  }
+  if (!p.accumulate && threadIdx.x < LR_COLS && c0 + (int)threadIdx.x < dv)      // tokens behind the end of the sequence
+    for (int64_t t = n; t < c.T; ++t) o[t * p.os.t + c0 + threadIdx.x] = 0.f;
   if (p.s_out) {
-    float* s = p.s_out + (int64_t)blockIdx.x * dk * dv;
+    float* s = p.s_out + (int64_t)bh * dk * dv;
     const float f = (p.reverse && n > 0) ? l : 1.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int i = rl + RL * r;
+      const int i = rl + 16 * r;
       if (i >= dk) continue;
       if (VEC) {
-        if (4 * cg < dv)
-          *reinterpret_cast<float4*>(s + (int64_t)i * dv + 4 * cg) = make_float4(f * S[r][0], f * S[r][1], f * S[r][2], f * S[r][3]);
+        if (col(0) < dv) *reinterpret_cast<float4*>(s + (int64_t)i * dv + col(0)) = make_float4(f * S[r][0], f * S[r][1], f * S[r][2], f * S[r][3]);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -124,7 +114,7 @@ __global__ void __launch_bounds__(256) la_recurrent_kernel(LaCommon c, LaRuns ru
   }
 }
 
-// One launch for up to three runs over the same sequences (the extents of the widest decide the block).
+// One launch for up to three runs over the same sequences.
 int la_recurrent(const LaCommon& c, const LaRun* runs, int count) {
   LaRuns all = {};
   int dk = 0, dv = 0;
@@ -135,17 +125,13 @@ int la_recurrent(const LaCommon& c, const LaRun* runs, int count) {
     dv = std::max(dv, runs[i].dv);
     vec = vec && runs[i].dv % 4 == 0 && aligned16(runs[i].s_in) && aligned16(runs[i].s_out);
   }
-  const int cg = dv <= 32 ? 8 : dv <= 64 ? 16 : 32, rpw = 32 / cg;
-  const int warps = (int)std::min<int64_t>(8, ceil_div(dk, rpw * 4));
-  const int rows = (int)ceil_div(dk, warps * rpw);      // per thread
-  const dim3 grid((unsigned)((int64_t)c.B * c.H), (unsigned)count);
-  const cudaStream_t st = state().stream;
-  if (rows <= 4 && vec) la_recurrent_kernel<4, true><<<grid, warps * 32, 0, st>>>(c, all, cg);
-  else if (rows <= 4) la_recurrent_kernel<4, false><<<grid, warps * 32, 0, st>>>(c, all, cg);
-  else if (rows <= 8 && vec) la_recurrent_kernel<8, true><<<grid, warps * 32, 0, st>>>(c, all, cg);
-  else if (rows <= 8) la_recurrent_kernel<8, false><<<grid, warps * 32, 0, st>>>(c, all, cg);
-  else if (vec) la_recurrent_kernel<16, true><<<grid, warps * 32, 0, st>>>(c, all, cg);
-  else la_recurrent_kernel<16, false><<<grid, warps * 32, 0, st>>>(c, all, cg);
+  const int slabs = (int)ceil_div(dv, LR_COLS);
+  B200_REQUIRE((int64_t)c.B * c.H * slabs < (1ll << 31), "linear attention: extent too large");
+  const dim3 grid((unsigned)((int64_t)c.B * c.H * slabs), (unsigned)count);
+  auto kernel = dk <= 32 ? (vec ? la_recurrent_kernel<2, true> : la_recurrent_kernel<2, false>)
+                : dk <= 64 ? (vec ? la_recurrent_kernel<4, true> : la_recurrent_kernel<4, false>)
+                           : (vec ? la_recurrent_kernel<8, true> : la_recurrent_kernel<8, false>);
+  kernel<<<grid, LR_THREADS, 0, state().stream>>>(c, all, slabs);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }

@@ -47,6 +47,14 @@ __device__ __forceinline__ int la_length(const LaCommon& c, int b) {
   return !(f >= 1.f) ? 0 : f >= (float)c.T ? c.T : (int)f;
 }
 
+// l^e, e >= 0, by squarings in 64 bits
+__device__ __forceinline__ double la_power(double l, int e) {
+  double f = 1.;
+  for (; e > 0; e >>= 1, l *= l)
+    if (e & 1) f *= l;
+  return f;
+}
+
 int la_recurrent(const LaCommon& c, const LaRun* runs, int count);                      // linear_attention.cu
 int la_chunked(const LaCommon& c, const LaRun* runs, int count, float* work);           // linear_attention_chunks.cu
 int64_t la_chunked_work(int64_t T, int64_t BH, int dk, int dv, bool backward);          // floats

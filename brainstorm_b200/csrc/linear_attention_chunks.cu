@@ -62,12 +62,22 @@ __device__ __forceinline__ void lc_mma3(float (&c)[4], const uint32_t (&ah)[4], 
   lc_mma(c, ah, bh0, bh1);
 }
 __device__ __forceinline__ uint32_t lc_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// two values as (hi, hi) and (lo, lo)
+// two values as (hi, hi) and (lo, lo): lo = fp16(x - hi), the difference in one mixed-precision operation
 __device__ __forceinline__ void lc_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = lc_bits(h);
-  lo = lc_bits(__floats2half2_rn(x - f.x, y - f.y));
+  asm("{\n\t.reg .f32 r0, r1;\n\t.reg .b16 h0, h1, m;\n\t"
+      "cvt.rn.f16x2.f32 %0, %3, %2;\n\t"
+      "mov.b32 {h0, h1}, %0;\n\t"
+      "mov.b16 m, 0xBC00;\n\t"                       // -1
+      "fma.rn.f32.f16 r0, h0, m, %2;\n\t"
+      "fma.rn.f32.f16 r1, h1, m, %3;\n\t"
+      "cvt.rn.f16x2.f32 %1, r1, r0;\n\t}"
+      : "=&r"(hi), "=r"(lo)
+      : "f"(x), "f"(y));
+}
+// (hi + lo) of two values
+__device__ __forceinline__ float2 lc_join(uint32_t hi, uint32_t lo) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi)), b = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+  return make_float2(a.x + b.x, a.y + b.y);
 }
 // |x|, 0 for a value that is not finite (which must not decide a scale)
 __device__ __forceinline__ float lc_size(float x) {
@@ -91,9 +101,29 @@ __device__ __forceinline__ float4 lc_row4(const float* row, int c, int d) {
   if (VEC) return c < d ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
   return make_float4(c < d ? row[c] : 0.f, c + 1 < d ? row[c + 1] : 0.f, c + 2 < d ? row[c + 2] : 0.f, c + 3 < d ? row[c + 3] : 0.f);
 }
+// Largest magnitude; FINITE leaves out what is not finite (a NaN is never taken).
+template <bool FINITE>
 __device__ __forceinline__ float lc_max4(float m, float4 x) {
-  return fmaxf(m, fmaxf(fmaxf(lc_size(x.x), lc_size(x.y)), fmaxf(lc_size(x.z), lc_size(x.w))));
+  if (FINITE) return fmaxf(m, fmaxf(fmaxf(lc_size(x.x), lc_size(x.y)), fmaxf(lc_size(x.z), lc_size(x.w))));
+  return fmaxf(fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
 }
+template <bool FINITE, int N>
+__device__ __forceinline__ float lc_max(const float4 (&x)[N]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = lc_max4<FINITE>(m, x[i]);
+  return m;
+}
+template <bool FINITE, int M>
+__device__ __forceinline__ float lc_max(const float (&x)[M][8][4]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = lc_max4<FINITE>(m, make_float4(x[i][j][0], x[i][j][1], x[i][j][2], x[i][j][3]));
+  return m;
+}
+#define LC_INF __int_as_float(0x7f800000)
 __device__ __forceinline__ void lc_put4(uint8_t* hi, uint8_t* lo, int row, int c, int pitch, float4 x, float s) {
   uint32_t h0, l0, h1, l1;
   lc_split(x.x * s, x.y * s, h0, l0);
@@ -105,7 +135,7 @@ __device__ __forceinline__ void lc_put4(uint8_t* hi, uint8_t* lo, int row, int c
 
 template <int DK>
 struct LcSmem {
-  static constexpr int KP = DK * 2, VP = LC_COLS * 2;      // row pitch in bytes
+  static constexpr int KP = DK * 2, VP = LC_COLS * 2;      // row pitch in bytes; hi and lo parts of q, k, v and the state
   static constexpr int Q_HI = 0, Q_LO = LC * KP, K_HI = 2 * LC * KP, K_LO = 3 * LC * KP, V_HI = 4 * LC * KP, V_LO = V_HI + LC * VP,
                        S_HI = V_LO + LC * VP, S_LO = S_HI + DK * VP, BYTES = S_LO + DK * VP;
 };
@@ -117,9 +147,10 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
   constexpr int MT = DK / 64;                        // 16-row tiles of the state in a warp
   constexpr int LPR = DK / 4, RPP = LC_THREADS / LPR;   // lanes per row of k, rows in a pass
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ float pw[LC + 1];                       // powers of the decay
+  __shared__ float pw_pad[16 + LC + 1];              // powers of the decay, zeros before
   __shared__ float q_inv[LC];                        // 1 / scale of each row of q
   __shared__ float red[3][4];
+  const float* pw = pw_pad + 16;
 
   const LaChunkRun& cr = runs.run[blockIdx.y];
   const LaRun& p = cr.r;
@@ -143,12 +174,16 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
   const float l = c.decay[h];
   const int64_t states = (int64_t)dk * p.dv;
 
-  const float* q = STATE_ONLY ? nullptr : p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h;
-  const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h;
-  const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + v0;
-  float* o = STATE_ONLY ? nullptr : p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h + v0;
+  // step s of the walk is token s, or n_all - 1 - s: a start and a signed pitch
+  const int64_t tok0 = p.reverse ? n_all - 1 : 0;
+  const int64_t q_t = p.reverse ? -p.qs.t : p.qs.t, k_t = p.reverse ? -p.ks.t : p.ks.t, v_t = p.reverse ? -p.vs.t : p.vs.t,
+                o_t = p.reverse ? -p.os.t : p.os.t;
+  const float* q = STATE_ONLY ? nullptr : p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h + tok0 * p.qs.t;
+  const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h + tok0 * p.ks.t;
+  const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + v0 + tok0 * p.vs.t;
+  float* o_base = STATE_ONLY ? nullptr : p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h + v0;
 
-  if (tid <= LC) pw[tid] = tid == 0 ? 1.f : (float)pow((double)l, (double)tid);
+  if (tid < 16 + LC + 1) pw_pad[tid] = tid < 16 ? 0.f : (float)la_power(l, tid - 16);
 
   // state: 16-row tiles w and w + 4 (rows 16 (w + 4 m) + g and + 8), columns 8 nt + t2, t2 + 1
   float S[MT][8][4];
@@ -162,8 +197,8 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
   auto col_of = [&](int nt, int e) { return 8 * nt + t2 + (e & 1); };
   if (!STATE_ONLY) {
     const float* s0 = segments > 1 ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : p.s_in ? p.s_in + bh * states : nullptr;
-    const int tr = segments > 1 ? cr.work_t : p.s_in_t;
-    if (s0)
+    const bool tr = segments > 1 ? cr.work_t : p.s_in_t;
+    if (s0 && tr) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -171,52 +206,71 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int i = row_of(m, e), j = col_of(nt, e);
-            if (i < dk && j < dv) S[m][nt][e] = tr ? s0[(int64_t)(v0 + j) * dk + i] : s0[(int64_t)i * p.dv + v0 + j];
+            if (i < dk && j < dv) S[m][nt][e] = s0[(int64_t)(v0 + j) * dk + i];
           }
-  }
-  bool undecayed = !STATE_ONLY && p.reverse && seg == 0;          // the incoming state counts in full at the first token
-
-  for (int64_t c0 = first; c0 < n_end; c0 += LC) {
-    const int n = (int)min((int64_t)LC, n_end - c0);
-    auto token = [&](int i) { return p.reverse ? n_all - 1 - (c0 + i) : c0 + i; };
-    // ---- load k and v, the scales of k, v and the state
-    float4 kr[LC / RPP], vr[8];
-    float mk = 0.f, mv = 0.f, ms = 0.f;
-    const int kc = (tid % LPR) * 4, vc = (tid & 15) * 4;
-#pragma unroll
-    for (int it = 0; it < LC / RPP; ++it) {
-      const int i = it * RPP + tid / LPR;
-      kr[it] = i < n ? lc_row4<VEC>(k + token(i) * p.ks.t, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int i = it * 8 + (tid >> 4);
-      vr[it] = i < n ? lc_row4<VEC>(v + token(i) * p.vs.t, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int it = 0; it < LC / RPP; ++it) mk = lc_max4(mk, kr[it]);
-#pragma unroll
-    for (int it = 0; it < 8; ++it) mv = lc_max4(mv, vr[it]);
-    if (!STATE_ONLY)
+    } else if (s0) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) ms = fmaxf(ms, lc_size(S[m][nt][e]));
-    mk = warp_max(mk);
-    mv = warp_max(mv);
-    if (!STATE_ONLY) ms = warp_max(ms);
-    if (lane == 0) {
-      red[0][w] = mk;
-      red[1][w] = mv;
-      red[2][w] = ms;
+          for (int e = 0; e < 4; e += 2) {
+            const int i = row_of(m, e), j = col_of(nt, e);
+            const float* at = s0 + (int64_t)i * p.dv + v0 + j;
+            if (VEC) {
+              if (i < dk && j < dv) {
+                const float2 x = *reinterpret_cast<const float2*>(at);
+                S[m][nt][e] = x.x;
+                S[m][nt][e + 1] = x.y;
+              }
+            } else {
+              if (i < dk && j < dv) S[m][nt][e] = at[0];
+              if (i < dk && j + 1 < dv) S[m][nt][e + 1] = at[1];
+            }
+          }
     }
+  }
+  bool undecayed = !STATE_ONLY && p.reverse && seg == 0;          // the incoming state counts in full at the first token
+
+  for (int64_t c0 = first; c0 < n_end; c0 += LC) {
+    const int n = (int)min((int64_t)LC, n_end - c0);
+    // ---- load k and v, the scales of k, v and the state
+    float4 kr[LC / RPP], vr[8];
+    const int kc = (tid % LPR) * 4, vc = (tid & 15) * 4;
+    {
+      const float* kp = k + (c0 + tid / LPR) * k_t;
+      const float* vp = v + (c0 + (tid >> 4)) * v_t;
+#pragma unroll
+      for (int it = 0; it < LC / RPP; ++it, kp += RPP * k_t)
+        kr[it] = it * RPP + tid / LPR < n ? lc_row4<VEC>(kp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int it = 0; it < 8; ++it, vp += 8 * v_t)
+        vr[it] = it * 8 + (tid >> 4) < n ? lc_row4<VEC>(vp, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    auto publish = [&](float mk, float mv, float ms) {
+      mk = warp_max(mk);
+      mv = warp_max(mv);
+      if (!STATE_ONLY) ms = warp_max(ms);
+      if (lane == 0) {
+        red[0][w] = mk;
+        red[1][w] = mv;
+        red[2][w] = ms;
+      }
+    };
+    auto largest = [&](int i) { return fmaxf(fmaxf(red[i][0], red[i][1]), fmaxf(red[i][2], red[i][3])); };
+    publish(lc_max<false>(kr), lc_max<false>(vr), STATE_ONLY ? 0.f : lc_max<false>(S));
     __syncthreads();      // scales in place; every warp is done with the tiles of the chunk before
+    float mk = largest(0), mv = largest(1), ms = largest(2);
+    if (fmaxf(fmaxf(mk, mv), ms) == LC_INF) {                      // an infinity must not decide a scale
+      __syncthreads();
+      publish(lc_max<true>(kr), lc_max<true>(vr), STATE_ONLY ? 0.f : lc_max<true>(S));
+      __syncthreads();
+      mk = largest(0);
+      mv = largest(1);
+      ms = largest(2);
+    }
     float k_inv, v_inv, s_inv, w_inv = 1.f;
-    const float k_s = lc_scale(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])), &k_inv);
-    const float v_s = lc_scale(fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])), &v_inv);
-    const float s_s = lc_scale(fmaxf(fmaxf(red[2][0], red[2][1]), fmaxf(red[2][2], red[2][3])), &s_inv);
+    const float k_s = lc_scale(mk, &k_inv), v_s = lc_scale(mv, &v_inv), s_s = lc_scale(ms, &s_inv);
     // weights above one (a decay above one) are taken back below two
     float w_s = 1.f;
     const float w_max = fabsf(pw[n - 1]);
@@ -225,23 +279,21 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
       w_inv *= 0x1p13f;
     }
 #pragma unroll
-    for (int it = 0; it < LC / RPP; ++it) lc_put4(sm + L::K_HI, sm + L::K_LO, it * RPP + tid / LPR, kc, L::KP, kr[it], k_s);
-#pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const int i = it * 8 + (tid >> 4);
-      float f = v_s;
-      if (STATE_ONLY) f = i < n ? v_s * (pw[n - 1 - i] * w_s) : 0.f;
-      if (STATE_ONLY) lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, vc, L::KP, vr[it], f);
-      else lc_put4(sm + L::V_HI, sm + L::V_LO, i, vc, L::VP, vr[it], f);
+    for (int it = 0; it < LC / RPP; ++it) {
+      const int i = it * RPP + tid / LPR;
+      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], STATE_ONLY ? k_s * (i < n ? pw[n - 1 - i] * w_s : 0.f) : k_s);
     }
-    float acc_o[8][4];
+#pragma unroll
+    for (int it = 0; it < 8; ++it) lc_put4(sm + L::V_HI, sm + L::V_LO, it * 8 + (tid >> 4), vc, L::VP, vr[it], v_s);
     if (!STATE_ONLY) {
       // ---- q, scaled by row
+      const float* qp = q + (c0 + tid / LPR) * q_t;
 #pragma unroll 8
-      for (int it = 0; it < LC / RPP; ++it) {
+      for (int it = 0; it < LC / RPP; ++it, qp += RPP * q_t) {
         const int i = it * RPP + tid / LPR;
-        const float4 x = i < n ? lc_row4<VEC>(q + token(i) * p.qs.t, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float m = lc_max4(0.f, x), inv;
+        const float4 x = i < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float m = lc_max4<false>(0.f, x), inv;
+        if (__any_sync(0xffffffffu, m == LC_INF)) m = lc_max4<true>(0.f, x);
 #pragma unroll
         for (int s = 1; s < LPR; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
         const float sc = lc_scale(m, &inv);
@@ -263,124 +315,145 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
           }
     }
     __syncthreads();      // all tiles in place
-    if (!STATE_ONLY) {
-      const int i0 = 16 * w;                          // this warp's tokens
-      if (i0 < n) {
-        // ---- scores of the tokens up to this warp's, and q S, in one walk over dk
-        float P[8][4];
+    if (c0 + LC < n_end) {                              // the next chunk's rows on their way into L2
+      const int i = tid >> 1;
+      if (c0 + LC + i < n_end) {
+        for (int x = (tid & 1) * 32; x < dk; x += 64) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(k + (c0 + LC + i) * k_t + x));
+          if (!STATE_ONLY) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + (c0 + LC + i) * q_t + x));
+        }
+        if ((tid & 1) * 32 < dv) asm volatile("prefetch.global.L2 [%0];" ::"l"(v + (c0 + LC + i) * v_t + (tid & 1) * 32));
+      }
+    }
+    const int i0 = 16 * w;                            // this warp's tokens
+    if (!STATE_ONLY && i0 < n) {
+      // ---- scores of the tokens up to this warp's, and q S, in one walk over dk
+      float P[8][4], acc_o[8][4];
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) P[nt][e] = acc_o[nt][e] = 0.f;
+#pragma unroll 1
+      for (int ks = 0; ks < ks_n; ++ks) {
+        uint32_t qh[4], ql[4];
+        const uint32_t qa = lc_at(i0 + (lane & 15), 2 * ks + (lane >> 4), L::KP);
+        lc_ldmatrix(qh, lc_smem(sm + L::Q_HI) + qa);
+        lc_ldmatrix(ql, lc_smem(sm + L::Q_LO) + qa);
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+          if (jt <= w) {
+            uint32_t bh_[4], bl_[4];
+            const uint32_t ka = lc_at(16 * jt + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1), L::KP);
+            lc_ldmatrix(bh_, lc_smem(sm + L::K_HI) + ka);
+            lc_ldmatrix(bl_, lc_smem(sm + L::K_LO) + ka);
+            lc_mma3(P[2 * jt], qh, ql, bh_[0], bh_[1], bl_[0], bl_[1]);
+            lc_mma3(P[2 * jt + 1], qh, ql, bh_[2], bh_[3], bl_[2], bl_[3]);
+          }
+#pragma unroll
+        for (int vt = 0; vt < 4; ++vt)
+          if (2 * vt < nt_n) {
+            uint32_t bh_[4], bl_[4];
+            const uint32_t sa = lc_at(16 * ks + (lane & 15), 2 * vt + (lane >> 4), L::VP);
+            lc_ldmatrix_t(bh_, lc_smem(sm + L::S_HI) + sa);
+            lc_ldmatrix_t(bl_, lc_smem(sm + L::S_LO) + sa);
+            lc_mma3(acc_o[2 * vt], qh, ql, bh_[0], bh_[1], bl_[0], bl_[1]);
+            lc_mma3(acc_o[2 * vt + 1], qh, ql, bh_[2], bh_[3], bl_[2], bl_[3]);
+          }
+      }
+      // ---- weights and mask, then the scores' own scale for each row.  Element (nt, half, e) is apart by
+      // base - 8 (nt - half) - e tokens: the weight of half 1 is the one half 0 had a tile before.
+      const float* pb = pw + (i0 + g - t2);
+      float m0 = 0.f, m1 = 0.f, b0 = pb[8], b1 = pb[7];
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+        if (nt < 2 * w + 2) {
+          const float a0 = pb[-8 * nt], a1 = pb[-8 * nt - 1];
+          P[nt][0] *= a0;
+          P[nt][1] *= a1;
+          P[nt][2] *= b0;
+          P[nt][3] *= b1;
+          if (nt >= 2 * w) {                            // the tiles on the diagonal
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (g + (e >> 1) * 8 < 8 * (nt - 2 * w) + t2 + (e & 1)) P[nt][e] = 0.f;
+          }
+          m0 = fmaxf(m0, fmaxf(fabsf(P[nt][0]), fabsf(P[nt][1])));
+          m1 = fmaxf(m1, fmaxf(fabsf(P[nt][2]), fabsf(P[nt][3])));
+          b0 = a0;
+          b1 = a1;
+        }
+      if (__any_sync(0xffffffffu, fmaxf(m0, m1) == LC_INF)) {
+        m0 = m1 = 0.f;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
+          if (nt < 2 * w + 2) {
+            m0 = fmaxf(m0, fmaxf(lc_size(P[nt][0]), lc_size(P[nt][1])));
+            m1 = fmaxf(m1, fmaxf(lc_size(P[nt][2]), lc_size(P[nt][3])));
+          }
+      }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) P[nt][e] = acc_o[nt][e] = 0.f;
-#pragma unroll 2
-        for (int ks = 0; ks < ks_n; ++ks) {
-          uint32_t qh[4], ql[4];
-          const uint32_t qa = lc_at(i0 + (lane & 15), 2 * ks + (lane >> 4), L::KP);
-          lc_ldmatrix(qh, lc_smem(sm + L::Q_HI) + qa);
-          lc_ldmatrix(ql, lc_smem(sm + L::Q_LO) + qa);
+      for (int s = 1; s < 4; s <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, s));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, s));
+      }
+      float p_inv0, p_inv1;
+      const float p_s0 = lc_scale(m0, &p_inv0), p_s1 = lc_scale(m1, &p_inv1);
+      // ---- scores times v
+      float acc_p[8][4];
 #pragma unroll
-          for (int jt = 0; jt < 4; ++jt)
-            if (jt <= w) {
-              uint32_t bh_[4], bl_[4];
-              const uint32_t ka = lc_at(16 * jt + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1), L::KP);
-              lc_ldmatrix(bh_, lc_smem(sm + L::K_HI) + ka);
-              lc_ldmatrix(bl_, lc_smem(sm + L::K_LO) + ka);
-              lc_mma3(P[2 * jt], qh, ql, bh_[0], bh_[1], bl_[0], bl_[1]);
-              lc_mma3(P[2 * jt + 1], qh, ql, bh_[2], bh_[3], bl_[2], bl_[3]);
-            }
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc_p[nt][e] = 0.f;
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt)
+        if (jt <= w) {
+          uint32_t ah[4], al[4];
+          lc_split(P[2 * jt][0] * p_s0, P[2 * jt][1] * p_s0, ah[0], al[0]);
+          lc_split(P[2 * jt][2] * p_s1, P[2 * jt][3] * p_s1, ah[1], al[1]);
+          lc_split(P[2 * jt + 1][0] * p_s0, P[2 * jt + 1][1] * p_s0, ah[2], al[2]);
+          lc_split(P[2 * jt + 1][2] * p_s1, P[2 * jt + 1][3] * p_s1, ah[3], al[3]);
 #pragma unroll
           for (int vt = 0; vt < 4; ++vt)
             if (2 * vt < nt_n) {
               uint32_t bh_[4], bl_[4];
-              const uint32_t sa = lc_at(16 * ks + (lane & 15), 2 * vt + (lane >> 4), L::VP);
-              lc_ldmatrix_t(bh_, lc_smem(sm + L::S_HI) + sa);
-              lc_ldmatrix_t(bl_, lc_smem(sm + L::S_LO) + sa);
-              lc_mma3(acc_o[2 * vt], qh, ql, bh_[0], bh_[1], bl_[0], bl_[1]);
-              lc_mma3(acc_o[2 * vt + 1], qh, ql, bh_[2], bh_[3], bl_[2], bl_[3]);
+              const uint32_t va = lc_at(16 * jt + (lane & 15), 2 * vt + (lane >> 4), L::VP);
+              lc_ldmatrix_t(bh_, lc_smem(sm + L::V_HI) + va);
+              lc_ldmatrix_t(bl_, lc_smem(sm + L::V_LO) + va);
+              lc_mma3(acc_p[2 * vt], ah, al, bh_[0], bh_[1], bl_[0], bl_[1]);
+              lc_mma3(acc_p[2 * vt + 1], ah, al, bh_[2], bh_[3], bl_[2], bl_[3]);
             }
         }
-        // ---- weights and mask, then the scores' own scale for each row
-        float m0 = 0.f, m1 = 0.f;
+      // ---- out
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-          if (nt < 2 * w + 2) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int apart = i0 + g + (e >> 1) * 8 - col_of(nt, e);
-              P[nt][e] = apart >= 0 ? P[nt][e] * pw[apart < 0 ? 0 : apart] : 0.f;
-            }
-            m0 = fmaxf(m0, fmaxf(lc_size(P[nt][0]), lc_size(P[nt][1])));
-            m1 = fmaxf(m1, fmaxf(lc_size(P[nt][2]), lc_size(P[nt][3])));
-          }
-#pragma unroll
-        for (int s = 1; s < 4; s <<= 1) {
-          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, s));
-          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, s));
-        }
-        float p_inv0, p_inv1;
-        const float p_s0 = lc_scale(m0, &p_inv0), p_s1 = lc_scale(m1, &p_inv1);
-        // ---- scores times v
-        float acc_p[8][4];
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc_p[nt][e] = 0.f;
-#pragma unroll
-        for (int jt = 0; jt < 4; ++jt)
-          if (jt <= w) {
-            uint32_t ah[4], al[4];
-            lc_split(P[2 * jt][0] * p_s0, P[2 * jt][1] * p_s0, ah[0], al[0]);
-            lc_split(P[2 * jt][2] * p_s1, P[2 * jt][3] * p_s1, ah[1], al[1]);
-            lc_split(P[2 * jt + 1][0] * p_s0, P[2 * jt + 1][1] * p_s0, ah[2], al[2]);
-            lc_split(P[2 * jt + 1][2] * p_s1, P[2 * jt + 1][3] * p_s1, ah[3], al[3]);
-#pragma unroll
-            for (int vt = 0; vt < 4; ++vt)
-              if (2 * vt < nt_n) {
-                uint32_t bh_[4], bl_[4];
-                const uint32_t va = lc_at(16 * jt + (lane & 15), 2 * vt + (lane >> 4), L::VP);
-                lc_ldmatrix_t(bh_, lc_smem(sm + L::V_HI) + va);
-                lc_ldmatrix_t(bl_, lc_smem(sm + L::V_LO) + va);
-                lc_mma3(acc_p[2 * vt], ah, al, bh_[0], bh_[1], bl_[0], bl_[1]);
-                lc_mma3(acc_p[2 * vt + 1], ah, al, bh_[2], bh_[3], bl_[2], bl_[3]);
-              }
-          }
-        // ---- out
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int i = i0 + g + 8 * half;
-          if (i < n) {
-            const float qi = q_inv[i];
-            const float f_s = p.o_scale * pw[i + (undecayed ? 0 : 1)];
-            const float f_p = p.o_scale * p.k_scale;
-            const float p_inv = half ? p_inv1 : p_inv0;
-            float* row = o + token(i) * p.os.t;
+      for (int half = 0; half < 2; ++half) {
+        const int i = i0 + g + 8 * half;
+        if (i < n) {
+          const float qi = q_inv[i];
+          // the factors one after the other where their product could leave the range of float32
+          const float f_o0 = s_inv * qi, f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
+          const float f_p0 = (half ? p_inv1 : p_inv0) * v_inv, f_p1 = qi * k_inv * (p.o_scale * p.k_scale);
+          float* row = o_base + (tok0 * p.os.t + (c0 + i) * o_t);
+          if (VEC && !p.accumulate) {
 #pragma unroll
             for (int nt = 0; nt < 8; ++nt)
-              if (nt < nt_n)
+              if (8 * nt + t2 < dv)
+                *reinterpret_cast<float2*>(row + 8 * nt + t2) =
+                    make_float2(acc_o[nt][2 * half] * f_o0 * f_o1 + acc_p[nt][2 * half] * f_p0 * f_p1,
+                                acc_o[nt][2 * half + 1] * f_o0 * f_o1 + acc_p[nt][2 * half + 1] * f_p0 * f_p1);
+          } else {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int j = 8 * nt + t2 + e;
-                  const float x = acc_o[nt][2 * half + e] * s_inv * qi * f_s + acc_p[nt][2 * half + e] * p_inv * v_inv * (qi * k_inv) * f_p;
-                  if (j < dv) row[j] = p.accumulate ? row[j] + x : x;
-                }
+            for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int j = 8 * nt + t2 + e;
+                const float x = acc_o[nt][2 * half + e] * f_o0 * f_o1 + acc_p[nt][2 * half + e] * f_p0 * f_p1;
+                if (j < dv) row[j] = p.accumulate ? row[j] + x : x;
+              }
           }
         }
       }
-      // ---- v times its weights, over this warp's rows of q (which only this warp has read)
-      __syncwarp();
-#pragma unroll
-      for (int it = 0; it < 8; ++it) {
-        const int i = 16 * w + 2 * it + (lane >> 4), cc = (lane & 15) * 4;
-        const uint32_t at = lc_at(i, cc >> 3, L::VP) + ((cc & 4) << 1);
-        const uint2 hi = *reinterpret_cast<const uint2*>(sm + L::V_HI + at), lo = *reinterpret_cast<const uint2*>(sm + L::V_LO + at);
-        const float f = i < n ? pw[n - 1 - i] * w_s : 0.f;
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi.x)), a2 = __half22float2(*reinterpret_cast<const __half2*>(&lo.x));
-        const float2 d = __half22float2(*reinterpret_cast<const __half2*>(&hi.y)), d2 = __half22float2(*reinterpret_cast<const __half2*>(&lo.y));
-        lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, cc, L::KP, make_float4(a.x + a2.x, a.y + a2.y, d.x + d2.x, d.y + d2.y), f);
-      }
-      __syncthreads();    // weighted v in place; the state's tile has been read
     }
-    // ---- the state after the chunk
+    // ---- the state after the chunk; each element of k is met once here and takes its weight on the way
     const float keep = pw[n - (undecayed ? 1 : 0)];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -398,21 +471,34 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
             const uint32_t ka = lc_at(16 * kt + (lane & 7) + ((lane >> 4) << 3), (r0 >> 3) + ((lane >> 3) & 1), L::KP);
             lc_ldmatrix_t(ah, lc_smem(sm + L::K_HI) + ka);
             lc_ldmatrix_t(al, lc_smem(sm + L::K_LO) + ka);
+            if (!STATE_ONLY) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {             // tokens 16 kt + 8 e + t2 and the next
+                const int i = n - 1 - (16 * kt + 8 * e + t2);
+                const float x0 = (i >= 0 ? pw[i] : 0.f) * w_s, x1 = (i >= 1 ? pw[i - 1] : 0.f) * w_s;
+#pragma unroll
+                for (int r = 2 * e; r < 2 * e + 2; ++r) {
+                  const float2 x = lc_join(ah[r], al[r]);
+                  lc_split(x.x * x0, x.y * x1, ah[r], al[r]);
+                }
+              }
+            }
 #pragma unroll
             for (int vt = 0; vt < 4; ++vt)
               if (2 * vt < nt_n) {
                 uint32_t bh_[4], bl_[4];
-                const uint32_t va = lc_at(16 * kt + (lane & 15), 2 * vt + (lane >> 4), L::KP);
-                lc_ldmatrix_t(bh_, lc_smem(sm + L::Q_HI) + va);
-                lc_ldmatrix_t(bl_, lc_smem(sm + L::Q_LO) + va);
+                const uint32_t va = lc_at(16 * kt + (lane & 15), 2 * vt + (lane >> 4), L::VP);
+                lc_ldmatrix_t(bh_, lc_smem(sm + L::V_HI) + va);
+                lc_ldmatrix_t(bl_, lc_smem(sm + L::V_LO) + va);
                 lc_mma3(acc[2 * vt], ah, al, bh_[0], bh_[1], bl_[0], bl_[1]);
                 lc_mma3(acc[2 * vt + 1], ah, al, bh_[2], bh_[3], bl_[2], bl_[3]);
               }
           }
+        const float f0 = k_inv * w_inv, f1 = v_inv * p.k_scale;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) S[m][nt][e] = keep * S[m][nt][e] + acc[nt][e] * (k_inv * w_inv) * v_inv * p.k_scale;
+          for (int e = 0; e < 4; ++e) S[m][nt][e] = keep * S[m][nt][e] + acc[nt][e] * f0 * f1;
       }
     }
     undecayed = false;
@@ -420,7 +506,7 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
 
   if (!STATE_ONLY && !p.accumulate)       // tokens behind the end of the sequence
     for (int64_t t = max((int64_t)n_all, first); t < limit; ++t)
-      for (int j = tid; j < dv; j += LC_THREADS) o[t * p.os.t + j] = 0.f;
+      for (int j = tid; j < dv; j += LC_THREADS) o_base[t * p.os.t + j] = 0.f;
   float* out = STATE_ONLY ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : segments == 1 && p.s_out ? p.s_out + bh * states : nullptr;
   if (out) {
     const float f = (!STATE_ONLY && p.reverse && n_all > 0) ? l : 1.f;
@@ -429,9 +515,15 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 4; e += 2) {
           const int i = row_of(m, e), j = col_of(nt, e);
-          if (i < dk && j < dv) out[(int64_t)i * p.dv + v0 + j] = f * S[m][nt][e];
+          float* at = out + (int64_t)i * p.dv + v0 + j;
+          if (VEC) {
+            if (i < dk && j < dv) *reinterpret_cast<float2*>(at) = make_float2(f * S[m][nt][e], f * S[m][nt][e + 1]);
+          } else {
+            if (i < dk && j < dv) at[0] = f * S[m][nt][e];
+            if (i < dk && j + 1 < dv) at[1] = f * S[m][nt][e + 1];
+          }
         }
   }
 }
@@ -448,30 +540,39 @@ __global__ void __launch_bounds__(256) la_segments_kernel(LaCommon c, LaChunkRun
   const double l = c.decay[h];
   float S = 0.f;
   if (p.s_in) S = p.s_in[bh * states + (p.s_in_t ? (e % p.dv) * p.dk + e / p.dv : e)];
-  const float full = (float)pow(l, (double)seg_tokens);
-  for (int s = 0; s < segments; ++s) {
-    float* at = cr.work + ((int64_t)s * c.B * c.H + bh) * states + e;
-    const float add = *at;
-    *at = S;
-    const int64_t left = (int64_t)n - (int64_t)s * seg_tokens;
-    const int count = (int)(left < 0 ? 0 : left < seg_tokens ? left : seg_tokens);
-    const int times = (p.reverse && s == 0 && count > 0) ? count - 1 : count;
-    const float f = times == 0 ? 1.f : times == seg_tokens ? full : (float)pow(l, (double)times);
-    if (count > 0) S = f * S + add;
+  const float full = (float)la_power(l, seg_tokens);
+  for (int s0 = 0; s0 < segments; s0 += 4) {
+    float add[4];
+    float* at = cr.work + ((int64_t)s0 * c.B * c.H + bh) * states + e;
+    const int64_t step = (int64_t)c.B * c.H * states;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) add[i] = s0 + i < segments ? at[i * step] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = s0 + i;
+      if (s >= segments) break;
+      at[i * step] = S;
+      const int64_t left = (int64_t)n - (int64_t)s * seg_tokens;
+      const int count = (int)(left < 0 ? 0 : left < seg_tokens ? left : seg_tokens);
+      const int times = (p.reverse && s == 0 && count > 0) ? count - 1 : count;
+      const float f = times == 0 ? 1.f : times == seg_tokens ? full : (float)la_power(l, times);
+      if (count > 0) S = f * S + add[i];
+    }
   }
   if (p.s_out) p.s_out[bh * states + e] = (p.reverse && n > 0) ? (float)l * S : S;
 }
 
 // Segments for `blocks` blocks of one segment: as many as use the resident blocks of the GPU best, where
-// every pass over a part costs its chunks and a state pass costs about half of that.
+// the main pass costs its chunks, the state pass 0.4 of that, and a segment's state about three chunks to
+// write, hand through and read.
 static int lc_segments(int64_t T, int64_t blocks, int resident) {
   const int64_t chunks = ceil_div(T, LC);
   int best = 1;
   double best_cost = (double)chunks * (double)ceil_div(blocks, resident);
   for (int s = 2; s <= 64 && 2 * s <= chunks; ++s) {
     const int64_t per = ceil_div(chunks, s);
-    const double cost = 1.5 * (double)per * (double)ceil_div(blocks * s, resident) + 2.0;
-    if (cost < 0.9 * best_cost) {
+    const double cost = (1.4 * (double)per + 3.0) * (double)ceil_div(blocks * s, resident);
+    if (cost < best_cost) {
       best = s;
       best_cost = cost;
     }
@@ -534,7 +635,8 @@ int la_chunked(const LaCommon& c, const LaRun* runs, int count, float* work) {
     for (const float* a : {runs[i].q, runs[i].k, runs[i].v}) vec = vec && aligned16(a);
     for (const LaStrides* s : {&runs[i].qs, &runs[i].ks, &runs[i].vs}) vec = vec && s->t % 4 == 0 && s->b % 4 == 0 && s->h % 4 == 0;
     // a slab starts at a multiple of 8 columns: aligned when the rows are
-    vec = vec && runs[i].dk % 4 == 0 && runs[i].dv % 4 == 0;
+    vec = vec && runs[i].dk % 4 == 0 && runs[i].dv % 4 == 0 && aligned16(runs[i].o) && aligned16(runs[i].s_in) && aligned16(runs[i].s_out) &&
+          runs[i].os.t % 4 == 0 && runs[i].os.b % 4 == 0 && runs[i].os.h % 4 == 0;
   }
   const LcPlan p = lc_plan(c.T, BH, lc_dk(runs, count), dv_max, count);
   B200_REQUIRE(BH <= 65535 || p.segments == 1, "linear attention: extent too large");
