@@ -134,6 +134,11 @@ __device__ __forceinline__ void gn_sum_into(float4* s, const float (&v)[E]) {
   }
 }
 
+// A row on its way into L2: its 128-byte lines are asked for by the row's threads.
+__device__ __forceinline__ void gn_prefetch(const float* row, int width, int G, int t) {
+  for (int c = 32 * t; c < width; c += 32 * G) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
+}
+
 // Sum over the G threads of a row, in a fixed order; valid in all of them.  All threads of the block
 // call it together.
 __device__ __forceinline__ float gn_row_sum(float v, int G, float* smem) {
@@ -237,6 +242,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
         gn_load<E, VEC>(y, p.y + row * p.ld_y, p.width, G, t);
         if (p.gate) gn_load<E, VEC>(g, p.gate + row * p.ld_gate, p.width, G, t);
         r_post = p.r_post[row];
+      }
+      const int64_t next = row + (int64_t)gridDim.x * per_block;
+      if (next < p.rows) {
+        if (p.dh) {
+          gn_prefetch(p.dh + next * p.ld_dh, p.width, G, t);
+          gn_prefetch(p.x_out + next * p.ld_x_out, p.width, G, t);
+        }
+        if (p.dx_out) gn_prefetch(p.dx_out + next * p.ld_dx_out, p.width, G, t);
+        if (p.y) gn_prefetch(p.y + next * p.ld_y, p.width, G, t);
+        if (p.gate) gn_prefetch(p.gate + next * p.ld_gate, p.width, G, t);
       }
     }
     if (p.dh) {

@@ -5,7 +5,10 @@
 // Bound for a single token: HBM, the state is read once and written once (8 dk dv bytes) and everything
 // else is small; the state, k, q and v are all asked for at once, and a block of 128 threads with up to 8
 // 128-bit loads each leaves room for many blocks on an SM.  For several tokens: latency, one barrier each.
+#include <string.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "linear_attention.cuh"
 
@@ -17,31 +20,32 @@ struct LaRuns {
 
 constexpr int LR_COLS = 32, LR_THREADS = 128;
 
-// Thread: four columns cg (of 8 groups), rows rl + 16 r, r < R.  VEC: the four columns lie side by side
-// (128-bit accesses); else they are 8 apart (coalesced 32-bit ones).
+// Thread: four columns cg (of 8 groups), rows R rl + r, r < R.  VEC: the four columns lie side by side, and all
+// accesses but those of the outputs are of 128 (R = 2: 64) bits; else the columns are 8 apart (coalesced 32-bit
+// accesses).
 template <int R, bool VEC>
 __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 5 : 8) la_recurrent_kernel(LaCommon c, LaRuns runs, int max_slabs) {
   __shared__ float part[2][4][LR_COLS];
   const LaRun& p = runs.run[blockIdx.y];
-  const int bh = blockIdx.x / max_slabs, c0 = (blockIdx.x - bh * max_slabs) * LR_COLS;
+  const unsigned bh = blockIdx.x / (unsigned)max_slabs;
+  const int c0 = (int)(blockIdx.x - bh * max_slabs) * LR_COLS;
   const int dk = p.dk, dv = p.dv;
   if (c0 >= dv) return;
-  const int b = bh / c.H, h = bh - b * c.H;
+  const int b = (int)(bh / (unsigned)c.H), h = (int)bh - b * c.H;
   const int n = la_length(c, b);
   const float l = c.decay[h];
   const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t tok0 = p.reverse ? n - 1 : 0, dir = p.reverse ? -1 : 1;
-  const float* q = p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h + tok0 * p.qs.t;
-  const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h + tok0 * p.ks.t;
-  const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + tok0 * p.vs.t;
-  float* o = p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h;
+  auto at = [&](const LaStrides& x) { return (int64_t)b * x.b + (int64_t)(x.div == 1 ? h : h / x.div) * x.h; };
+  const float *q = p.q + at(p.qs) + tok0 * p.qs.t, *k = p.k + at(p.ks) + tok0 * p.ks.t, *v = p.v + at(p.vs) + tok0 * p.vs.t;
+  float* o = p.o + at(p.os);
   auto col = [&](int j) { return c0 + (VEC ? 4 * cg + j : cg + 8 * j); };
 
   float S[R][4], kk[R], qq[R], vv[4];
   const float* s_in = p.s_in ? p.s_in + (int64_t)bh * dk * dv : nullptr;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int i = rl + 16 * r;
+    const int i = R * rl + r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) S[r][j] = 0.f;
     if (!s_in || i >= dk) continue;
@@ -58,14 +62,50 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 5 : 8) la_recurrent_kerne
   }
   auto fetch = [&](int step) {
     const float *qt = q + dir * step * p.qs.t, *kt = k + dir * step * p.ks.t, *vt = v + dir * step * p.vs.t;
+    const int i = R * rl;
+    if (VEC) {
+      using V = typename std::conditional<R == 2, float2, float4>::type;
+      constexpr int W = R == 2 ? 2 : 4;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int i = rl + 16 * r;
-      qq[r] = i < dk ? qt[i] : 0.f;
-      kk[r] = i < dk ? kt[i] * p.k_scale : 0.f;
+      for (int r = 0; r < R; r += W) {        // dk is a multiple of 4: a vector is inside or outside as a whole
+        V a = {}, x = {};
+        if (i + r < dk) {
+          a = *reinterpret_cast<const V*>(qt + i + r);
+          x = *reinterpret_cast<const V*>(kt + i + r);
+        }
+        memcpy(qq + r, &a, sizeof(V));
+        memcpy(kk + r, &x, sizeof(V));
+      }
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (col(0) < dv) x = *reinterpret_cast<const float4*>(vt + col(0));
+      memcpy(vv, &x, sizeof(x));
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        qq[r] = i + r < dk ? qt[i + r] : 0.f;
+        kk[r] = i + r < dk ? kt[i + r] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vv[j] = col(j) < dv ? vt[col(j)] : 0.f;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vv[j] = col(j) < dv ? vt[col(j)] : 0.f;
+    for (int j = 0; j < 4; ++j) vv[j] *= p.k_scale;
+  };
+  auto store_state = [&](float f) {
+    if (!p.s_out) return;
+    float* s = p.s_out + (int64_t)bh * dk * dv;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = R * rl + r;
+      if (i >= dk) continue;
+      if (VEC) {
+        if (col(0) < dv) *reinterpret_cast<float4*>(s + (int64_t)i * dv + col(0)) = make_float4(f * S[r][0], f * S[r][1], f * S[r][2], f * S[r][3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col(j) < dv) s[(int64_t)i * dv + col(j)] = f * S[r][j];
+      }
+    }
   };
   if (n > 0) fetch(0);
   for (int step = 0; step < n; ++step) {
@@ -79,6 +119,7 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 5 : 8) la_recurrent_kerne
         acc[j] += qq[r] * S[r][j];
       }
     if (step + 1 < n) fetch(step + 1);
+    else store_state(p.reverse ? l : 1.f);
 #pragma unroll
     for (int m = 8; m < 32; m <<= 1)
 #pragma unroll
@@ -96,22 +137,7 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 5 : 8) la_recurrent_kerne
   }
   if (!p.accumulate && threadIdx.x < LR_COLS && c0 + (int)threadIdx.x < dv)      // tokens behind the end of the sequence
     for (int64_t t = n; t < c.T; ++t) o[t * p.os.t + c0 + threadIdx.x] = 0.f;
-  if (p.s_out) {
-    float* s = p.s_out + (int64_t)bh * dk * dv;
-    const float f = (p.reverse && n > 0) ? l : 1.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int i = rl + 16 * r;
-      if (i >= dk) continue;
-      if (VEC) {
-        if (col(0) < dv) *reinterpret_cast<float4*>(s + (int64_t)i * dv + col(0)) = make_float4(f * S[r][0], f * S[r][1], f * S[r][2], f * S[r][3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col(j) < dv) s[(int64_t)i * dv + col(j)] = f * S[r][j];
-      }
-    }
-  }
+  if (n == 0) store_state(1.f);
 }
 
 // One launch for up to three runs over the same sequences.
@@ -123,7 +149,9 @@ int la_recurrent(const LaCommon& c, const LaRun* runs, int count) {
     all.run[i] = runs[i];
     dk = std::max(dk, runs[i].dk);
     dv = std::max(dv, runs[i].dv);
-    vec = vec && runs[i].dv % 4 == 0 && aligned16(runs[i].s_in) && aligned16(runs[i].s_out);
+    vec = vec && runs[i].dk % 4 == 0 && runs[i].dv % 4 == 0 && aligned16(runs[i].s_in) && aligned16(runs[i].s_out);
+    for (const float* a : {runs[i].q, runs[i].k, runs[i].v}) vec = vec && aligned16(a);
+    for (const LaStrides* x : {&runs[i].qs, &runs[i].ks, &runs[i].vs}) vec = vec && x->t % 4 == 0 && x->b % 4 == 0 && x->h % 4 == 0;
   }
   const int slabs = (int)ceil_div(dv, LR_COLS);
   B200_REQUIRE((int64_t)c.B * c.H * slabs < (1ll << 31), "linear attention: extent too large");

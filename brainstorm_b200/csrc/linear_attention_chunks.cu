@@ -4,9 +4,9 @@
 //
 //   o_i = sum_{j <= i} l^{i-j} (q_i . k_j) v_j + l^{i+1} q_i S        S' = l^n S + sum_j l^{n-1-j} k_j (x) v_j
 //
-// One block of four warps walks the chunks of one (sequence, head), or of a segment of them, for up to 64
-// columns of v, with the state in registers.  All four products run on mma.sync.m16n8k16 in fp32 accuracy:
-// every operand x is scaled by a power of two (per tile, per row for q and the scores) and split into two
+// One block of eight warps walks the chunks of one (sequence, head), or of a segment of them, for up to 64
+// columns of v: four warps for the outputs, four that keep the state in their registers.  All four products run on mma.sync.m16n8k16 in fp32 accuracy:
+// every operand x is scaled by a power of two (per tile, per row for the scores) and split into two
 // half-precision parts, hi = fp16(x), lo = fp16(x - hi), 22 bits together, and a product is hi.hi + hi.lo +
 // lo.hi.  A value more than 2^17 below the largest of its tile begins to lose bits (the error stays below
 // 2^-39 of that largest value).
@@ -31,7 +31,7 @@ namespace b200 {
 
 constexpr int LC = 64;                // tokens in a chunk
 constexpr int LC_COLS = 64;           // columns of v in a block
-constexpr int LC_THREADS = 128;
+constexpr int LC_THREADS = 256;
 
 struct LaChunkRun {
   LaRun r;
@@ -49,17 +49,44 @@ __device__ __forceinline__ void lc_ldmatrix(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void lc_ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
+// Not volatile: a function of registers, which the compiler may move between the loads.
 __device__ __forceinline__ void lc_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// c += (ah + al)(bh + bl) without al.bl; the small terms first
-__device__ __forceinline__ void lc_mma3(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t bh0, uint32_t bh1, uint32_t bl0,
-                                        uint32_t bl1) {
-  lc_mma(c, al, bh0, bh1);
-  lc_mma(c, ah, bl0, bl1);
-  lc_mma(c, ah, bh0, bh1);
+// Four 8-column tiles: c += (ah + al)(bh + bl) without al.bl, the small terms first.  Term by term, so that four
+// products lie between two that add to the same registers.
+__device__ __forceinline__ void lc_mma3(float (&c0)[4], float (&c1)[4], float (&c2)[4], float (&c3)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4],
+                                        const uint32_t (&bh)[8], const uint32_t (&bl)[8]) {
+  lc_mma(c0, al, bh[0], bh[1]);
+  lc_mma(c1, al, bh[2], bh[3]);
+  lc_mma(c2, al, bh[4], bh[5]);
+  lc_mma(c3, al, bh[6], bh[7]);
+  lc_mma(c0, ah, bl[0], bl[1]);
+  lc_mma(c1, ah, bl[2], bl[3]);
+  lc_mma(c2, ah, bl[4], bl[5]);
+  lc_mma(c3, ah, bl[6], bl[7]);
+  lc_mma(c0, ah, bh[0], bh[1]);
+  lc_mma(c1, ah, bh[2], bh[3]);
+  lc_mma(c2, ah, bh[4], bh[5]);
+  lc_mma(c3, ah, bh[6], bh[7]);
+}
+// c (16 x 64) += a (16 x 16) b, b the 16 rows from `row` of a tile of 64 columns, whose first nt_n 8-column tiles count
+__device__ __forceinline__ void lc_rows(float (&c)[8][4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t hi, uint32_t lo, int row, int lane,
+                                        int nt_n) {
+#pragma unroll
+  for (int vt = 0; vt < 4; vt += 2)
+    if (2 * vt < nt_n) {
+      uint32_t bh[8], bl[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t at = (uint32_t)((row + (lane & 15)) * 128 + (((2 * (vt + u) + (lane >> 4)) ^ (lane & 7)) << 4));
+        lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bh + 4 * u), hi + at);
+        lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bl + 4 * u), lo + at);
+      }
+      lc_mma3(c[2 * vt], c[2 * vt + 1], c[2 * vt + 2], c[2 * vt + 3], ah, al, bh, bl);
+    }
 }
 __device__ __forceinline__ uint32_t lc_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // two values as (hi, hi) and (lo, lo): lo = fp16(x - hi), the difference in one mixed-precision operation
@@ -123,6 +150,8 @@ __device__ __forceinline__ float lc_max(const float (&x)[M][8][4]) {
     for (int j = 0; j < 8; ++j) m = lc_max4<FINITE>(m, make_float4(x[i][j][0], x[i][j][1], x[i][j][2], x[i][j][3]));
   return m;
 }
+// All threads of the block, from whichever role's code.
+__device__ __forceinline__ void lc_barrier() { asm volatile("bar.sync 0, %0;" ::"n"(LC_THREADS) : "memory"); }
 #define LC_INF __int_as_float(0x7f800000)
 __device__ __forceinline__ void lc_put4(uint8_t* hi, uint8_t* lo, int row, int c, int pitch, float4 x, float s) {
   uint32_t h0, l0, h1, l1;
@@ -140,16 +169,17 @@ struct LcSmem {
                        S_HI = V_LO + LC * VP, S_LO = S_HI + DK * VP, BYTES = S_LO + DK * VP;
 };
 
-// DK: 64 or 128, the largest dk the block can hold.  VEC: 128-bit global loads.  STATE_ONLY: the state pass.
+// Warps 0 to 3 compute the outputs of 16 tokens each, warps 4 to 7 keep the state, in their registers; all eight
+// load and split the tiles.  DK: 64 or 128, the largest dk the block can hold.  VEC: 128-bit global loads.
+// STATE_ONLY: the state pass.
 template <int DK, bool VEC, bool STATE_ONLY>
-__global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs) {
+__global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs) {
   using L = LcSmem<DK>;
-  constexpr int MT = DK / 64;                        // 16-row tiles of the state in a warp
+  constexpr int MT = DK / 64;                        // 16-row tiles of the state in a state warp
   constexpr int LPR = DK / 4, RPP = LC_THREADS / LPR;   // lanes per row of k, rows in a pass
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ float pw_pad[16 + LC + 1];              // powers of the decay, zeros before
-  __shared__ float q_inv[LC];                        // 1 / scale of each row of q
-  __shared__ float red[3][4];
+  __shared__ float red[3][8];
   const float* pw = pw_pad + 16;
 
   const LaChunkRun& cr = runs.run[blockIdx.y];
@@ -170,7 +200,7 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
   const int v0 = slab * width, dv = min(width, p.dv - v0), dk = p.dk;
   const int nt_n = (dv + 7) >> 3;                                  // 8-column tiles in use
   const int ks_n = (dk + 15) >> 4;                                 // 16-deep steps over dk
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t2 = (lane & 3) * 2;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w = warp & 3, g = lane >> 2, t2 = (lane & 3) * 2;
   const float l = c.decay[h];
   const int64_t states = (int64_t)dk * p.dv;
 
@@ -185,148 +215,96 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
 
   if (tid < 16 + LC + 1) pw_pad[tid] = tid < 16 ? 0.f : (float)la_power(l, tid - 16);
 
-  // state: 16-row tiles w and w + 4 (rows 16 (w + 4 m) + g and + 8), columns 8 nt + t2, t2 + 1
-  float S[MT][8][4];
+  constexpr int KN = LC / RPP, VN = LC * 16 / LC_THREADS;          // passes over k and v
+  constexpr int QP = 128 / LPR, QN = LC / QP;                      // rows of q in a pass of the output warps, passes
+  const int kc = (tid % LPR) * 4, vc = (tid & 15) * 4;
+  auto load_kv = [&](float4 (&kr)[KN], float4 (&vr)[VN], int64_t c0, int n) {
+    const float* kp = k + (c0 + tid / LPR) * k_t;
+    const float* vp = v + (c0 + (tid >> 4)) * v_t;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int it = 0; it < KN; ++it, kp += RPP * k_t)
+      kr[it] = it * RPP + tid / LPR < n ? lc_row4<VEC>(kp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[m][nt][e] = 0.f;
-  auto row_of = [&](int m, int e) { return 16 * (w + 4 * m) + g + (e >> 1) * 8; };
-  auto col_of = [&](int nt, int e) { return 8 * nt + t2 + (e & 1); };
-  if (!STATE_ONLY) {
-    const float* s0 = segments > 1 ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : p.s_in ? p.s_in + bh * states : nullptr;
-    const bool tr = segments > 1 ? cr.work_t : p.s_in_t;
-    if (s0 && tr) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = row_of(m, e), j = col_of(nt, e);
-            if (i < dk && j < dv) S[m][nt][e] = s0[(int64_t)(v0 + j) * dk + i];
-          }
-    } else if (s0) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const int i = row_of(m, e), j = col_of(nt, e);
-            const float* at = s0 + (int64_t)i * p.dv + v0 + j;
-            if (VEC) {
-              if (i < dk && j < dv) {
-                const float2 x = *reinterpret_cast<const float2*>(at);
-                S[m][nt][e] = x.x;
-                S[m][nt][e + 1] = x.y;
-              }
-            } else {
-              if (i < dk && j < dv) S[m][nt][e] = at[0];
-              if (i < dk && j + 1 < dv) S[m][nt][e + 1] = at[1];
-            }
-          }
+    for (int it = 0; it < VN; ++it, vp += LC / VN * v_t)
+      vr[it] = it * (LC / VN) + (tid >> 4) < n ? lc_row4<VEC>(vp, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  // The largest magnitudes of the chunk's tiles and of the state; mx is this warp's of q (output warps) or of the state.
+  auto publish = [&](float mk, float mv, float mx) {
+    mk = warp_max(mk);
+    mv = warp_max(mv);
+    mx = warp_max(mx);
+    if (lane == 0) {
+      red[0][warp] = mk;
+      red[1][warp] = mv;
+      red[2][warp] = mx;
     }
-  }
-  bool undecayed = !STATE_ONLY && p.reverse && seg == 0;          // the incoming state counts in full at the first token
-
-  for (int64_t c0 = first; c0 < n_end; c0 += LC) {
-    const int n = (int)min((int64_t)LC, n_end - c0);
-    // ---- load k and v, the scales of k, v and the state
-    float4 kr[LC / RPP], vr[8];
-    const int kc = (tid % LPR) * 4, vc = (tid & 15) * 4;
-    {
-      const float* kp = k + (c0 + tid / LPR) * k_t;
-      const float* vp = v + (c0 + (tid >> 4)) * v_t;
-#pragma unroll
-      for (int it = 0; it < LC / RPP; ++it, kp += RPP * k_t)
-        kr[it] = it * RPP + tid / LPR < n ? lc_row4<VEC>(kp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int it = 0; it < 8; ++it, vp += 8 * v_t)
-        vr[it] = it * 8 + (tid >> 4) < n ? lc_row4<VEC>(vp, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    auto publish = [&](float mk, float mv, float ms) {
-      mk = warp_max(mk);
-      mv = warp_max(mv);
-      if (!STATE_ONLY) ms = warp_max(ms);
-      if (lane == 0) {
-        red[0][w] = mk;
-        red[1][w] = mv;
-        red[2][w] = ms;
-      }
-    };
-    auto largest = [&](int i) { return fmaxf(fmaxf(red[i][0], red[i][1]), fmaxf(red[i][2], red[i][3])); };
-    publish(lc_max<false>(kr), lc_max<false>(vr), STATE_ONLY ? 0.f : lc_max<false>(S));
-    __syncthreads();      // scales in place; every warp is done with the tiles of the chunk before
-    float mk = largest(0), mv = largest(1), ms = largest(2);
-    if (fmaxf(fmaxf(mk, mv), ms) == LC_INF) {                      // an infinity must not decide a scale
-      __syncthreads();
-      publish(lc_max<true>(kr), lc_max<true>(vr), STATE_ONLY ? 0.f : lc_max<true>(S));
-      __syncthreads();
-      mk = largest(0);
-      mv = largest(1);
-      ms = largest(2);
-    }
-    float k_inv, v_inv, s_inv, w_inv = 1.f;
-    const float k_s = lc_scale(mk, &k_inv), v_s = lc_scale(mv, &v_inv), s_s = lc_scale(ms, &s_inv);
-    // weights above one (a decay above one) are taken back below two
-    float w_s = 1.f;
-    const float w_max = fabsf(pw[n - 1]);
+    lc_barrier();
+  };
+  auto largest4 = [](const float* r) { return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])); };
+  struct Scales {
+    float k, v, q, s, w, k_inv, v_inv, q_inv, s_inv, w_inv;
+  };
+  auto collect = [&](Scales& x, int n) {       // false: an infinity must not decide a scale
+    const float mk = fmaxf(largest4(red[0]), largest4(red[0] + 4)), mv = fmaxf(largest4(red[1]), largest4(red[1] + 4));
+    const float mq = largest4(red[2]), ms = largest4(red[2] + 4);
+    if (fmaxf(fmaxf(mk, mv), fmaxf(mq, ms)) == LC_INF) return false;
+    x.k = lc_scale(mk, &x.k_inv);
+    x.v = lc_scale(mv, &x.v_inv);
+    x.q = lc_scale(mq, &x.q_inv);
+    x.s = lc_scale(ms, &x.s_inv);
+    x.w = x.w_inv = 1.f;
+    const float w_max = fabsf(pw[n - 1]);      // weights above one (a decay above one) are taken back below two
     if (w_max > 1.f) {
-      w_s = lc_scale(w_max, &w_inv) * 0x1p-13f;
-      w_inv *= 0x1p13f;
+      x.w = lc_scale(w_max, &x.w_inv) * 0x1p-13f;
+      x.w_inv *= 0x1p13f;
     }
+    return true;
+  };
+  auto put_kv = [&](const float4 (&kr)[KN], const float4 (&vr)[VN], const Scales& x, int n) {
 #pragma unroll
-    for (int it = 0; it < LC / RPP; ++it) {
+    for (int it = 0; it < KN; ++it) {
       const int i = it * RPP + tid / LPR;
-      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], STATE_ONLY ? k_s * (i < n ? pw[n - 1 - i] * w_s : 0.f) : k_s);
+      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], STATE_ONLY ? x.k * (i < n ? pw[n - 1 - i] * x.w : 0.f) : x.k);
     }
 #pragma unroll
-    for (int it = 0; it < 8; ++it) lc_put4(sm + L::V_HI, sm + L::V_LO, it * 8 + (tid >> 4), vc, L::VP, vr[it], v_s);
-    if (!STATE_ONLY) {
-      // ---- q, scaled by row
-      const float* qp = q + (c0 + tid / LPR) * q_t;
-#pragma unroll 8
-      for (int it = 0; it < LC / RPP; ++it, qp += RPP * q_t) {
-        const int i = it * RPP + tid / LPR;
-        const float4 x = i < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float m = lc_max4<false>(0.f, x), inv;
-        if (__any_sync(0xffffffffu, m == LC_INF)) m = lc_max4<true>(0.f, x);
+    for (int it = 0; it < VN; ++it) lc_put4(sm + L::V_HI, sm + L::V_LO, it * (LC / VN) + (tid >> 4), vc, L::VP, vr[it], x.v);
+  };
+  auto prefetch = [&](const float* a, int64_t pitch, int d, int64_t c0) {      // a tile of the next chunk on its way into L2
+    const int x = (tid & 1) * 32, i = (tid & 127) >> 1;
+    if (c0 + LC + i < n_end)
+      for (int e = x; e < d; e += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(a + (c0 + LC + i) * pitch + e));
+  };
+
+  if (warp < 4) {
+    // ================ outputs: warp w, tokens 16 w .. 16 w + 15 of the chunk ================
+    const int i0 = 16 * w;
+    bool undecayed = p.reverse && seg == 0;            // the incoming state counts in full at the first token
+    for (int64_t c0 = first; c0 < n_end; c0 += LC) {
+      const int n = (int)min((int64_t)LC, n_end - c0);
+      float4 kr[KN], vr[VN], qr[QN];
+      load_kv(kr, vr, c0, n);
+      if (!STATE_ONLY) {
+        const float* qp = q + (c0 + tid / LPR) * q_t;
 #pragma unroll
-        for (int s = 1; s < LPR; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-        const float sc = lc_scale(m, &inv);
-        lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, kc, L::KP, x, sc);
-        if (tid % LPR == 0) q_inv[i] = inv;
+        for (int it = 0; it < QN; ++it, qp += QP * q_t)
+          qr[it] = it * QP + tid / LPR < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      // ---- the state
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            uint32_t hi, lo;
-            lc_split(S[m][nt][e] * s_s, S[m][nt][e + 1] * s_s, hi, lo);
-            const uint32_t at = lc_at(row_of(m, e), nt, L::VP) + t2 * 2;
-            *reinterpret_cast<uint32_t*>(sm + L::S_HI + at) = hi;
-            *reinterpret_cast<uint32_t*>(sm + L::S_LO + at) = lo;
-          }
-    }
-    __syncthreads();      // all tiles in place
-    if (c0 + LC < n_end) {                              // the next chunk's rows on their way into L2
-      const int i = tid >> 1;
-      if (c0 + LC + i < n_end) {
-        for (int x = (tid & 1) * 32; x < dk; x += 64) {
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(k + (c0 + LC + i) * k_t + x));
-          if (!STATE_ONLY) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + (c0 + LC + i) * q_t + x));
-        }
-        if ((tid & 1) * 32 < dv) asm volatile("prefetch.global.L2 [%0];" ::"l"(v + (c0 + LC + i) * v_t + (tid & 1) * 32));
+      Scales x;
+      publish(lc_max<false>(kr), lc_max<false>(vr), STATE_ONLY ? 0.f : lc_max<false>(qr));      // the tiles of the chunk before are free
+      if (!collect(x, n)) {
+        lc_barrier();
+        publish(lc_max<true>(kr), lc_max<true>(vr), STATE_ONLY ? 0.f : lc_max<true>(qr));
+        collect(x, n);
       }
-    }
-    const int i0 = 16 * w;                            // this warp's tokens
-    if (!STATE_ONLY && i0 < n) {
+      put_kv(kr, vr, x, n);
+      if (!STATE_ONLY) {
+#pragma unroll
+        for (int it = 0; it < QN; ++it) lc_put4(sm + L::Q_HI, sm + L::Q_LO, it * QP + tid / LPR, kc, L::KP, qr[it], x.q);
+      }
+      lc_barrier();       // all tiles in place
+      if (STATE_ONLY) continue;
+      prefetch(q, q_t, dk, c0);
+      if (i0 >= n) continue;
       // ---- scores of the tokens up to this warp's, and q S, in one walk over dk
       float P[8][4], acc_o[8][4];
 #pragma unroll
@@ -340,25 +318,18 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
         lc_ldmatrix(qh, lc_smem(sm + L::Q_HI) + qa);
         lc_ldmatrix(ql, lc_smem(sm + L::Q_LO) + qa);
 #pragma unroll
-        for (int jt = 0; jt < 4; ++jt)
-          if (jt <= w) {
-            uint32_t bh_[4], bl_[4];
-            const uint32_t ka = lc_at(16 * jt + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1), L::KP);
-            lc_ldmatrix(bh_, lc_smem(sm + L::K_HI) + ka);
-            lc_ldmatrix(bl_, lc_smem(sm + L::K_LO) + ka);
-            lc_mma3(P[2 * jt], qh, ql, bh_[0], bh_[1], bl_[0], bl_[1]);
-            lc_mma3(P[2 * jt + 1], qh, ql, bh_[2], bh_[3], bl_[2], bl_[3]);
-          }
+        for (int jt = 0; jt < 4; jt += 2)
+          if (jt <= w) {                                // 32 tokens; their second half may be masked as a whole
+            uint32_t bh_[8], bl_[8];
 #pragma unroll
-        for (int vt = 0; vt < 4; ++vt)
-          if (2 * vt < nt_n) {
-            uint32_t bh_[4], bl_[4];
-            const uint32_t sa = lc_at(16 * ks + (lane & 15), 2 * vt + (lane >> 4), L::VP);
-            lc_ldmatrix_t(bh_, lc_smem(sm + L::S_HI) + sa);
-            lc_ldmatrix_t(bl_, lc_smem(sm + L::S_LO) + sa);
-            lc_mma3(acc_o[2 * vt], qh, ql, bh_[0], bh_[1], bl_[0], bl_[1]);
-            lc_mma3(acc_o[2 * vt + 1], qh, ql, bh_[2], bh_[3], bl_[2], bl_[3]);
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t ka = lc_at(16 * (jt + u) + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1), L::KP);
+              lc_ldmatrix(*reinterpret_cast<uint32_t(*)[4]>(bh_ + 4 * u), lc_smem(sm + L::K_HI) + ka);
+              lc_ldmatrix(*reinterpret_cast<uint32_t(*)[4]>(bl_ + 4 * u), lc_smem(sm + L::K_LO) + ka);
+            }
+            lc_mma3(P[2 * jt], P[2 * jt + 1], P[2 * jt + 2], P[2 * jt + 3], qh, ql, bh_, bl_);
           }
+        lc_rows(acc_o, qh, ql, lc_smem(sm + L::S_HI), lc_smem(sm + L::S_LO), 16 * ks, lane, nt_n);
       }
       // ---- weights and mask, then the scores' own scale for each row.  Element (nt, half, e) is apart by
       // base - 8 (nt - half) - e tokens: the weight of half 1 is the one half 0 had a tile before.
@@ -412,26 +383,16 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
           lc_split(P[2 * jt][2] * p_s1, P[2 * jt][3] * p_s1, ah[1], al[1]);
           lc_split(P[2 * jt + 1][0] * p_s0, P[2 * jt + 1][1] * p_s0, ah[2], al[2]);
           lc_split(P[2 * jt + 1][2] * p_s1, P[2 * jt + 1][3] * p_s1, ah[3], al[3]);
-#pragma unroll
-          for (int vt = 0; vt < 4; ++vt)
-            if (2 * vt < nt_n) {
-              uint32_t bh_[4], bl_[4];
-              const uint32_t va = lc_at(16 * jt + (lane & 15), 2 * vt + (lane >> 4), L::VP);
-              lc_ldmatrix_t(bh_, lc_smem(sm + L::V_HI) + va);
-              lc_ldmatrix_t(bl_, lc_smem(sm + L::V_LO) + va);
-              lc_mma3(acc_p[2 * vt], ah, al, bh_[0], bh_[1], bl_[0], bl_[1]);
-              lc_mma3(acc_p[2 * vt + 1], ah, al, bh_[2], bh_[3], bl_[2], bl_[3]);
-            }
+          lc_rows(acc_p, ah, al, lc_smem(sm + L::V_HI), lc_smem(sm + L::V_LO), 16 * jt, lane, nt_n);
         }
       // ---- out
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int i = i0 + g + 8 * half;
         if (i < n) {
-          const float qi = q_inv[i];
           // the factors one after the other where their product could leave the range of float32
-          const float f_o0 = s_inv * qi, f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
-          const float f_p0 = (half ? p_inv1 : p_inv0) * v_inv, f_p1 = qi * k_inv * (p.o_scale * p.k_scale);
+          const float f_o0 = x.s_inv * x.q_inv, f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
+          const float f_p0 = (half ? p_inv1 : p_inv0) * x.v_inv, f_p1 = x.q_inv * x.k_inv * (p.o_scale * p.k_scale);
           float* row = o_base + (tok0 * p.os.t + (c0 + i) * o_t);
           if (VEC && !p.accumulate) {
 #pragma unroll
@@ -452,8 +413,92 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
           }
         }
       }
+      undecayed = false;
     }
-    // ---- the state after the chunk; each element of k is met once here and takes its weight on the way
+    if (!STATE_ONLY && !p.accumulate)       // tokens behind the end of the sequence
+      for (int64_t t = max((int64_t)n_all, first); t < limit; ++t)
+        for (int j = tid; j < dv; j += 128) o_base[t * p.os.t + j] = 0.f;
+    return;
+  }
+
+  // ================ the state: warp w, 16-row tiles w and w + 4 (rows 16 (w + 4 m) + g and + 8), columns 8 nt + t2, t2 + 1 ================
+  auto row_of = [&](int m, int e) { return 16 * (w + 4 * m) + g + (e >> 1) * 8; };
+  auto col_of = [&](int nt, int e) { return 8 * nt + t2 + (e & 1); };
+  float S[MT][8][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[m][nt][e] = 0.f;
+  if (!STATE_ONLY) {
+    const float* s0 = segments > 1 ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : p.s_in ? p.s_in + bh * states : nullptr;
+    const bool tr = segments > 1 ? cr.work_t : p.s_in_t;
+    if (s0 && tr) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = row_of(m, e), j = col_of(nt, e);
+            if (i < dk && j < dv) S[m][nt][e] = s0[(int64_t)(v0 + j) * dk + i];
+          }
+    } else if (s0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const int i = row_of(m, e), j = col_of(nt, e);
+            const float* at = s0 + (int64_t)i * p.dv + v0 + j;
+            if (VEC) {
+              if (i < dk && j < dv) {
+                const float2 x = *reinterpret_cast<const float2*>(at);
+                S[m][nt][e] = x.x;
+                S[m][nt][e + 1] = x.y;
+              }
+            } else {
+              if (i < dk && j < dv) S[m][nt][e] = at[0];
+              if (i < dk && j + 1 < dv) S[m][nt][e + 1] = at[1];
+            }
+          }
+    }
+  }
+  bool undecayed = !STATE_ONLY && p.reverse && seg == 0;
+  for (int64_t c0 = first; c0 < n_end; c0 += LC) {
+    const int n = (int)min((int64_t)LC, n_end - c0);
+    Scales x;
+    {
+      float4 kr[KN], vr[VN];
+      load_kv(kr, vr, c0, n);
+      publish(lc_max<false>(kr), lc_max<false>(vr), STATE_ONLY ? 0.f : lc_max<false>(S));
+      if (!collect(x, n)) {
+        lc_barrier();
+        publish(lc_max<true>(kr), lc_max<true>(vr), STATE_ONLY ? 0.f : lc_max<true>(S));
+        collect(x, n);
+      }
+      put_kv(kr, vr, x, n);
+    }
+    if (!STATE_ONLY) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            uint32_t hi, lo;
+            lc_split(S[m][nt][e] * x.s, S[m][nt][e + 1] * x.s, hi, lo);
+            const uint32_t at = lc_at(row_of(m, e), nt, L::VP) + t2 * 2;
+            *reinterpret_cast<uint32_t*>(sm + L::S_HI + at) = hi;
+            *reinterpret_cast<uint32_t*>(sm + L::S_LO + at) = lo;
+          }
+    }
+    lc_barrier();         // all tiles in place
+    prefetch(k, k_t, dk, c0);
+    prefetch(v, v_t, dv, c0);
+    // each element of k is met once here and takes its weight on the way
     const float keep = pw[n - (undecayed ? 1 : 0)];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -475,38 +520,26 @@ __global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(
 #pragma unroll
               for (int e = 0; e < 2; ++e) {             // tokens 16 kt + 8 e + t2 and the next
                 const int i = n - 1 - (16 * kt + 8 * e + t2);
-                const float x0 = (i >= 0 ? pw[i] : 0.f) * w_s, x1 = (i >= 1 ? pw[i - 1] : 0.f) * w_s;
+                const float w0 = (i >= 0 ? pw[i] : 0.f) * x.w, w1 = (i >= 1 ? pw[i - 1] : 0.f) * x.w;
 #pragma unroll
                 for (int r = 2 * e; r < 2 * e + 2; ++r) {
-                  const float2 x = lc_join(ah[r], al[r]);
-                  lc_split(x.x * x0, x.y * x1, ah[r], al[r]);
+                  const float2 y = lc_join(ah[r], al[r]);
+                  lc_split(y.x * w0, y.y * w1, ah[r], al[r]);
                 }
               }
             }
-#pragma unroll
-            for (int vt = 0; vt < 4; ++vt)
-              if (2 * vt < nt_n) {
-                uint32_t bh_[4], bl_[4];
-                const uint32_t va = lc_at(16 * kt + (lane & 15), 2 * vt + (lane >> 4), L::VP);
-                lc_ldmatrix_t(bh_, lc_smem(sm + L::V_HI) + va);
-                lc_ldmatrix_t(bl_, lc_smem(sm + L::V_LO) + va);
-                lc_mma3(acc[2 * vt], ah, al, bh_[0], bh_[1], bl_[0], bl_[1]);
-                lc_mma3(acc[2 * vt + 1], ah, al, bh_[2], bh_[3], bl_[2], bl_[3]);
-              }
+            lc_rows(acc, ah, al, lc_smem(sm + L::V_HI), lc_smem(sm + L::V_LO), 16 * kt, lane, nt_n);
           }
-        const float f0 = k_inv * w_inv, f1 = v_inv * p.k_scale;
+        const float f0 = x.k_inv * x.w_inv, f1 = x.v_inv * p.k_scale;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) S[m][nt][e] = keep * S[m][nt][e] + acc[nt][e] * f0 * f1;
       }
     }
+
     undecayed = false;
   }
-
-  if (!STATE_ONLY && !p.accumulate)       // tokens behind the end of the sequence
-    for (int64_t t = max((int64_t)n_all, first); t < limit; ++t)
-      for (int j = tid; j < dv; j += LC_THREADS) o_base[t * p.os.t + j] = 0.f;
   float* out = STATE_ONLY ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : segments == 1 && p.s_out ? p.s_out + bh * states : nullptr;
   if (out) {
     const float f = (!STATE_ONLY && p.reverse && n_all > 0) ? l : 1.f;
@@ -591,7 +624,7 @@ static LcPlan lc_plan(int64_t T, int64_t BH, int dk, int dv_max, int count) {
   LcPlan p;
   p.dk = dk <= 64 ? 64 : 128;
   p.slabs = (int)ceil_div(dv_max, LC_COLS);
-  p.segments = lc_segments(T, BH * p.slabs * count, state().sm_count * (p.dk == 64 ? 3 : 2));
+  p.segments = lc_segments(T, BH * p.slabs * count, state().sm_count * 2);
   p.seg_tokens = (int)(ceil_div(ceil_div(T, LC), p.segments) * LC);
   p.segments = (int)ceil_div(T, p.seg_tokens);
   return p;
