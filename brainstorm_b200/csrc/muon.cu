@@ -9,12 +9,9 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "ns_gemm.cuh"
 
 namespace b200 {
-int gemm_tc(int transa, int transb, int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b, int64_t ldb, float* c,
-            int64_t ldc, int accumulate);
-int gemm_simt(int transa, int transb, int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b, int64_t ldb, float* c,
-              int64_t ldc, int accumulate);
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int MU_NORM_BLOCKS = 128;      // per matrix
@@ -55,70 +52,62 @@ __device__ __forceinline__ float muon_inverse_norm(const double* partial, int co
   return (float)(1. / (sqrt(t) + 1e-7));
 }
 
-// X = u / |u|, X^T when tall
+// X = u / |u| and its transpose, as planes.  Tiles of 32 x 32 through shared memory; block z: matrix.
+// straight receives u's own orientation, turned the transposed one.
 __global__ void __launch_bounds__(256) muon_start_kernel(const float* grad, const float* momentum, int rows, int cols, float beta, int nesterov,
-                                                         const double* partial, int partials, int tall, float* X) {
+                                                         const double* partial, int partials, NsMatrix straight, NsMatrix turned) {
   __shared__ double red[8];
   __shared__ float tile[32][33];
   const int64_t size = (int64_t)rows * cols;
   const float* g = grad + blockIdx.z * size;
   const float* m = momentum + blockIdx.z * size;
-  float* x = X + blockIdx.z * size;
-  const float inv = muon_inverse_norm(partial + blockIdx.z * partials, partials, red);
+  const float inv = NS_SCALE * muon_inverse_norm(partial + blockIdx.z * partials, partials, red);
   const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t plane = (int64_t)gridDim.z * straight.rows * straight.ld, plane_t = (int64_t)gridDim.z * turned.rows * turned.ld;
+  __half* s = straight.data + (int64_t)blockIdx.z * straight.rows * straight.ld;
+  __half* t = turned.data + (int64_t)blockIdx.z * turned.rows * turned.ld;
+  auto put = [](__half* at, int64_t plane, float x) {
+    const __half h = __float2half_rn(x);
+    at[0] = h;
+    at[plane] = __float2half_rn(x - __half2float(h));
+  };
+#pragma unroll
   for (int y = ty; y < 32; y += 8) {
     const int r = r0 + y, c = c0 + tx;
+    float x = 0.f;
     if (r < rows && c < cols) {
       const int64_t i = (int64_t)r * cols + c;
-      const float u = nesterov ? g[i] + beta * m[i] : m[i];
-      if (tall) tile[y][tx] = u * inv;
-      else x[i] = u * inv;
+      x = (nesterov ? g[i] + beta * m[i] : m[i]) * inv;
+      put(s + (int64_t)r * straight.ld + c, plane, x);
     }
+    tile[y][tx] = x;
   }
-  if (!tall) return;
   __syncthreads();
+#pragma unroll
   for (int y = ty; y < 32; y += 8) {
     const int c = c0 + y, r = r0 + tx;
-    if (r < rows && c < cols) x[(int64_t)c * rows + r] = tile[tx][y];
+    if (r < rows && c < cols) put(t + (int64_t)c * turned.ld + r, plane_t, tile[tx][y]);
   }
 }
 
-__global__ void __launch_bounds__(256) muon_combine_kernel(const float* a, const float* aa, float* out, int64_t n, float fa, float faa) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = fa * a[i] + faa * aa[i];
-}
-
-// update = X (or its transpose), p = keep * p - rate * X
-__global__ void __launch_bounds__(256) muon_apply_kernel(const float* X, float* update, float* param, int rows, int cols, int tall, float keep,
-                                                         float rate) {
-  __shared__ float tile[32][33];
-  const int64_t size = (int64_t)rows * cols;
-  const float* x = X + blockIdx.z * size;
-  float* u = update + blockIdx.z * size;
-  float* p = param + blockIdx.z * size;
-  const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  if (tall) {
-    for (int y = ty; y < 32; y += 8) {
-      const int c = c0 + y, r = r0 + tx;
-      if (r < rows && c < cols) tile[tx][y] = x[(int64_t)c * rows + r];
-    }
-    __syncthreads();
-  }
-  for (int y = ty; y < 32; y += 8) {
-    const int r = r0 + y, c = c0 + tx;
-    if (r < rows && c < cols) {
-      const int64_t i = (int64_t)r * cols + c;
-      const float v = tall ? tile[y][tx] : x[i];
-      u[i] = v;
-      p[i] = keep * p[i] - rate * v;
-    }
+// update = X, p = keep * p - rate * X, X in the parameters' own orientation
+__global__ void __launch_bounds__(256) muon_apply_kernel(NsMatrix X, float* update, float* param, float keep, float rate) {
+  const int64_t size = (int64_t)X.rows * X.cols, plane = (int64_t)gridDim.y * X.rows * X.ld;
+  const __half* x = X.data + (int64_t)blockIdx.y * X.rows * X.ld;
+  float* u = update + blockIdx.y * size;
+  float* p = param + blockIdx.y * size;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = X.ld == X.cols ? 0 : i / X.cols;
+    const int64_t at = i + r * (X.ld - X.cols);
+    const float v = (__half2float(x[at]) + __half2float(x[at + plane])) * (1.f / NS_SCALE);
+    u[i] = v;
+    p[i] = keep * p[i] - rate * v;
   }
 }
 
-static int muon_gemm(int transb, int64_t M, int64_t N, int64_t K, const float* a, const float* b, float* c) {
-  const int64_t ldb = transb ? K : N;
-  const int rc = gemm_tc(0, transb, M, N, K, a, K, b, ldb, c, N, 0);
-  return rc != B200_ERR_UNSUPPORTED ? rc : gemm_simt(0, transb, M, N, K, a, K, b, ldb, c, N, 0);
-}
+static int64_t muon_pitch(int64_t n) { return (n + 7) & ~(int64_t)7; }
+// Planes of a (rows, cols) stack, in floats, a multiple of 128 bytes.
+static int64_t muon_planes(int64_t batch, int64_t rows, int64_t cols) { return (batch * rows * muon_pitch(cols) + 31) & ~(int64_t)31; }
 
 }  // namespace b200
 
@@ -126,8 +115,8 @@ using namespace b200;
 
 B200_API int64_t b200_muon_scratch_floats(int64_t batch, int64_t rows, int64_t cols) {
   if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-  const int64_t m = std::min(rows, cols);
-  return 2 * batch * rows * cols + 3 * m * m + 2 * batch * MU_NORM_BLOCKS + 16;
+  const int64_t m = std::min(rows, cols), n = std::max(rows, cols);
+  return 2 * muon_planes(batch, m, n) + 2 * muon_planes(batch, n, m) + 2 * muon_planes(batch, m, m) + 2 * batch * MU_NORM_BLOCKS + 64;
 }
 
 B200_API int b200_muon_update(float* param, const float* grad, float* momentum, float* update, int64_t batch, int64_t rows, int64_t cols,
@@ -137,40 +126,37 @@ B200_API int b200_muon_update(float* param, const float* grad, float* momentum, 
   B200_REQUIRE(batch >= 0 && rows >= 0 && cols >= 0, "negative extent");
   B200_REQUIRE(steps >= 0 && steps <= 100, "muon: %d steps", steps);
   if (batch == 0 || rows == 0 || cols == 0) return B200_OK;
-  B200_REQUIRE(rows < (1 << 20) && cols < (1 << 20) && batch < 65536, "muon: extent too large");
+  B200_REQUIRE(rows < (1 << 20) && cols < (1 << 20) && batch < 32768, "muon: extent too large");
   B200_REQUIRE(param && grad && momentum && update && scratch, "muon: NULL operand");
-  B200_REQUIRE(scratch_floats >= b200_muon_scratch_floats(batch, rows, cols) && ((uintptr_t)scratch & 15) == 0, "muon: scratch too small");
+  B200_REQUIRE(scratch_floats >= b200_muon_scratch_floats(batch, rows, cols) && ((uintptr_t)scratch & 15) == 0, "muon: scratch too small or misaligned");
   const cudaStream_t st = state().stream;
-  const int tall = rows > cols;
+  const bool tall = rows > cols;
   const int64_t m = tall ? cols : rows, n = tall ? rows : cols, size = m * n;
-  double* partial = (double*)scratch;
-  float* X = scratch + 2 * ((batch * MU_NORM_BLOCKS + 1) & ~(int64_t)1);
-  float* Y = X + batch * size;
-  float* A = Y + batch * size;
-  float* AA = A + m * m;
+  float* at = (float*)(((uintptr_t)scratch + 127) & ~(uintptr_t)127);      // TMA wants 16 bytes, whole lines are better
+  auto planes = [&](int64_t r, int64_t c) {
+    NsMatrix x = {(__half*)at, (int)r, (int)c, (int)muon_pitch(c)};
+    at += muon_planes(batch, r, c);
+    return x;
+  };
+  NsMatrix X[2] = {planes(m, n), planes(m, n)}, Y[2] = {planes(n, m), planes(n, m)}, A = planes(m, m), B = planes(m, m);      // Y = X^T
+  double* partial = (double*)at;
   const unsigned nb = (unsigned)std::min<int64_t>(MU_NORM_BLOCKS, ceil_div(size, 1024));
   muon_momentum_kernel<<<dim3(nb, (unsigned)batch), 256, 0, st>>>(grad, momentum, size, beta, nesterov, partial);
   B200_LAUNCH_CHECK();
   const dim3 tiles((unsigned)ceil_div(cols, 32), (unsigned)ceil_div(rows, 32), (unsigned)batch);
-  muon_start_kernel<<<tiles, 256, 0, st>>>(grad, momentum, (int)rows, (int)cols, beta, nesterov, partial, (int)nb, tall, X);
+  muon_start_kernel<<<tiles, 256, 0, st>>>(grad, momentum, (int)rows, (int)cols, beta, nesterov, partial, (int)nb, tall ? Y[0] : X[0], tall ? X[0] : Y[0]);
   B200_LAUNCH_CHECK();
-  const unsigned eb = (unsigned)std::min<int64_t>(ceil_div(std::max(size, m * m), 256), (int64_t)state().sm_count * 8);
-  float *from = X, *to = Y;
-  for (int i = 0; i < steps; ++i) {
-    for (int64_t b = 0; b < batch; ++b) {
-      const float* x = from + b * size;
-      float* y = to + b * size;
-      if (int rc = muon_gemm(1, m, m, n, x, x, A)) return rc;
-      if (int rc = muon_gemm(0, m, m, m, A, A, AA)) return rc;
-      muon_combine_kernel<<<eb, 256, 0, st>>>(A, AA, A, m * m, NS_B, NS_C);
-      B200_LAUNCH_CHECK();
-      if (int rc = muon_gemm(0, m, n, m, A, x, y)) return rc;
-      muon_combine_kernel<<<eb, 256, 0, st>>>(x, y, y, size, NS_A, 1.f);
-      B200_LAUNCH_CHECK();
-    }
-    std::swap(from, to);
+  int now = 0;
+  for (int i = 0; i < steps; ++i, now ^= 1) {
+    const bool last = i == steps - 1;
+    if (int rc = ns_gemm(X[now], X[now], nullptr, &A, &A, (int)batch, 1.f, 0.f, true)) return rc;
+    if (int rc = ns_gemm(A, A, &A, &B, &B, (int)batch, NS_C, NS_B, true)) return rc;
+    // the last result is only needed as the parameters lie
+    if (int rc = ns_gemm(B, Y[now], &X[now], last && tall ? nullptr : &X[now ^ 1], last && !tall ? nullptr : &Y[now ^ 1], (int)batch, 1.f, NS_A, false))
+      return rc;
   }
-  muon_apply_kernel<<<tiles, 256, 0, st>>>(from, update, param, (int)rows, (int)cols, tall, 1.f - learning_rate * weight_decay, learning_rate);
+  const unsigned eb = (unsigned)std::min<int64_t>(ceil_div(size, 1024), (int64_t)state().sm_count * 8);
+  muon_apply_kernel<<<dim3(eb, (unsigned)batch), 256, 0, st>>>(tall ? Y[now] : X[now], update, param, 1.f - learning_rate * weight_decay, learning_rate);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
