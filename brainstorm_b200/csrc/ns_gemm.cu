@@ -1,21 +1,27 @@
-// out = alpha a b^T + beta add in fp32 accuracy on tcgen05.mma kind::f16, for operands that are already split
+// out = alpha a b^T + diagonal I in fp32 accuracy on tcgen05.mma kind::f16, for operands that are already split
 // into two half-precision planes (hi = fp16(x), lo = fp16(x - hi), 22 bits together): what the Newton-Schulz
-// iteration of muon.cu multiplies.  Its matrices stay below 3 in magnitude, so one fixed scale keeps them in
+// iteration of muon.cu multiplies.  Its matrices stay below 4 in magnitude, so one fixed scale keeps them in
 // the range of half precision, and the epilogue of one product writes the planes the next one reads: nothing
 // is split inside the main loop.
 //
-//  * a b = hi.hi + hi.lo + lo.hi: three MMAs for each 128 x BN x 16 step, at twice the rate and half the operand
+//  * a b = hi.hi + hi.lo + lo.hi: three MMAs for each step of 16 along K, at twice the rate and half the operand
 //    bytes of three TF32 MMAs of depth 8.
-//  * The tensor core truncates when it adds into its accumulator.  Each k-block of 64 is therefore a chunk of
-//    its own: its eight small products first, while the accumulator is small, then its four large ones; the
-//    finished chunk is added to fp32 registers with rounding while the next runs in the other half of tensor
-//    memory.
+//  * Operands lie as they are: K along the rows (K-major) or across them (MN-major), both in the 128-byte swizzle, so
+//    nothing is ever transposed in memory.
+//  * Large products run on pairs of SMs (cta_group::2, 256 x 256 tiles), smaller ones on single SMs (128 x 128,
+//    128 x 64).  Bound: shared memory, 128 bytes a clock.  Per MMA of depth 16 a single SM reads 8 KB of operands of a
+//    128 x 128 tile and TMA writes 5.3 KB: 104 clocks against the 64 of the tensor pipe (measured 120); a 128 x 256
+//    tile 12 + 8 KB: 156 against 128 (measured 165); the pair stages half of b on each side.
+//  * The tensor core truncates when it adds into its accumulator.  Every 64 along K are therefore a chunk of
+//    their own, the small products first; the finished chunk is added to fp32 registers with rounding while the
+//    next runs in the other half of tensor memory.
 //  * Roles (320 threads): warp 0 TMA, warp 1 MMA and tensor memory, warps 2 to 9 drain and epilogue (a lane owns
-//    a row; two groups of four warps own half the columns each).
-//  * The transpose leaves straight from the registers: 32 lanes hold 32 rows of a column; neighbouring lanes
-//    trade halves so that each stores 32 bits.
-//  * A symmetric product computes the tiles that reach the upper triangle; an element above the diagonal is
-//    stored at both places, so the result is symmetric bit for bit.
+//    a row; two groups of four warps own half the columns each).  One thread issues the MMAs; the descriptors
+//    of stages and steps are additions to one (with a descriptor built for each, issue took 180 clocks an MMA).
+//  * A symmetric product computes and stores the blocks on and above the diagonal.  Where a product needs a block
+//    below it, the block above is loaded as an MN-major operand in its place: K-block by K-block, the
+//    instruction descriptor says which.  (Storing both halves made the epilogue cost 0.15 ms of a 0.51 ms update of four
+//    1000 x 1000 matrices.)
 //  * Every wait is bounded, as in the general GEMM.
 #include <cuda.h>
 
@@ -30,31 +36,36 @@ int* device_error_flag();       // gemm_tc.cu
 
 constexpr int NS_BM = 128, NS_BK = 64, NS_THREADS = 320;
 
-template <int BN>
+// BN: columns of a tile; PAIR: the tile is 256 x 256, this CTA holds 128 rows of a, 128 rows of b and 128 x 256 of the
+// accumulator.
+template <int BN, bool PAIR>
 struct NsConfig {
-  static constexpr int A_BYTES = NS_BM * NS_BK * 2, B_BYTES = BN * NS_BK * 2;      // one plane
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
+  static constexpr int A_BYTES = NS_BM * NS_BK * 2, B_BYTES = B_ROWS * NS_BK * 2;  // one plane
   static constexpr int STAGE_BYTES = 2 * (A_BYTES + B_BYTES);
-  static constexpr int STAGES = BN == 256 ? 2 : BN == 128 ? 3 : 4;
+  static constexpr int STAGES = BN == 64 ? 4 : 3;
   static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int ACC = BN / 2;                                                // columns of a drain group
+  static constexpr int ACC = BN / 2;                                               // columns of a drain group
+  static constexpr int W = BN == 128 ? 64 : 32;                                    // columns of an epilogue step
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
 };
 
-struct NsEpilogue {
-  const __half* add;            // NULL or planes like out's
-  __half *out, *out_t;
-  int ld_add, ld_out, ld_out_t;
-  float alpha, beta;
+struct NsOut {
+  __half* data;
+  int ld;
+  float alpha, diagonal;
 };
+// How an operand lies: 0 K-major, 1 MN-major, else symmetric with blocks of that many rows (NsMatrix::upper).
+__device__ __forceinline__ bool ns_mn(int lies, int r0, int k0) { return lies <= 1 ? lies : k0 / lies < r0 / lies; }
 
 // Tile t of the walk: bands of 8 row tiles, column by column inside a band, so that the blocks that run
 // together share rows of both operands in L2.  Symmetric: only tiles that reach the diagonal or lie above it.
-__device__ __forceinline__ bool ns_tile(int t, int tiles_m, int tiles_n, int bn, bool symmetric, int* i, int* j) {
+__device__ __forceinline__ bool ns_tile(int t, int tiles_m, int tiles_n, int bm, int bn, bool symmetric, int* i, int* j) {
   for (int band = 0; band < tiles_m; band += 8) {
     const int rows = min(8, tiles_m - band);
-    for (int c = symmetric ? band * NS_BM / bn : 0; c < tiles_n; ++c) {
-      // rows of this band whose tile at column c reaches the diagonal: 128 i <= bn (c + 1) - 1
-      const int fit = symmetric ? min(rows, (bn * (c + 1) - 1) / NS_BM - band + 1) : rows;
+    for (int c = symmetric ? band * bm / bn : 0; c < tiles_n; ++c) {
+      // rows of this band whose tile at column c reaches the diagonal: bm i <= bn (c + 1) - 1
+      const int fit = symmetric ? min(rows, (bn * (c + 1) - 1) / bm - band + 1) : rows;
       if (!symmetric) {         // all columns of the band alike
         if (t >= rows * tiles_n) break;
         *i = band + t % rows;
@@ -72,92 +83,98 @@ __device__ __forceinline__ bool ns_tile(int t, int tiles_m, int tiles_n, int bn,
   }
   return false;
 }
-static int ns_tiles(int tiles_m, int tiles_n, int bn, bool symmetric) {
+static int ns_tiles(int tiles_m, int tiles_n, int bm, int bn, bool symmetric) {
   if (!symmetric) return tiles_m * tiles_n;
   int n = 0;
   for (int band = 0; band < tiles_m; band += 8) {
     const int rows = std::min(8, tiles_m - band);
-    for (int c = band * NS_BM / bn; c < tiles_n; ++c) n += std::min(rows, (bn * (c + 1) - 1) / NS_BM - band + 1);
+    for (int c = band * bm / bn; c < tiles_n; ++c) n += std::min(rows, (bn * (c + 1) - 1) / bm - band + 1);
   }
   return n;
 }
 
 __device__ __forceinline__ uint32_t ns_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
-// 32 columns of one row: from acc (row `row`, columns col ..) to the planes.
-template <bool DIAGONAL>
-__device__ __forceinline__ void ns_store(const float* acc, const NsEpilogue& e, int64_t plane, int64_t plane_t, int row, int col, int M, int N) {
-  uint32_t hi[16], lo[16];
-  const bool in = row < M;
-  const float alpha = e.alpha / NS_SCALE;
+// W columns (64 or 32) of a warp's 32 rows: from acc (lane: row row0 + lane; columns col ..) to the planes.  Rows go
+// through shared memory (`buf`, this warp's: both planes, 32 rows of W halves and 16 bytes), so that whole rows of a
+// tile meet global memory together: a lane that stored its own row touched 32 lines an instruction, which made the
+// epilogue of a 128 x 256 tile take 33 to 56 thousand clocks beside a main loop of 133 thousand (K = 4096).
+template <int W>
+__device__ __forceinline__ void ns_store(const float* acc, uint8_t* buf, const NsOut& e, int64_t plane, int row0, int col, int M) {
+  constexpr int PITCH = W * 2 + 16, PLANE = 32 * PITCH, LPR = W / 8, RPI = 32 / LPR;     // lanes per row, rows per instruction
+  const int lane = threadIdx.x & 31;
+  uint8_t* mine = buf + lane * PITCH;
+  const float alpha = e.alpha / NS_SCALE, diagonal = e.diagonal * NS_SCALE;
+  const int on = row0 + lane - col;                        // the diagonal's place among this lane's columns
 #pragma unroll
-  for (int c8 = 0; c8 < 4; ++c8) {
-    float add[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (e.add && in && col + 8 * c8 < e.ld_add) {
-      const int64_t at = (int64_t)row * e.ld_add + col + 8 * c8;
-      const uint4 h = *reinterpret_cast<const uint4*>(e.add + at), l = *reinterpret_cast<const uint4*>(e.add + plane + at);
-      const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hw[u])), b = __half22float2(*reinterpret_cast<const __half2*>(&lw[u]));
-        add[2 * u] = a.x + b.x;
-        add[2 * u + 1] = a.y + b.y;
-      }
-    }
+  for (int c8 = 0; c8 < W / 8; ++c8) {
+    uint32_t hi[4], lo[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float x = alpha * acc[8 * c8 + 2 * u] + e.beta * add[2 * u], y = alpha * acc[8 * c8 + 2 * u + 1] + e.beta * add[2 * u + 1];
+      const int c = 8 * c8 + 2 * u;
+      float x = alpha * acc[c], y = alpha * acc[c + 1];
+      if (on == c) x += diagonal;
+      if (on == c + 1) y += diagonal;
       const __half2 h = __floats2half2_rn(x, y);
       const float2 f = __half22float2(h);
-      hi[4 * c8 + u] = ns_bits(h);
-      lo[4 * c8 + u] = ns_bits(__floats2half2_rn(x - f.x, y - f.y));
+      hi[u] = ns_bits(h);
+      lo[u] = ns_bits(__floats2half2_rn(x - f.x, y - f.y));
     }
+    *reinterpret_cast<uint4*>(mine + 16 * c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(mine + PLANE + 16 * c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  if (e.out && in) {
+  __syncwarp();
+  const int lr = lane / LPR, lc = col + 8 * (lane % LPR);
 #pragma unroll
-    for (int c8 = 0; c8 < 4; ++c8) {
-      const int c = col + 8 * c8;
-      if (c >= e.ld_out) continue;
-      __half* at = e.out + (int64_t)row * e.ld_out + c;
-      if (!DIAGONAL || c >= row) {
-        *reinterpret_cast<uint4*>(at) = make_uint4(hi[4 * c8], hi[4 * c8 + 1], hi[4 * c8 + 2], hi[4 * c8 + 3]);
-        *reinterpret_cast<uint4*>(at + plane) = make_uint4(lo[4 * c8], lo[4 * c8 + 1], lo[4 * c8 + 2], lo[4 * c8 + 3]);
-      } else if (c + 7 >= row) {              // the group that the diagonal crosses in this row
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (c + u >= row) {
-            reinterpret_cast<uint16_t*>(at)[u] = (uint16_t)(hi[4 * c8 + u / 2] >> (16 * (u & 1)));
-            reinterpret_cast<uint16_t*>(at + plane)[u] = (uint16_t)(lo[4 * c8 + u / 2] >> (16 * (u & 1)));
-          }
-      }
-    }
+  for (int i = 0; i < LPR; ++i) {
+    const int r = row0 + lr + RPI * i;
+    const uint8_t* from = buf + (lr + RPI * i) * PITCH + 16 * (lane % LPR);
+    const uint4 h = *reinterpret_cast<const uint4*>(from), l = *reinterpret_cast<const uint4*>(from + PLANE);
+    if (r >= M || lc >= e.ld) continue;
+    __half* at = e.data + (int64_t)r * e.ld + lc;
+    *reinterpret_cast<uint4*>(at) = h;
+    *reinterpret_cast<uint4*>(at + plane) = l;
   }
-  if (e.out_t) {
-    const int odd = row & 1, r0 = row - odd;
+  __syncwarp();
+}
+
+// The end of a drain warp's work: its 32 rows x ACC columns.
+template <class Cfg>
+__device__ __forceinline__ void ns_finish(const float (&acc)[Cfg::ACC], uint8_t* smem, int drain_warp, NsOut e, int row0, int col0, int M, int N,
+                                          int b, int batch) {
+  constexpr int W = Cfg::W;
+  static_assert(8 * 2 * 32 * (W * 2 + 16) <= Cfg::STAGES * Cfg::STAGE_BYTES, "epilogue staging does not fit");
+  uint8_t* buf = smem + drain_warp * 2 * 32 * (W * 2 + 16);
+  e.data += (int64_t)b * M * e.ld;
+  const int64_t plane = (int64_t)batch * M * e.ld;
+  if (row0 >= M) return;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) {            // columns 2 u and 2 u + 1: the even lane takes the first, the odd one the second
-      const uint32_t ph = __shfl_xor_sync(0xffffffffu, hi[u], 1), pl = __shfl_xor_sync(0xffffffffu, lo[u], 1);
-      const uint32_t wh = odd ? __byte_perm(ph, hi[u], 0x7632) : __byte_perm(hi[u], ph, 0x5410);
-      const uint32_t wl = odd ? __byte_perm(pl, lo[u], 0x7632) : __byte_perm(lo[u], pl, 0x5410);
-      const int c = col + 2 * u + odd;
-      if (c >= N || r0 >= M) continue;
-      __half* at = e.out_t + (int64_t)c * e.ld_out_t + r0;
-      if (!DIAGONAL || c > r0 + 1) {
-        *reinterpret_cast<uint32_t*>(at) = wh;
-        *reinterpret_cast<uint32_t*>(at + plane_t) = wl;
-      } else if (c == r0 + 1) {               // the second row of the pair is the diagonal
-        *reinterpret_cast<uint16_t*>(at) = (uint16_t)wh;
-        *reinterpret_cast<uint16_t*>(at + plane_t) = (uint16_t)wl;
-      }
+  for (int cc = 0; cc < Cfg::ACC / W; ++cc)
+    if (col0 + W * cc < N) ns_store<W>(acc + W * cc, buf, e, plane, row0, col0 + W * cc, M);
+}
+
+// One operand's box row: rows [r0, r0 + ROWS) of both planes, 64 along K from k0, in the stage at `at`.
+//  K-major:  rows of 64 halves (128 bytes), eight of them 1024 bytes.
+//  MN-major: boxes of 64 K-rows x 64 operand rows (128 bytes each K-row), 8192 bytes apart.
+template <int ROWS>
+__device__ __forceinline__ void ns_load(uint32_t at, int plane_bytes, const CUtensorMap* map, const CUtensorMap* map_mn, bool mn, int k0, int r0, int batch, int b, uint32_t bar) {
+#pragma unroll
+  for (int plane = 0; plane < 2; ++plane) {
+    if (!mn) {
+      tma_load_3d(at + plane * plane_bytes, map, k0, r0, plane * batch + b, bar);
+    } else {
+#pragma unroll
+      for (int j = 0; j < ROWS / 64; ++j) tma_load_3d(at + plane * plane_bytes + j * 8192, map_mn, r0 + 64 * j, k0, plane * batch + b, bar);
     }
   }
 }
 
 template <int BN>
 __global__ void __launch_bounds__(NS_THREADS, 1)
-ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, NsEpilogue e, int M, int N, int K, int batch,
-               int symmetric, int* error_flag) {
-  using Cfg = NsConfig<BN>;
+ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_mn, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_b_mn, NsOut e, int M, int N, int K, int batch,
+               int a_lies, int b_lies, int symmetric, int* error_flag) {
+  using Cfg = NsConfig<BN, false>;
   constexpr int S = Cfg::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -169,7 +186,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.y;
   int ti = 0, tj = 0;
-  ns_tile(blockIdx.x, (M + NS_BM - 1) / NS_BM, (N + BN - 1) / BN, BN, symmetric, &ti, &tj);
+  ns_tile(blockIdx.x, (M + NS_BM - 1) / NS_BM, (N + BN - 1) / BN, NS_BM, BN, symmetric, &ti, &tj);
   const int m0 = ti * NS_BM, n0 = tj * BN;
   const int num_kb = (K + NS_BK - 1) / NS_BK;
   const uint32_t bar0 = smem_u32(bars), smem_base = smem_u32(smem);
@@ -177,8 +194,6 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
   auto acc_full_bar = [&](int i) { return bar0 + 8u * (2 * S + i); };
   auto acc_empty_bar = [&](int i) { return bar0 + 8u * (2 * S + 2 + i); };
-  auto a_at = [&](int s, int plane) { return smem_base + s * Cfg::STAGE_BYTES + plane * Cfg::A_BYTES; };
-  auto b_at = [&](int s, int plane) { return smem_base + s * Cfg::STAGE_BYTES + 2 * Cfg::A_BYTES + plane * Cfg::B_BYTES; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -187,7 +202,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full_bar(i), 1);
-      mbar_init(acc_empty_bar(i), 256);
+      mbar_init(acc_empty_bar(i), 8);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -212,11 +227,9 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const int s = kb % S;
         if (!mbar_wait(empty_bar(s), ((kb / S) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full_bar(s), Cfg::STAGE_BYTES);
-#pragma unroll
-        for (int plane = 0; plane < 2; ++plane) {
-          tma_load_3d(a_at(s, plane), &map_a, kb * NS_BK, m0, plane * batch + b, full_bar(s));
-          tma_load_3d(b_at(s, plane), &map_b, kb * NS_BK, n0, plane * batch + b, full_bar(s));
-        }
+        const uint32_t at = smem_base + s * Cfg::STAGE_BYTES;
+        ns_load<NS_BM>(at, Cfg::A_BYTES, &map_a, &map_a_mn, ns_mn(a_lies, m0, kb * NS_BK), kb * NS_BK, m0, batch, b, full_bar(s));
+        ns_load<BN>(at + 2 * Cfg::A_BYTES, Cfg::B_BYTES, &map_b, &map_b_mn, ns_mn(b_lies, n0, kb * NS_BK), kb * NS_BK, n0, batch, b, full_bar(s));
         issued = kb + 1;
       }
       if (*abort_flag) {        // copies already issued must land before shared memory is released
@@ -226,28 +239,34 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
     __syncwarp();
   } else if (warp == 1) {
-    // D = F32, A = B = F16, both K-major, N >> 3, M >> 4
-    const uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(NS_BM >> 4) << 24);
-    bool ok = true;
-    for (int kb = 0; kb < num_kb && ok; ++kb) {
-      const int s = kb % S, buf = kb & 1;
-      ok = mbar_wait(acc_empty_bar(buf), ((kb >> 1) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (kb / S) & 1, abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      if (lane == 0) {
+    if (lane == 0) {
+      // D = F32, A = B = F16, N >> 3, M >> 4; the majors are set for each k-block
+      const uint32_t idesc0 = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(NS_BM >> 4) << 24);
+      // descriptors of stage 0; stages, planes and steps along K are additions to their address field (16-byte units)
+      const uint64_t da0 = smem_desc(smem_base, 8192, 1024, 2), db0 = smem_desc(smem_base + 2 * Cfg::A_BYTES, 8192, 1024, 2);
+      bool ok = true;
+      int s = 0;
+      for (int kb = 0; kb < num_kb; ++kb, s = s + 1 == S ? 0 : s + 1) {
+        const int buf = kb & 1;
+        ok = mbar_wait(acc_empty_bar(buf), ((kb >> 1) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (kb / S) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const bool a_mn = ns_mn(a_lies, m0, kb * NS_BK), b_mn = ns_mn(b_lies, n0, kb * NS_BK);
+        const uint32_t idesc = idesc0 | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
+        const uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;       // 16 K-rows of 128 bytes, or 32 bytes
         const uint32_t d = tmem_d + (uint32_t)(buf * BN);
-        auto desc = [&](uint32_t at, int k) { return smem_desc(at + 32 * k, 16, 1024, 2); };
+        const uint64_t ah = da0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), al = ah + (Cfg::A_BYTES >> 4);
+        const uint64_t bh = db0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), bl = bh + (Cfg::B_BYTES >> 4);
 #pragma unroll
         for (int k = 0; k < NS_BK / 16; ++k) {          // the small products first
-          mma_f16(d, desc(a_at(s, 1), k), desc(b_at(s, 0), k), idesc, k > 0);
-          mma_f16(d, desc(a_at(s, 0), k), desc(b_at(s, 1), k), idesc, 1);
+          mma_f16(d, al + a_step * k, bh + b_step * k, idesc, k > 0);
+          mma_f16(d, ah + a_step * k, bl + b_step * k, idesc, 1);
         }
 #pragma unroll
-        for (int k = 0; k < NS_BK / 16; ++k) mma_f16(d, desc(a_at(s, 0), k), desc(b_at(s, 0), k), idesc, 1);
+        for (int k = 0; k < NS_BK / 16; ++k) mma_f16(d, ah + a_step * k, bh + b_step * k, idesc, 1);
         mma_commit(empty_bar(s));
         mma_commit(acc_full_bar(buf));
       }
-      __syncwarp();
     }
     __syncwarp();
   } else {
@@ -265,21 +284,11 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       tc_fence_after();
       drain_add<Cfg::ACC>(tmem_d + lane_bits + (uint32_t)(buf * BN + group * Cfg::ACC), acc);
       tc_fence_before();
-      mbar_arrive(acc_empty_bar(buf));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty_bar(buf));
     }
-    if (ok) {
-      const int row = m0 + q * 32 + lane;
-      e.add += e.add ? (int64_t)b * M * e.ld_add : 0;
-      e.out += e.out ? (int64_t)b * M * e.ld_out : 0;
-      e.out_t += e.out_t ? (int64_t)b * N * e.ld_out_t : 0;
-      const int64_t plane = (int64_t)batch * M * (e.out ? e.ld_out : e.ld_add), plane_t = (int64_t)batch * N * e.ld_out_t;
-#pragma unroll
-      for (int cc = 0; cc < Cfg::ACC / 32; ++cc) {
-        const int col = n0 + group * Cfg::ACC + 32 * cc;
-        if (symmetric && col < m0 + q * 32 + 32) ns_store<true>(acc + 32 * cc, e, plane, plane_t, row, col, M, N);
-        else if (col < N) ns_store<false>(acc + 32 * cc, e, plane, plane_t, row, col, M, N);
-      }
-    }
+    // every MMA has completed (the last chunk is drained): the stages are free
+    if (__all_sync(0xffffffffu, ok)) ns_finish<Cfg>(acc, smem, warp - 2, e, m0 + q * 32, n0 + group * Cfg::ACC, M, N, b, batch);
   }
   tc_fence_before();
   __syncthreads();
@@ -290,11 +299,160 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (threadIdx.x == 0 && *abort_flag && error_flag) *error_flag = 1;
 }
 
+// The same on pairs of SMs: two CTAs of a cluster (consecutive blockIdx.x) compute a 256 x 256 tile.  Each stages its own
+// 128 rows of a and its own 128 of the 256 rows of b; one thread of rank 0 issues the MMAs, which read both CTAs'
+// stages and leave each CTA's 128 x 256 of the product in its own tensor memory.  Rank 1's warp 1 tells rank 0
+// when its tiles have landed; "stage free" and "chunk ready" are committed to both.  Set-up and the release of
+// tensor memory stand between cluster barriers.
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NS_THREADS, 1)
+ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_mn, const __grid_constant__ CUtensorMap map_b,
+               const __grid_constant__ CUtensorMap map_b_mn, NsOut e, int M, int N, int K, int batch,
+                    int a_lies, int b_lies, int symmetric, int* error_flag) {
+  using Cfg = NsConfig<256, true>;
+  constexpr int S = Cfg::STAGES, BN = 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * Cfg::STAGE_BYTES);
+  // bars[0..S) full, [S..2S) empty, [2S..3S) the peer's tiles landed (rank 0's count), then chunk ready x 2, chunk drained x 2
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * S + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.y;
+  const uint32_t rank = cluster_rank();
+  int ti = 0, tj = 0;
+  ns_tile(blockIdx.x >> 1, (M + 255) / 256, (N + 255) / 256, 256, 256, symmetric, &ti, &tj);
+  const int m0 = ti * 256 + 128 * (int)rank, n0 = tj * 256;
+  // One instruction descriptor serves both CTAs.  With blocks of 128 the K-blocks of the tile's own first 128 are taken
+  // across the rows for both: they lie on the diagonal for the one and are stored above it for the other.
+  const int a_r = ti * 256 + (a_lies == 128 ? 128 : 0), b_r = n0 + (b_lies == 128 ? 128 : 0);
+  const int num_kb = (K + NS_BK - 1) / NS_BK;
+  const uint32_t bar0 = smem_u32(bars), smem_base = smem_u32(smem);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
+  auto peer_bar = [&](int s) { return bar0 + 8u * (2 * S + s); };
+  auto acc_full_bar = [&](int i) { return bar0 + 8u * (3 * S + i); };
+  auto acc_empty_bar = [&](int i) { return bar0 + 8u * (3 * S + 2 + i); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+      mbar_init(peer_bar(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full_bar(i), 1);
+      mbar_init(acc_empty_bar(i), 16);       // the drain warps of both CTAs
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_launch_dependents();
+  if (warp == 0 && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_d = *tmem_slot;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("fence.proxy.async;" ::: "memory");
+      int issued = 0;
+      for (int kb = 0; kb < num_kb; ++kb) {
+        const int s = kb % S;
+        if (!mbar_wait(empty_bar(s), ((kb / S) & 1) ^ 1, abort_flag)) break;
+        mbar_expect_tx(full_bar(s), Cfg::STAGE_BYTES);
+        const uint32_t at = smem_base + s * Cfg::STAGE_BYTES;
+        ns_load<NS_BM>(at, Cfg::A_BYTES, &map_a, &map_a_mn, ns_mn(a_lies, a_r, kb * NS_BK), kb * NS_BK, m0, batch, b, full_bar(s));
+        ns_load<128>(at + 2 * Cfg::A_BYTES, Cfg::B_BYTES, &map_b, &map_b_mn, ns_mn(b_lies, b_r, kb * NS_BK), kb * NS_BK, n0 + 128 * (int)rank, batch, b, full_bar(s));
+        issued = kb + 1;
+      }
+      if (*abort_flag) {
+        for (int kb = issued > S ? issued - S : 0; kb < issued; ++kb)
+          for (uint32_t it = 0; it < TC_SPIN_LIMIT && !mbar_try_wait(full_bar(kb % S), (kb / S) & 1); ++it) __nanosleep(64);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 1) {
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!mbar_wait(full_bar(kb % S), (kb / S) & 1, abort_flag)) break;
+        mbar_arrive_cluster(cluster_addr(peer_bar(kb % S), 0));
+      }
+    } else if (lane == 0) {
+      // D = F32, A = B = F16, N >> 3, M >> 4; the majors are set for each k-block
+      const uint32_t idesc0 = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+      // descriptors of stage 0; stages, planes and steps along K are additions to their address field (16-byte units)
+      const uint64_t da0 = smem_desc(smem_base, 8192, 1024, 2), db0 = smem_desc(smem_base + 2 * Cfg::A_BYTES, 8192, 1024, 2);
+      bool ok = true;
+      int s = 0;
+      for (int kb = 0; kb < num_kb; ++kb, s = s + 1 == S ? 0 : s + 1) {
+        const int buf = kb & 1;
+        ok = mbar_wait_cluster(acc_empty_bar(buf), ((kb >> 1) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (kb / S) & 1, abort_flag) &&
+             mbar_wait_cluster(peer_bar(s), (kb / S) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const bool a_mn = ns_mn(a_lies, a_r, kb * NS_BK), b_mn = ns_mn(b_lies, b_r, kb * NS_BK);
+        const uint32_t idesc = idesc0 | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
+        const uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;       // 16 K-rows of 128 bytes, or 32 bytes
+        const uint32_t d = tmem_d + (uint32_t)(buf * BN);
+        const uint64_t ah = da0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), al = ah + (Cfg::A_BYTES >> 4);
+        const uint64_t bh = db0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), bl = bh + (Cfg::B_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < NS_BK / 16; ++k) {
+          mma_f16_pair(d, al + a_step * k, bh + b_step * k, idesc, k > 0);
+          mma_f16_pair(d, ah + a_step * k, bl + b_step * k, idesc, 1);
+        }
+#pragma unroll
+        for (int k = 0; k < NS_BK / 16; ++k) mma_f16_pair(d, ah + a_step * k, bh + b_step * k, idesc, 1);
+        mma_commit_pair(empty_bar(s));                       // this CTA's stage and chunk, and the peer's
+        mma_commit_pair(cluster_addr(empty_bar(s), 1));
+        mma_commit_pair(acc_full_bar(buf));
+        mma_commit_pair(cluster_addr(acc_full_bar(buf), 1));
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, group = (warp - 2) >> 2;
+    const uint32_t lane_bits = (uint32_t)(q * 32) << 16;
+    float acc[Cfg::ACC];
+#pragma unroll
+    for (int j = 0; j < Cfg::ACC; ++j) acc[j] = 0.f;
+    bool ok = true;
+    for (int kb = 0; kb < num_kb && ok; ++kb) {
+      const int buf = kb & 1;
+      ok = mbar_wait(acc_full_bar(buf), (kb >> 1) & 1, abort_flag);
+      __syncwarp();
+      if (!ok) break;
+      tc_fence_after();
+      drain_add<Cfg::ACC>(tmem_d + lane_bits + (uint32_t)(buf * BN + group * Cfg::ACC), acc);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty_bar(buf), 0));
+    }
+    if (__all_sync(0xffffffffu, ok)) ns_finish<Cfg>(acc, smem, warp - 2, e, m0 + q * 32, n0 + group * Cfg::ACC, M, N, b, batch);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();        // nobody in the pair reads shared or tensor memory of the other any more
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_d, Cfg::TMEM_COLS);
+  }
+  if (threadIdx.x == 0 && *abort_flag && error_flag) *error_flag = 1;
+}
+
 typedef CUresult (*NsEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Both planes of a stack: K along the rows, rows, then plane and matrix; boxes of 64 x box_rows.
-static int ns_map(const NsMatrix& a, int batch, int box_rows, CUtensorMap* out) {
+// Both planes of a stack: along the rows, rows, then plane and matrix.  K-major boxes of 64 x rows, MN-major 64 x 64.
+static int ns_map(const NsMatrix& a, bool mn, int batch, int rows, CUtensorMap* out) {
   static NsEncodeFn encode = nullptr;
   if (!encode) {
     void* fn = nullptr;
@@ -305,42 +463,60 @@ static int ns_map(const NsMatrix& a, int batch, int box_rows, CUtensorMap* out) 
   }
   const cuuint64_t dims[3] = {(cuuint64_t)a.cols, (cuuint64_t)a.rows, (cuuint64_t)2 * batch};
   const cuuint64_t strides[2] = {(cuuint64_t)a.ld * 2, (cuuint64_t)a.ld * a.rows * 2};
-  const cuuint32_t box[3] = {(cuuint32_t)NS_BK, (cuuint32_t)box_rows, 1u}, one[3] = {1u, 1u, 1u};
+  const cuuint32_t box[3] = {64u, mn ? 64u : (cuuint32_t)rows, 1u}, one[3] = {1u, 1u, 1u};
   const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.data, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
   return B200_OK;
 }
 
-template <int BN>
-static int ns_launch(const NsMatrix& a, const NsMatrix& b, const NsEpilogue& e, int batch, bool symmetric) {
-  CUtensorMap ma, mb;
-  if (int rc = ns_map(a, batch, NS_BM, &ma)) return rc;
-  if (int rc = ns_map(b, batch, BN, &mb)) return rc;
-  int* flag = device_error_flag();
-  B200_REQUIRE(flag != nullptr, "the device error flag cannot be set up");
+typedef void (*NsKernel)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, NsOut, int, int, int, int, int, int, int, int*);
+
+int ns_gemm(const NsMatrix& a, bool a_t, const NsMatrix& b, bool b_t, NsMatrix* out, int batch, float alpha, float diagonal, bool symmetric) {
   static bool ready = false;
   if (!ready) {
-    B200_CUDA(cudaFuncSetAttribute(ns_gemm_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, NsConfig<BN>::SMEM_BYTES));
+    B200_CUDA(cudaFuncSetAttribute((NsKernel)ns_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NsConfig<256, true>::SMEM_BYTES));
+    B200_CUDA(cudaFuncSetAttribute((NsKernel)ns_gemm_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, NsConfig<128, false>::SMEM_BYTES));
+    B200_CUDA(cudaFuncSetAttribute((NsKernel)ns_gemm_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, NsConfig<64, false>::SMEM_BYTES));
     ready = true;
   }
-  const int tiles = ns_tiles((int)ceil_div(a.rows, NS_BM), (int)ceil_div(b.rows, BN), BN, symmetric);
-  B200_CUDA(launch_maybe_pdl(true, ns_gemm_kernel<BN>, dim3((unsigned)tiles, (unsigned)batch), dim3(NS_THREADS), (size_t)NsConfig<BN>::SMEM_BYTES,
-                             state().stream, ma, mb, e, a.rows, b.rows, a.cols, batch, symmetric ? 1 : 0, flag));
+  int* flag = device_error_flag();
+  B200_REQUIRE(flag != nullptr, "the device error flag cannot be set up");
+  const int M = out->rows, N = out->cols, K = a_t ? a.rows : a.cols;
+  const NsOut e = {out->data, out->ld, alpha, diagonal};
+  // The form with the least waves times clocks of a k-block (64 along K, 12 MMAs): pairs 1700 for 256 x 256, single SMs
+  // 1450 for 128 x 128 and 1320 for 128 x 64 (measured).
+  const int sms = state().sm_count;
+  auto cost = [&](int bm, int bn, int slots, int clocks, int* tiles) {
+    *tiles = ns_tiles((int)ceil_div(M, bm), (int)ceil_div(N, bn), bm, bn, symmetric);
+    return ceil_div((int64_t)*tiles * batch, slots) * clocks;
+  };
+  int tp, t128, t64;
+  const int64_t cp = cost(256, 256, sms / 2, 1700, &tp), c128 = cost(128, 128, sms, 1450, &t128), c64 = cost(128, 64, sms, 1320, &t64);
+  const int form = c64 < c128 && c64 < cp ? 64 : c128 <= cp ? 128 : 256;
+  const int tiles = form == 64 ? t64 : form == 128 ? t128 : 2 * tp;
+  NsKernel kernel = form == 256 ? (NsKernel)ns_gemm_pair_kernel : form == 128 ? (NsKernel)ns_gemm_kernel<128> : (NsKernel)ns_gemm_kernel<64>;
+  const size_t smem = form == 256 ? NsConfig<256, true>::SMEM_BYTES : form == 128 ? NsConfig<128, false>::SMEM_BYTES : NsConfig<64, false>::SMEM_BYTES;
+  out->upper = symmetric ? (form == 256 ? 256 : 128) : 0;
+  CUtensorMap ma, ma_mn, mb, mb_mn;
+  if (int rc = ns_map(a, false, batch, NS_BM, &ma)) return rc;
+  if (int rc = ns_map(a, true, batch, NS_BM, &ma_mn)) return rc;
+  if (int rc = ns_map(b, false, batch, form == 64 ? 64 : 128, &mb)) return rc;
+  if (int rc = ns_map(b, true, batch, 64, &mb_mn)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)tiles, (unsigned)batch);
+  cfg.blockDim = dim3(NS_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = state().stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, ma_mn, mb, mb_mn, e, M, N, K, batch, a.upper ? a.upper : (int)a_t, b.upper ? b.upper : (int)b_t,
+                               symmetric ? 1 : 0, flag));
   B200_LAUNCH_CHECK();
   return B200_OK;
-}
-
-int ns_gemm(const NsMatrix& a, const NsMatrix& b, const NsMatrix* add, const NsMatrix* out, const NsMatrix* out_t, int batch, float alpha,
-            float beta, bool symmetric) {
-  NsEpilogue e = {add ? add->data : nullptr, out ? out->data : nullptr, out_t ? out_t->data : nullptr, add ? add->ld : 0, out ? out->ld : 0,
-                  out_t ? out_t->ld : 0, alpha, beta};
-  // the widest tile whose tiles still fill the GPU
-  const int64_t tm = ceil_div(a.rows, NS_BM);
-  const int sms = state().sm_count;
-  if (batch * (int64_t)ns_tiles((int)tm, (int)ceil_div(b.rows, 256), 256, symmetric) >= sms) return ns_launch<256>(a, b, e, batch, symmetric);
-  if (batch * (int64_t)ns_tiles((int)tm, (int)ceil_div(b.rows, 128), 128, symmetric) * 2 >= sms) return ns_launch<128>(a, b, e, batch, symmetric);
-  return ns_launch<64>(a, b, e, batch, symmetric);
 }
 
 }  // namespace b200

@@ -7,16 +7,16 @@
 namespace b200 {
 
 // A matrix (or a stack of them) as hi and lo planes: value = (hi + lo) / NS_SCALE.  Plane p of matrix b
-// starts at (p * batch + b) * rows * ld; ld is a multiple of 8.
+// starts at (p * batch + b) * rows * ld; ld is a multiple of 8.  `upper`: the matrix is symmetric and only its
+// blocks (i, j) of upper x upper with j >= i are stored (0: all of it).
 struct NsMatrix {
   __half* data;
-  int rows, cols, ld;
+  int rows, cols, ld, upper;
 };
 constexpr float NS_SCALE = 4096.f;
 
-// out = alpha * a b^T + beta * add, for each matrix of the stack; a is (M, K), b is (N, K), both with K along
-// the rows.  symmetric: the product is known to be symmetric; one triangle is computed and stored twice.
-// out_t, if given, receives the transpose (N, M).  add may be NULL, out may be NULL when out_t is given.
-int ns_gemm(const NsMatrix& a, const NsMatrix& b, const NsMatrix* add, const NsMatrix* out, const NsMatrix* out_t, int batch, float alpha,
-            float beta, bool symmetric);
+// out = alpha * op(a) op(b)^T + diagonal * I, for each matrix of the stack; op(x) is x, (rows, K), or with _t the
+// transpose of x, stored (K, rows).  symmetric: the product is known to be symmetric; only its upper blocks are
+// computed, and out->upper is set.
+int ns_gemm(const NsMatrix& a, bool a_t, const NsMatrix& b, bool b_t, NsMatrix* out, int batch, float alpha, float diagonal, bool symmetric);
 }  // namespace b200
