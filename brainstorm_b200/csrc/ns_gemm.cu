@@ -10,11 +10,14 @@
 //    nothing is ever transposed in memory.
 //  * Large products run on pairs of SMs (cta_group::2, 256 x 256 tiles), smaller ones on single SMs (128 x 128,
 //    128 x 64).  Bound: shared memory, 128 bytes a clock.  Per MMA of depth 16 a single SM reads 8 KB of operands of a
-//    128 x 128 tile and TMA writes 5.3 KB: 104 clocks against the 64 of the tensor pipe (measured 120); a 128 x 256
-//    tile 12 + 8 KB: 156 against 128 (measured 165); the pair stages half of b on each side.
-//  * The tensor core truncates when it adds into its accumulator.  Every 64 along K are therefore a chunk of
-//    their own, the small products first; the finished chunk is added to fp32 registers with rounding while the
-//    next runs in the other half of tensor memory.
+//    128 x 128 tile and TMA writes 5.3 KB: 104 clocks against the 64 of the tensor pipe (measured 120).  A 128 x 256
+//    tile on one SM wants 12 + 8 KB, 156 clocks against 128 (measured 165, and two stages do not cover a load); the
+//    pair stages half of b on each side.
+//  * The tensor core truncates when it adds into its accumulator.  Every 64 along K (128 on pairs) are therefore a
+//    chunk of their own, in each k-block the small products first; the finished chunk is added to fp32 registers
+//    with rounding while the next runs in the other half of tensor memory.  On pairs the way of a chunk from the
+//    issuing SM to the drain warps of both and back is longer than the MMAs of 64 along K: with such chunks a
+//    4096 x 4096 update took 4.6 ms, with 128 it takes 3.7.
 //  * Roles (320 threads): warp 0 TMA, warp 1 MMA and tensor memory, warps 2 to 9 drain and epilogue (a lane owns
 //    a row; two groups of four warps own half the columns each).  One thread issues the MMAs; the descriptors
 //    of stages and steps are additions to one (with a descriptor built for each, issue took 180 clocks an MMA).
@@ -34,21 +37,29 @@ namespace b200 {
 
 int* device_error_flag();       // gemm_tc.cu
 
-constexpr int NS_BM = 128, NS_BK = 64, NS_THREADS = 320;
+constexpr int NS_BM = 128, NS_THREADS = 320;
 
 // BN: columns of a tile; PAIR: the tile is 256 x 256, this CTA holds 128 rows of a, 128 rows of b and 128 x 256 of the
 // accumulator.
-template <int BN, bool PAIR>
+template <int BN_, bool PAIR>
 struct NsConfig {
-  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
-  static constexpr int A_BYTES = NS_BM * NS_BK * 2, B_BYTES = B_ROWS * NS_BK * 2;  // one plane
+  static constexpr int BN = BN_, BK = 64, B_ROWS = PAIR ? BN / 2 : BN;
+  static constexpr int A_BYTES = NS_BM * BK * 2, B_BYTES = B_ROWS * BK * 2;        // one plane
   static constexpr int STAGE_BYTES = 2 * (A_BYTES + B_BYTES);
-  static constexpr int STAGES = BN == 64 ? 4 : 3;
+  static constexpr int STAGES = 196608 / STAGE_BYTES;
+  static constexpr int CHUNK = (PAIR ? 128 : 64) / BK;                             // stages between two drains
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int ACC = BN / 2;                                               // columns of a drain group
   static constexpr int W = BN == 128 ? 64 : 32;                                    // columns of an epilogue step
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+  // Descriptors, both in the 128-byte swizzle.  K-major: rows of 64 halves, eight of them one group.  MN-major: boxes of 64
+  // K-rows x 64 operand rows (128 bytes a K-row), eight K-rows one group.
+  __device__ static uint64_t desc_k(uint32_t at) { return smem_desc(at, 16, 1024, 2); }
+  __device__ static uint64_t desc_mn(uint32_t at) { return smem_desc(at, BK * 128, 1024, 2); }
 };
+using NsPair = NsConfig<256, true>;
+using Ns128 = NsConfig<128, false>;
+using Ns64 = NsConfig<64, false>;
 
 struct NsOut {
   __half* data;
@@ -153,29 +164,28 @@ __device__ __forceinline__ void ns_finish(const float (&acc)[Cfg::ACC], uint8_t*
     if (col0 + W * cc < N) ns_store<W>(acc + W * cc, buf, e, plane, row0, col0 + W * cc, M);
 }
 
-// One operand's box row: rows [r0, r0 + ROWS) of both planes, 64 along K from k0, in the stage at `at`.
-//  K-major:  rows of 64 halves (128 bytes), eight of them 1024 bytes.
-//  MN-major: boxes of 64 K-rows x 64 operand rows (128 bytes each K-row), 8192 bytes apart.
-template <int ROWS>
-__device__ __forceinline__ void ns_load(uint32_t at, int plane_bytes, const CUtensorMap* map, const CUtensorMap* map_mn, bool mn, int k0, int r0, int batch, int b, uint32_t bar) {
+// ROWS rows of an operand from r0, BK along K from k0, both planes, into the stage at `at`.
+template <int ROWS, int BK>
+__device__ __forceinline__ void ns_load(uint32_t at, const CUtensorMap* map, const CUtensorMap* map_mn, bool mn, int k0, int r0, int batch, int b,
+                                        uint32_t bar) {
 #pragma unroll
   for (int plane = 0; plane < 2; ++plane) {
+    const uint32_t to = at + plane * ROWS * BK * 2;
     if (!mn) {
-      tma_load_3d(at + plane * plane_bytes, map, k0, r0, plane * batch + b, bar);
+      tma_load_3d(to, map, k0, r0, plane * batch + b, bar);
     } else {
 #pragma unroll
-      for (int j = 0; j < ROWS / 64; ++j) tma_load_3d(at + plane * plane_bytes + j * 8192, map_mn, r0 + 64 * j, k0, plane * batch + b, bar);
+      for (int j = 0; j < ROWS / 64; ++j) tma_load_3d(to + j * BK * 128, map_mn, r0 + 64 * j, k0, plane * batch + b, bar);
     }
   }
 }
 
-template <int BN>
+template <class Cfg>
 __global__ void __launch_bounds__(NS_THREADS, 1)
 ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_mn, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b_mn, NsOut e, int M, int N, int K, int batch,
                int a_lies, int b_lies, int symmetric, int* error_flag) {
-  using Cfg = NsConfig<BN, false>;
-  constexpr int S = Cfg::STAGES;
+  constexpr int S = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, CH = Cfg::CHUNK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * Cfg::STAGE_BYTES);
@@ -188,7 +198,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   int ti = 0, tj = 0;
   ns_tile(blockIdx.x, (M + NS_BM - 1) / NS_BM, (N + BN - 1) / BN, NS_BM, BN, symmetric, &ti, &tj);
   const int m0 = ti * NS_BM, n0 = tj * BN;
-  const int num_kb = (K + NS_BK - 1) / NS_BK;
+  const int num_kb = (K + BK - 1) / BK;
   const uint32_t bar0 = smem_u32(bars), smem_base = smem_u32(smem);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
@@ -228,8 +238,8 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (!mbar_wait(empty_bar(s), ((kb / S) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full_bar(s), Cfg::STAGE_BYTES);
         const uint32_t at = smem_base + s * Cfg::STAGE_BYTES;
-        ns_load<NS_BM>(at, Cfg::A_BYTES, &map_a, &map_a_mn, ns_mn(a_lies, m0, kb * NS_BK), kb * NS_BK, m0, batch, b, full_bar(s));
-        ns_load<BN>(at + 2 * Cfg::A_BYTES, Cfg::B_BYTES, &map_b, &map_b_mn, ns_mn(b_lies, n0, kb * NS_BK), kb * NS_BK, n0, batch, b, full_bar(s));
+        ns_load<NS_BM, BK>(at, &map_a, &map_a_mn, ns_mn(a_lies, m0, kb * BK), kb * BK, m0, batch, b, full_bar(s));
+        ns_load<BN, BK>(at + 2 * Cfg::A_BYTES, &map_b, &map_b_mn, ns_mn(b_lies, n0, kb * BK), kb * BK, n0, batch, b, full_bar(s));
         issued = kb + 1;
       }
       if (*abort_flag) {        // copies already issued must land before shared memory is released
@@ -243,29 +253,32 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       // D = F32, A = B = F16, N >> 3, M >> 4; the majors are set for each k-block
       const uint32_t idesc0 = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(NS_BM >> 4) << 24);
       // descriptors of stage 0; stages, planes and steps along K are additions to their address field (16-byte units)
-      const uint64_t da0 = smem_desc(smem_base, 8192, 1024, 2), db0 = smem_desc(smem_base + 2 * Cfg::A_BYTES, 8192, 1024, 2);
+      const uint64_t da_k = Cfg::desc_k(smem_base), da_mn = Cfg::desc_mn(smem_base);
+      const uint64_t db_k = Cfg::desc_k(smem_base + 2 * Cfg::A_BYTES), db_mn = Cfg::desc_mn(smem_base + 2 * Cfg::A_BYTES);
       bool ok = true;
       int s = 0;
       for (int kb = 0; kb < num_kb; ++kb, s = s + 1 == S ? 0 : s + 1) {
-        const int buf = kb & 1;
-        ok = mbar_wait(acc_empty_bar(buf), ((kb >> 1) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (kb / S) & 1, abort_flag);
+        const int chunk = kb / CH, buf = chunk & 1;
+        const bool fresh = kb % CH == 0, last = kb % CH == CH - 1 || kb == num_kb - 1;
+        if (fresh) ok = mbar_wait(acc_empty_bar(buf), ((chunk >> 1) & 1) ^ 1, abort_flag);
+        ok = ok && mbar_wait(full_bar(s), (kb / S) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const bool a_mn = ns_mn(a_lies, m0, kb * NS_BK), b_mn = ns_mn(b_lies, n0, kb * NS_BK);
+        const bool a_mn = ns_mn(a_lies, m0, kb * BK), b_mn = ns_mn(b_lies, n0, kb * BK);
         const uint32_t idesc = idesc0 | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
         const uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;       // 16 K-rows of 128 bytes, or 32 bytes
         const uint32_t d = tmem_d + (uint32_t)(buf * BN);
-        const uint64_t ah = da0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), al = ah + (Cfg::A_BYTES >> 4);
-        const uint64_t bh = db0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), bl = bh + (Cfg::B_BYTES >> 4);
+        const uint64_t ah = (a_mn ? da_mn : da_k) + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), al = ah + (Cfg::A_BYTES >> 4);
+        const uint64_t bh = (b_mn ? db_mn : db_k) + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), bl = bh + (Cfg::B_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < NS_BK / 16; ++k) {          // the small products first
-          mma_f16(d, al + a_step * k, bh + b_step * k, idesc, k > 0);
+        for (int k = 0; k < BK / 16; ++k) {          // the small products first
+          mma_f16(d, al + a_step * k, bh + b_step * k, idesc, !(fresh && k == 0));
           mma_f16(d, ah + a_step * k, bl + b_step * k, idesc, 1);
         }
 #pragma unroll
-        for (int k = 0; k < NS_BK / 16; ++k) mma_f16(d, ah + a_step * k, bh + b_step * k, idesc, 1);
+        for (int k = 0; k < BK / 16; ++k) mma_f16(d, ah + a_step * k, bh + b_step * k, idesc, 1);
         mma_commit(empty_bar(s));
-        mma_commit(acc_full_bar(buf));
+        if (last) mma_commit(acc_full_bar(buf));
       }
     }
     __syncwarp();
@@ -276,9 +289,10 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
     for (int j = 0; j < Cfg::ACC; ++j) acc[j] = 0.f;
     bool ok = true;
-    for (int kb = 0; kb < num_kb && ok; ++kb) {
-      const int buf = kb & 1;
-      ok = mbar_wait(acc_full_bar(buf), (kb >> 1) & 1, abort_flag);
+    const int chunks = (num_kb + CH - 1) / CH;
+    for (int chunk = 0; chunk < chunks && ok; ++chunk) {
+      const int buf = chunk & 1;
+      ok = mbar_wait(acc_full_bar(buf), (chunk >> 1) & 1, abort_flag);
       __syncwarp();
       if (!ok) break;
       tc_fence_after();
@@ -308,8 +322,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NS_THREADS, 1)
 ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_mn, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CUtensorMap map_b_mn, NsOut e, int M, int N, int K, int batch,
                     int a_lies, int b_lies, int symmetric, int* error_flag) {
-  using Cfg = NsConfig<256, true>;
-  constexpr int S = Cfg::STAGES, BN = 256;
+  using Cfg = NsPair;
+  constexpr int S = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, CH = Cfg::CHUNK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * Cfg::STAGE_BYTES);
@@ -326,7 +340,7 @@ ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   // One instruction descriptor serves both CTAs.  With blocks of 128 the K-blocks of the tile's own first 128 are taken
   // across the rows for both: they lie on the diagonal for the one and are stored above it for the other.
   const int a_r = ti * 256 + (a_lies == 128 ? 128 : 0), b_r = n0 + (b_lies == 128 ? 128 : 0);
-  const int num_kb = (K + NS_BK - 1) / NS_BK;
+  const int num_kb = (K + BK - 1) / BK;
   const uint32_t bar0 = smem_u32(bars), smem_base = smem_u32(smem);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
@@ -369,8 +383,8 @@ ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if (!mbar_wait(empty_bar(s), ((kb / S) & 1) ^ 1, abort_flag)) break;
         mbar_expect_tx(full_bar(s), Cfg::STAGE_BYTES);
         const uint32_t at = smem_base + s * Cfg::STAGE_BYTES;
-        ns_load<NS_BM>(at, Cfg::A_BYTES, &map_a, &map_a_mn, ns_mn(a_lies, a_r, kb * NS_BK), kb * NS_BK, m0, batch, b, full_bar(s));
-        ns_load<128>(at + 2 * Cfg::A_BYTES, Cfg::B_BYTES, &map_b, &map_b_mn, ns_mn(b_lies, b_r, kb * NS_BK), kb * NS_BK, n0 + 128 * (int)rank, batch, b, full_bar(s));
+        ns_load<NS_BM, BK>(at, &map_a, &map_a_mn, ns_mn(a_lies, a_r, kb * BK), kb * BK, m0, batch, b, full_bar(s));
+        ns_load<128, BK>(at + 2 * Cfg::A_BYTES, &map_b, &map_b_mn, ns_mn(b_lies, b_r, kb * BK), kb * BK, n0 + 128 * (int)rank, batch, b, full_bar(s));
         issued = kb + 1;
       }
       if (*abort_flag) {
@@ -389,32 +403,36 @@ ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       // D = F32, A = B = F16, N >> 3, M >> 4; the majors are set for each k-block
       const uint32_t idesc0 = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
       // descriptors of stage 0; stages, planes and steps along K are additions to their address field (16-byte units)
-      const uint64_t da0 = smem_desc(smem_base, 8192, 1024, 2), db0 = smem_desc(smem_base + 2 * Cfg::A_BYTES, 8192, 1024, 2);
+      const uint64_t da_k = Cfg::desc_k(smem_base), da_mn = Cfg::desc_mn(smem_base);
+      const uint64_t db_k = Cfg::desc_k(smem_base + 2 * Cfg::A_BYTES), db_mn = Cfg::desc_mn(smem_base + 2 * Cfg::A_BYTES);
       bool ok = true;
       int s = 0;
       for (int kb = 0; kb < num_kb; ++kb, s = s + 1 == S ? 0 : s + 1) {
-        const int buf = kb & 1;
-        ok = mbar_wait_cluster(acc_empty_bar(buf), ((kb >> 1) & 1) ^ 1, abort_flag) && mbar_wait(full_bar(s), (kb / S) & 1, abort_flag) &&
-             mbar_wait_cluster(peer_bar(s), (kb / S) & 1, abort_flag);
+        const int chunk = kb / CH, buf = chunk & 1;
+        const bool fresh = kb % CH == 0, last = kb % CH == CH - 1 || kb == num_kb - 1;
+        if (fresh) ok = mbar_wait_cluster(acc_empty_bar(buf), ((chunk >> 1) & 1) ^ 1, abort_flag);
+        ok = ok && mbar_wait(full_bar(s), (kb / S) & 1, abort_flag) && mbar_wait_cluster(peer_bar(s), (kb / S) & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const bool a_mn = ns_mn(a_lies, a_r, kb * NS_BK), b_mn = ns_mn(b_lies, b_r, kb * NS_BK);
+        const bool a_mn = ns_mn(a_lies, a_r, kb * BK), b_mn = ns_mn(b_lies, b_r, kb * BK);
         const uint32_t idesc = idesc0 | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
         const uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;       // 16 K-rows of 128 bytes, or 32 bytes
         const uint32_t d = tmem_d + (uint32_t)(buf * BN);
-        const uint64_t ah = da0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), al = ah + (Cfg::A_BYTES >> 4);
-        const uint64_t bh = db0 + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), bl = bh + (Cfg::B_BYTES >> 4);
+        const uint64_t ah = (a_mn ? da_mn : da_k) + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), al = ah + (Cfg::A_BYTES >> 4);
+        const uint64_t bh = (b_mn ? db_mn : db_k) + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), bl = bh + (Cfg::B_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < NS_BK / 16; ++k) {
-          mma_f16_pair(d, al + a_step * k, bh + b_step * k, idesc, k > 0);
+        for (int k = 0; k < BK / 16; ++k) {
+          mma_f16_pair(d, al + a_step * k, bh + b_step * k, idesc, !(fresh && k == 0));
           mma_f16_pair(d, ah + a_step * k, bl + b_step * k, idesc, 1);
         }
 #pragma unroll
-        for (int k = 0; k < NS_BK / 16; ++k) mma_f16_pair(d, ah + a_step * k, bh + b_step * k, idesc, 1);
+        for (int k = 0; k < BK / 16; ++k) mma_f16_pair(d, ah + a_step * k, bh + b_step * k, idesc, 1);
         mma_commit_pair(empty_bar(s));                       // this CTA's stage and chunk, and the peer's
         mma_commit_pair(cluster_addr(empty_bar(s), 1));
-        mma_commit_pair(acc_full_bar(buf));
-        mma_commit_pair(cluster_addr(acc_full_bar(buf), 1));
+        if (last) {
+          mma_commit_pair(acc_full_bar(buf));
+          mma_commit_pair(cluster_addr(acc_full_bar(buf), 1));
+        }
       }
     }
     __syncwarp();
@@ -425,9 +443,10 @@ ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll
     for (int j = 0; j < Cfg::ACC; ++j) acc[j] = 0.f;
     bool ok = true;
-    for (int kb = 0; kb < num_kb && ok; ++kb) {
-      const int buf = kb & 1;
-      ok = mbar_wait(acc_full_bar(buf), (kb >> 1) & 1, abort_flag);
+    const int chunks = (num_kb + CH - 1) / CH;
+    for (int chunk = 0; chunk < chunks && ok; ++chunk) {
+      const int buf = chunk & 1;
+      ok = mbar_wait(acc_full_bar(buf), (chunk >> 1) & 1, abort_flag);
       __syncwarp();
       if (!ok) break;
       tc_fence_after();
@@ -473,47 +492,53 @@ static int ns_map(const NsMatrix& a, bool mn, int batch, int rows, CUtensorMap* 
 typedef void (*NsKernel)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, NsOut, int, int, int, int, int, int, int, int*);
 
 int ns_gemm(const NsMatrix& a, bool a_t, const NsMatrix& b, bool b_t, NsMatrix* out, int batch, float alpha, float diagonal, bool symmetric) {
+  // tile height and width, SMs of a tile, clocks for 64 along K (12 MMAs; measured), rows of b in a box
+  struct Form {
+    NsKernel kernel;
+    int bm, bn, sms, clocks, b_rows, smem;
+  };
+  static const Form forms[] = {{(NsKernel)ns_gemm_kernel<Ns128>, 128, 128, 1, 1450, 128, Ns128::SMEM_BYTES},
+                               {(NsKernel)ns_gemm_kernel<Ns64>, 128, 64, 1, 1320, 64, Ns64::SMEM_BYTES},
+                               {(NsKernel)ns_gemm_pair_kernel, 256, 256, 2, 1700, 128, NsPair::SMEM_BYTES}};
   static bool ready = false;
   if (!ready) {
-    B200_CUDA(cudaFuncSetAttribute((NsKernel)ns_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NsConfig<256, true>::SMEM_BYTES));
-    B200_CUDA(cudaFuncSetAttribute((NsKernel)ns_gemm_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, NsConfig<128, false>::SMEM_BYTES));
-    B200_CUDA(cudaFuncSetAttribute((NsKernel)ns_gemm_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, NsConfig<64, false>::SMEM_BYTES));
+    for (const Form& f : forms) B200_CUDA(cudaFuncSetAttribute(f.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, f.smem));
     ready = true;
   }
   int* flag = device_error_flag();
   B200_REQUIRE(flag != nullptr, "the device error flag cannot be set up");
   const int M = out->rows, N = out->cols, K = a_t ? a.rows : a.cols;
   const NsOut e = {out->data, out->ld, alpha, diagonal};
-  // The form with the least waves times clocks of a k-block (64 along K, 12 MMAs): pairs 1700 for 256 x 256, single SMs
-  // 1450 for 128 x 128 and 1320 for 128 x 64 (measured).
-  const int sms = state().sm_count;
-  auto cost = [&](int bm, int bn, int slots, int clocks, int* tiles) {
-    *tiles = ns_tiles((int)ceil_div(M, bm), (int)ceil_div(N, bn), bm, bn, symmetric);
-    return ceil_div((int64_t)*tiles * batch, slots) * clocks;
-  };
-  int tp, t128, t64;
-  const int64_t cp = cost(256, 256, sms / 2, 1700, &tp), c128 = cost(128, 128, sms, 1450, &t128), c64 = cost(128, 64, sms, 1320, &t64);
-  const int form = c64 < c128 && c64 < cp ? 64 : c128 <= cp ? 128 : 256;
-  const int tiles = form == 64 ? t64 : form == 128 ? t128 : 2 * tp;
-  NsKernel kernel = form == 256 ? (NsKernel)ns_gemm_pair_kernel : form == 128 ? (NsKernel)ns_gemm_kernel<128> : (NsKernel)ns_gemm_kernel<64>;
-  const size_t smem = form == 256 ? NsConfig<256, true>::SMEM_BYTES : form == 128 ? NsConfig<128, false>::SMEM_BYTES : NsConfig<64, false>::SMEM_BYTES;
-  out->upper = symmetric ? (form == 256 ? 256 : 128) : 0;
+  // the form with the least waves times clocks
+  const Form* best = nullptr;
+  int64_t least = 0;
+  int tiles = 0;
+  for (const Form& f : forms) {
+    const int t = ns_tiles((int)ceil_div(M, f.bm), (int)ceil_div(N, f.bn), f.bm, f.bn, symmetric);
+    const int64_t cost = ceil_div((int64_t)t * batch, state().sm_count / f.sms) * f.clocks;
+    if (!best || cost < least) {
+      best = &f;
+      least = cost;
+      tiles = t * f.sms;
+    }
+  }
+  out->upper = symmetric ? std::max(best->bm, best->bn) < 256 ? 128 : 256 : 0;
   CUtensorMap ma, ma_mn, mb, mb_mn;
   if (int rc = ns_map(a, false, batch, NS_BM, &ma)) return rc;
   if (int rc = ns_map(a, true, batch, NS_BM, &ma_mn)) return rc;
-  if (int rc = ns_map(b, false, batch, form == 64 ? 64 : 128, &mb)) return rc;
-  if (int rc = ns_map(b, true, batch, 64, &mb_mn)) return rc;
+  if (int rc = ns_map(b, false, batch, best->b_rows, &mb)) return rc;
+  if (int rc = ns_map(b, true, batch, best->b_rows, &mb_mn)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)tiles, (unsigned)batch);
   cfg.blockDim = dim3(NS_THREADS);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = best->smem;
   cfg.stream = state().stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  B200_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, ma_mn, mb, mb_mn, e, M, N, K, batch, a.upper ? a.upper : (int)a_t, b.upper ? b.upper : (int)b_t,
+  B200_CUDA(cudaLaunchKernelEx(&cfg, best->kernel, ma, ma_mn, mb, mb_mn, e, M, N, K, batch, a.upper ? a.upper : (int)a_t, b.upper ? b.upper : (int)b_t,
                                symmetric ? 1 : 0, flag));
   B200_LAUNCH_CHECK();
   return B200_OK;
