@@ -72,20 +72,32 @@ __device__ __forceinline__ void lc_mma3(float (&c0)[4], float (&c1)[4], float (&
   lc_mma(c2, ah, bh[4], bh[5]);
   lc_mma(c3, ah, bh[6], bh[7]);
 }
-// c (16 x 64) += a (16 x 16) b, b the 16 rows from `row` of a tile of 64 columns, whose first nt_n 8-column tiles count
-__device__ __forceinline__ void lc_rows(float (&c)[8][4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t hi, uint32_t lo, int row, int lane,
-                                        int nt_n) {
+// the same for two tiles
+__device__ __forceinline__ void lc_mma3(float (&c0)[4], float (&c1)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], const uint32_t (&bh)[8],
+                                        const uint32_t (&bl)[8]) {
+  lc_mma(c0, al, bh[0], bh[1]);
+  lc_mma(c1, al, bh[2], bh[3]);
+  lc_mma(c0, ah, bl[0], bl[1]);
+  lc_mma(c1, ah, bl[2], bl[3]);
+  lc_mma(c0, ah, bh[0], bh[1]);
+  lc_mma(c1, ah, bh[2], bh[3]);
+}
+// c (16 x 8 N) += a (16 x 16) b, b the 16 rows from `row` of a tile of 64 columns, from its 8-column tile `first` on; tiles
+// from nt_n on do not count
+template <int N>
+__device__ __forceinline__ void lc_rows(float (&c)[N][4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t hi, uint32_t lo, int row, int lane,
+                                        int nt_n, int first = 0) {
 #pragma unroll
-  for (int vt = 0; vt < 4; vt += 2)
-    if (2 * vt < nt_n) {
+  for (int nt = 0; nt < N; nt += 4)
+    if (first + nt < nt_n) {
       uint32_t bh[8], bl[8];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint32_t at = (uint32_t)((row + (lane & 15)) * 128 + (((2 * (vt + u) + (lane >> 4)) ^ (lane & 7)) << 4));
+        const uint32_t at = (uint32_t)((row + (lane & 15)) * 128 + (((first + nt + 2 * u + (lane >> 4)) ^ (lane & 7)) << 4));
         lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bh + 4 * u), hi + at);
         lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bl + 4 * u), lo + at);
       }
-      lc_mma3(c[2 * vt], c[2 * vt + 1], c[2 * vt + 2], c[2 * vt + 3], ah, al, bh, bl);
+      lc_mma3(c[nt], c[nt + 1], c[nt + 2], c[nt + 3], ah, al, bh, bl);
     }
 }
 __device__ __forceinline__ uint32_t lc_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -171,9 +183,8 @@ struct LcSmem {
 
 // Warps 0 to 3 compute the outputs of 16 tokens each, warps 4 to 7 keep the state, in their registers; all eight
 // load and split the tiles.  DK: 64 or 128, the largest dk the block can hold.  VEC: 128-bit global loads.
-// STATE_ONLY: the state pass.
-template <int DK, bool VEC, bool STATE_ONLY>
-__global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs) {
+template <int DK, bool VEC>
+__global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs, int sms) {
   using L = LcSmem<DK>;
   constexpr int MT = DK / 64;                        // 16-row tiles of the state in a state warp
   constexpr int LPR = DK / 4, RPP = LC_THREADS / LPR;   // lanes per row of k, rows in a pass
@@ -189,7 +200,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
   id /= max_slabs;
   const int seg = id % segments, bh = id / segments;
   const int slabs = (p.dv + LC_COLS - 1) / LC_COLS;
-  if (slab >= slabs || (STATE_ONLY && !cr.state_pass)) return;
+  if (slab >= slabs) return;
   const int b = bh / c.H, h = bh % c.H;
   const int n_all = la_length(c, b);
   const int64_t first = (int64_t)seg * seg_tokens;                 // steps of this segment
@@ -208,10 +219,10 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
   const int64_t tok0 = p.reverse ? n_all - 1 : 0;
   const int64_t q_t = p.reverse ? -p.qs.t : p.qs.t, k_t = p.reverse ? -p.ks.t : p.ks.t, v_t = p.reverse ? -p.vs.t : p.vs.t,
                 o_t = p.reverse ? -p.os.t : p.os.t;
-  const float* q = STATE_ONLY ? nullptr : p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h + tok0 * p.qs.t;
+  const float* q = p.q + (int64_t)b * p.qs.b + (int64_t)(h / p.qs.div) * p.qs.h + tok0 * p.qs.t;
   const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h + tok0 * p.ks.t;
   const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + v0 + tok0 * p.vs.t;
-  float* o_base = STATE_ONLY ? nullptr : p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h + v0;
+  float* o_base = p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h + v0;
 
   if (tid < 16 + LC + 1) pw_pad[tid] = tid < 16 ? 0.f : (float)la_power(l, tid - 16);
 
@@ -264,7 +275,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
 #pragma unroll
     for (int it = 0; it < KN; ++it) {
       const int i = it * RPP + tid / LPR;
-      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], STATE_ONLY ? x.k * (i < n ? pw[n - 1 - i] * x.w : 0.f) : x.k);
+      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], x.k);
     }
 #pragma unroll
     for (int it = 0; it < VN; ++it) lc_put4(sm + L::V_HI, sm + L::V_LO, it * (LC / VN) + (tid >> 4), vc, L::VP, vr[it], x.v);
@@ -276,33 +287,34 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
   };
 
   if (warp < 4) {
-    // ================ outputs: warp w, tokens 16 w .. 16 w + 15 of the chunk ================
-    const int i0 = 16 * w;
+    // ================ outputs: tokens 16 r .. 16 r + 15 of the chunk ================
+    // Later tokens meet more keys.  The two blocks of an SM take the rows in opposite order, so that its four schedulers
+    // get the same share.
+    const int r = (blockIdx.x / sms) & 1 ? 3 - w : w, i0 = 16 * r;
     bool undecayed = p.reverse && seg == 0;            // the incoming state counts in full at the first token
     for (int64_t c0 = first; c0 < n_end; c0 += LC) {
       const int n = (int)min((int64_t)LC, n_end - c0);
       float4 kr[KN], vr[VN], qr[QN];
       load_kv(kr, vr, c0, n);
-      if (!STATE_ONLY) {
+      {
         const float* qp = q + (c0 + tid / LPR) * q_t;
 #pragma unroll
         for (int it = 0; it < QN; ++it, qp += QP * q_t)
           qr[it] = it * QP + tid / LPR < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       Scales x;
-      publish(lc_max<false>(kr), lc_max<false>(vr), STATE_ONLY ? 0.f : lc_max<false>(qr));      // the tiles of the chunk before are free
+      publish(lc_max<false>(kr), lc_max<false>(vr), lc_max<false>(qr));      // the tiles of the chunk before are free
       if (!collect(x, n)) {
         lc_barrier();
-        publish(lc_max<true>(kr), lc_max<true>(vr), STATE_ONLY ? 0.f : lc_max<true>(qr));
+        publish(lc_max<true>(kr), lc_max<true>(vr), lc_max<true>(qr));
         collect(x, n);
       }
       put_kv(kr, vr, x, n);
-      if (!STATE_ONLY) {
+      {
 #pragma unroll
         for (int it = 0; it < QN; ++it) lc_put4(sm + L::Q_HI, sm + L::Q_LO, it * QP + tid / LPR, kc, L::KP, qr[it], x.q);
       }
       lc_barrier();       // all tiles in place
-      if (STATE_ONLY) continue;
       prefetch(q, q_t, dk, c0);
       if (i0 >= n) continue;
       // ---- scores of the tokens up to this warp's, and q S, in one walk over dk
@@ -319,15 +331,18 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
         lc_ldmatrix(ql, lc_smem(sm + L::Q_LO) + qa);
 #pragma unroll
         for (int jt = 0; jt < 4; jt += 2)
-          if (jt <= w) {                                // 32 tokens; their second half may be masked as a whole
+          if (jt <= r) {
             uint32_t bh_[8], bl_[8];
+            const bool both = jt < r;                   // the second 16 tokens of the 32 are not masked as a whole
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
+              if (u == 1 && !both) break;
               const uint32_t ka = lc_at(16 * (jt + u) + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1), L::KP);
               lc_ldmatrix(*reinterpret_cast<uint32_t(*)[4]>(bh_ + 4 * u), lc_smem(sm + L::K_HI) + ka);
               lc_ldmatrix(*reinterpret_cast<uint32_t(*)[4]>(bl_ + 4 * u), lc_smem(sm + L::K_LO) + ka);
             }
-            lc_mma3(P[2 * jt], P[2 * jt + 1], P[2 * jt + 2], P[2 * jt + 3], qh, ql, bh_, bl_);
+            if (both) lc_mma3(P[2 * jt], P[2 * jt + 1], P[2 * jt + 2], P[2 * jt + 3], qh, ql, bh_, bl_);
+            else lc_mma3(P[2 * jt], P[2 * jt + 1], qh, ql, bh_, bl_);
           }
         lc_rows(acc_o, qh, ql, lc_smem(sm + L::S_HI), lc_smem(sm + L::S_LO), 16 * ks, lane, nt_n);
       }
@@ -337,16 +352,16 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
       float m0 = 0.f, m1 = 0.f, b0 = pb[8], b1 = pb[7];
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
-        if (nt < 2 * w + 2) {
+        if (nt < 2 * r + 2) {
           const float a0 = pb[-8 * nt], a1 = pb[-8 * nt - 1];
           P[nt][0] *= a0;
           P[nt][1] *= a1;
           P[nt][2] *= b0;
           P[nt][3] *= b1;
-          if (nt >= 2 * w) {                            // the tiles on the diagonal
+          if (nt >= 2 * r) {                            // the tiles on the diagonal
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (g + (e >> 1) * 8 < 8 * (nt - 2 * w) + t2 + (e & 1)) P[nt][e] = 0.f;
+              if (g + (e >> 1) * 8 < 8 * (nt - 2 * r) + t2 + (e & 1)) P[nt][e] = 0.f;
           }
           m0 = fmaxf(m0, fmaxf(fabsf(P[nt][0]), fabsf(P[nt][1])));
           m1 = fmaxf(m1, fmaxf(fabsf(P[nt][2]), fabsf(P[nt][3])));
@@ -357,7 +372,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
         m0 = m1 = 0.f;
 #pragma unroll
         for (int nt = 0; nt < 8; ++nt)
-          if (nt < 2 * w + 2) {
+          if (nt < 2 * r + 2) {
             m0 = fmaxf(m0, fmaxf(lc_size(P[nt][0]), lc_size(P[nt][1])));
             m1 = fmaxf(m1, fmaxf(lc_size(P[nt][2]), lc_size(P[nt][3])));
           }
@@ -377,7 +392,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
         for (int e = 0; e < 4; ++e) acc_p[nt][e] = 0.f;
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt)
-        if (jt <= w) {
+        if (jt <= r) {
           uint32_t ah[4], al[4];
           lc_split(P[2 * jt][0] * p_s0, P[2 * jt][1] * p_s0, ah[0], al[0]);
           lc_split(P[2 * jt][2] * p_s1, P[2 * jt][3] * p_s1, ah[1], al[1]);
@@ -415,7 +430,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
       }
       undecayed = false;
     }
-    if (!STATE_ONLY && !p.accumulate)       // tokens behind the end of the sequence
+    if (!p.accumulate)       // tokens behind the end of the sequence
       for (int64_t t = max((int64_t)n_all, first); t < limit; ++t)
         for (int j = tid; j < dv; j += 128) o_base[t * p.os.t + j] = 0.f;
     return;
@@ -431,7 +446,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
     for (int nt = 0; nt < 8; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) S[m][nt][e] = 0.f;
-  if (!STATE_ONLY) {
+  {
     const float* s0 = segments > 1 ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : p.s_in ? p.s_in + bh * states : nullptr;
     const bool tr = segments > 1 ? cr.work_t : p.s_in_t;
     if (s0 && tr) {
@@ -466,22 +481,22 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
           }
     }
   }
-  bool undecayed = !STATE_ONLY && p.reverse && seg == 0;
+  bool undecayed = p.reverse && seg == 0;
   for (int64_t c0 = first; c0 < n_end; c0 += LC) {
     const int n = (int)min((int64_t)LC, n_end - c0);
     Scales x;
     {
       float4 kr[KN], vr[VN];
       load_kv(kr, vr, c0, n);
-      publish(lc_max<false>(kr), lc_max<false>(vr), STATE_ONLY ? 0.f : lc_max<false>(S));
+      publish(lc_max<false>(kr), lc_max<false>(vr), lc_max<false>(S));
       if (!collect(x, n)) {
         lc_barrier();
-        publish(lc_max<true>(kr), lc_max<true>(vr), STATE_ONLY ? 0.f : lc_max<true>(S));
+        publish(lc_max<true>(kr), lc_max<true>(vr), lc_max<true>(S));
         collect(x, n);
       }
       put_kv(kr, vr, x, n);
     }
-    if (!STATE_ONLY) {
+    {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -516,7 +531,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
             const uint32_t ka = lc_at(16 * kt + (lane & 7) + ((lane >> 4) << 3), (r0 >> 3) + ((lane >> 3) & 1), L::KP);
             lc_ldmatrix_t(ah, lc_smem(sm + L::K_HI) + ka);
             lc_ldmatrix_t(al, lc_smem(sm + L::K_LO) + ka);
-            if (!STATE_ONLY) {
+            {
 #pragma unroll
               for (int e = 0; e < 2; ++e) {             // tokens 16 kt + 8 e + t2 and the next
                 const int i = n - 1 - (16 * kt + 8 * e + t2);
@@ -540,9 +555,9 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
 
     undecayed = false;
   }
-  float* out = STATE_ONLY ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : segments == 1 && p.s_out ? p.s_out + bh * states : nullptr;
+  float* out = segments == 1 && p.s_out ? p.s_out + bh * states : nullptr;
   if (out) {
-    const float f = (!STATE_ONLY && p.reverse && n_all > 0) ? l : 1.f;
+    const float f = (p.reverse && n_all > 0) ? l : 1.f;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -559,6 +574,136 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
           }
         }
   }
+}
+
+// The state pass: what a segment adds to the state, into work[segment].  Warp: 16-row tiles w and w + 4 of the state, 32 of
+// the 64 columns.  The next chunk's rows are already on their way into registers while the tensor pipe works.
+template <int DK, bool VEC>
+__global__ void __launch_bounds__(LC_THREADS, 2) la_state_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs) {
+  constexpr int KP = DK * 2, VP = LC_COLS * 2, K_LO = LC * KP, V_HI = 2 * LC * KP, V_LO = V_HI + LC * VP;
+  constexpr int MT = DK / 64, LPR = DK / 4, RPP = LC_THREADS / LPR, KN = LC / RPP, VN = LC * 16 / LC_THREADS;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ float pw[LC + 1];
+  __shared__ float red[2][8];
+
+  const LaChunkRun& cr = runs.run[blockIdx.y];
+  const LaRun& p = cr.r;
+  int id = blockIdx.x;
+  const int slab = id % max_slabs;
+  id /= max_slabs;
+  const int seg = id % segments, bh = id / segments;
+  const int slabs = (p.dv + LC_COLS - 1) / LC_COLS;
+  if (slab >= slabs || !cr.state_pass) return;
+  const int b = bh / c.H, h = bh % c.H;
+  const int n_all = la_length(c, b);
+  const int64_t first = (int64_t)seg * seg_tokens, n_end = min((int64_t)n_all, first + seg_tokens);
+  const int width = ((p.dv + slabs - 1) / slabs + 7) & ~7;
+  const int v0 = slab * width, dv = min(width, p.dv - v0), dk = p.dk;
+  const int nt_n = (dv + 7) >> 3;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w = warp & 3, nt0 = 4 * (warp >> 2), g = lane >> 2, t2 = (lane & 3) * 2;
+  const int64_t tok0 = p.reverse ? n_all - 1 : 0;
+  const int64_t k_t = p.reverse ? -p.ks.t : p.ks.t, v_t = p.reverse ? -p.vs.t : p.vs.t;
+  const int kc = (tid % LPR) * 4, vc = (tid & 15) * 4;
+  const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h + (tok0 * p.ks.t + (first + tid / LPR) * k_t);
+  const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + v0 + (tok0 * p.vs.t + (first + (tid >> 4)) * v_t);
+  if (tid <= LC) pw[tid] = (float)la_power(c.decay[h], tid);
+
+  float4 kr[KN], vr[VN];
+  auto load = [&](int64_t c0) {       // rows of the chunk at c0 (a step of this segment); zero behind the end
+    const float* kp = k + (c0 - first) * k_t;
+    const float* vp = v + (c0 - first) * v_t;
+    const int n = (int)max((int64_t)0, min((int64_t)LC, n_end - c0));
+#pragma unroll
+    for (int it = 0; it < KN; ++it, kp += RPP * k_t)
+      kr[it] = it * RPP + tid / LPR < n ? lc_row4<VEC>(kp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int it = 0; it < VN; ++it, vp += LC / VN * v_t)
+      vr[it] = it * (LC / VN) + (tid >> 4) < n ? lc_row4<VEC>(vp, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  float S[MT][4][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[m][nt][e] = 0.f;
+  load(first);
+  for (int64_t c0 = first; c0 < n_end; c0 += LC) {
+    const int n = (int)min((int64_t)LC, n_end - c0);
+    auto publish = [&](float mk, float mv) {
+      mk = warp_max(mk);
+      mv = warp_max(mv);
+      if (lane == 0) {
+        red[0][warp] = mk;
+        red[1][warp] = mv;
+      }
+      __syncthreads();
+    };
+    auto largest = [&](int i) {
+      float m = red[i][0];
+#pragma unroll
+      for (int u = 1; u < 8; ++u) m = fmaxf(m, red[i][u]);
+      return m;
+    };
+    publish(lc_max<false>(kr), lc_max<false>(vr));
+    float mk = largest(0), mv = largest(1);
+    if (fmaxf(mk, mv) == LC_INF) {
+      __syncthreads();
+      publish(lc_max<true>(kr), lc_max<true>(vr));
+      mk = largest(0);
+      mv = largest(1);
+    }
+    float k_inv, v_inv, w_inv = 1.f, w_s = 1.f;
+    const float k_s = lc_scale(mk, &k_inv), v_s = lc_scale(mv, &v_inv), w_max = fabsf(pw[n - 1]);
+    if (w_max > 1.f) {
+      w_s = lc_scale(w_max, &w_inv) * 0x1p-13f;
+      w_inv *= 0x1p13f;
+    }
+#pragma unroll
+    for (int it = 0; it < KN; ++it) {
+      const int i = it * RPP + tid / LPR;
+      lc_put4(sm, sm + K_LO, i, kc, KP, kr[it], i < n ? k_s * (pw[n - 1 - i] * w_s) : 0.f);
+    }
+#pragma unroll
+    for (int it = 0; it < VN; ++it) lc_put4(sm + V_HI, sm + V_LO, it * (LC / VN) + (tid >> 4), vc, VP, vr[it], v_s);
+    __syncthreads();
+    if (c0 + LC < n_end) load(c0 + LC);
+    const float keep = pw[n], f0 = k_inv * w_inv, f1 = v_inv * p.k_scale;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int r0 = 16 * (w + 4 * m);
+      if (r0 < dk && nt0 < nt_n) {
+        float acc[4][4];
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+          if (16 * kt < n) {
+            uint32_t ah[4], al[4];
+            const uint32_t ka = lc_at(16 * kt + (lane & 7) + ((lane >> 4) << 3), (r0 >> 3) + ((lane >> 3) & 1), KP);
+            lc_ldmatrix_t(ah, lc_smem(sm) + ka);
+            lc_ldmatrix_t(al, lc_smem(sm + K_LO) + ka);
+            lc_rows(acc, ah, al, lc_smem(sm + V_HI), lc_smem(sm + V_LO), 16 * kt, lane, nt_n, nt0);
+          }
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[m][nt][e] = keep * S[m][nt][e] + acc[nt][e] * f0 * f1;
+      }
+    }
+  }
+  float* out = cr.work + ((int64_t)seg * c.B * c.H + bh) * ((int64_t)dk * p.dv) + v0;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 16 * (w + 4 * m) + g + (e >> 1) * 8, j = 8 * (nt0 + nt) + t2 + (e & 1);
+        if (i < dk && j < dv) out[(int64_t)i * p.dv + j] = S[m][nt][e];
+      }
 }
 
 // The state through the segments: work[seg] (what segment seg adds) becomes the state before it.
@@ -641,18 +786,19 @@ static int lc_launch(const LaCommon& c, const LaChunkRuns& all, int count, const
   const size_t smem = LcSmem<DK>::BYTES;
   const int64_t blocks = (int64_t)c.B * c.H * p.segments * p.slabs;
   B200_REQUIRE(blocks < (1ll << 31), "linear attention: extent too large");
-  auto main_kernel = vec ? la_chunk_kernel<DK, true, false> : la_chunk_kernel<DK, false, false>;
+  auto main_kernel = vec ? la_chunk_kernel<DK, true> : la_chunk_kernel<DK, false>;
   B200_CUDA(cudaFuncSetAttribute(main_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   if (p.segments > 1) {
-    auto state_kernel = vec ? la_chunk_kernel<DK, true, true> : la_chunk_kernel<DK, false, true>;
-    B200_CUDA(cudaFuncSetAttribute(state_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    state_kernel<<<dim3((unsigned)blocks, (unsigned)count), LC_THREADS, smem, st>>>(c, all, p.segments, p.seg_tokens, p.slabs);
+    auto state_kernel = vec ? la_state_kernel<DK, true> : la_state_kernel<DK, false>;
+    const size_t state_smem = (size_t)4 * LC * (DK + LC_COLS);       // both parts of k and v
+    B200_CUDA(cudaFuncSetAttribute(state_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)state_smem));
+    state_kernel<<<dim3((unsigned)blocks, (unsigned)count), LC_THREADS, state_smem, st>>>(c, all, p.segments, p.seg_tokens, p.slabs);
     B200_LAUNCH_CHECK();
     const int64_t most = (int64_t)all.run[0].r.dk * all.run[0].r.dv;      // the same product for every run
     la_segments_kernel<<<dim3((unsigned)ceil_div(most, 256), (unsigned)((int64_t)c.B * c.H), (unsigned)count), 256, 0, st>>>(c, all, p.segments, p.seg_tokens);
     B200_LAUNCH_CHECK();
   }
-  main_kernel<<<dim3((unsigned)blocks, (unsigned)count), LC_THREADS, smem, st>>>(c, all, p.segments, p.seg_tokens, p.slabs);
+  main_kernel<<<dim3((unsigned)blocks, (unsigned)count), LC_THREADS, smem, st>>>(c, all, p.segments, p.seg_tokens, p.slabs, b200::state().sm_count);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }

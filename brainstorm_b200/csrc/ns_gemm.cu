@@ -489,6 +489,11 @@ static int ns_map(const NsMatrix& a, bool mn, int batch, int rows, CUtensorMap* 
   return B200_OK;
 }
 
+// What the truncating accumulation of a chunk takes from a sum of one sign, on the average.  Measured as the factor that
+// makes five Newton-Schulz steps most exact at seven shapes from 64 x 3000 to 4096 x 4096: the error against 64 bits falls
+// from 2.2 - 4.2e-6 to 0.9 - 2.6e-6 (float32 products: 1.5 - 4.8e-6); a sum without a sign does not notice 2^-22.
+constexpr float NS_GAIN = 1.f + 0x1p-22f;
+
 typedef void (*NsKernel)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, NsOut, int, int, int, int, int, int, int, int*);
 
 int ns_gemm(const NsMatrix& a, bool a_t, const NsMatrix& b, bool b_t, NsMatrix* out, int batch, float alpha, float diagonal, bool symmetric) {
@@ -508,7 +513,7 @@ int ns_gemm(const NsMatrix& a, bool a_t, const NsMatrix& b, bool b_t, NsMatrix* 
   int* flag = device_error_flag();
   B200_REQUIRE(flag != nullptr, "the device error flag cannot be set up");
   const int M = out->rows, N = out->cols, K = a_t ? a.rows : a.cols;
-  const NsOut e = {out->data, out->ld, alpha, diagonal};
+  const NsOut e = {out->data, out->ld, alpha * NS_GAIN, diagonal};
   // the form with the least waves times clocks
   const Form* best = nullptr;
   int64_t least = 0;
