@@ -4,9 +4,9 @@
 //
 //   o_i = sum_{j <= i} l^{i-j} (q_i . k_j) v_j + l^{i+1} q_i S        S' = l^n S + sum_j l^{n-1-j} k_j (x) v_j
 //
-// One block of eight warps walks the chunks of one (sequence, head), or of a segment of them, for up to 64
-// columns of v: four warps for the outputs, four that keep the state in their registers.  All four products run on mma.sync.m16n8k16 in fp32 accuracy:
-// every operand x is scaled by a power of two (per tile, per row for the scores) and split into two
+// One block of four warps walks the chunks of one (sequence, head), or of a segment of them, for up to 64
+// columns of v, with the state in registers.  All four products run on mma.sync.m16n8k16 in fp32 accuracy:
+// every operand x is scaled by a power of two (per tile, per row for q and the scores) and split into two
 // half-precision parts, hi = fp16(x), lo = fp16(x - hi), 22 bits together, and a product is hi.hi + hi.lo +
 // lo.hi.  A value more than 2^17 below the largest of its tile begins to lose bits (the error stays below
 // 2^-39 of that largest value).
@@ -31,7 +31,8 @@ namespace b200 {
 
 constexpr int LC = 64;                // tokens in a chunk
 constexpr int LC_COLS = 64;           // columns of v in a block
-constexpr int LC_THREADS = 256;
+constexpr int LC_THREADS = 128;       // four warps
+constexpr int LS_THREADS = 256;       // of the state pass
 
 struct LaChunkRun {
   LaRun r;
@@ -82,18 +83,18 @@ __device__ __forceinline__ void lc_mma3(float (&c0)[4], float (&c1)[4], const ui
   lc_mma(c0, ah, bh[0], bh[1]);
   lc_mma(c1, ah, bh[2], bh[3]);
 }
-// c (16 x 8 N) += a (16 x 16) b, b the 16 rows from `row` of a tile of 64 columns, from its 8-column tile `first` on; tiles
+// c (16 x 8 N) += a (16 x 16) b, b the 16 rows from `row` of a tile of 64 columns; its 8-column tiles
 // from nt_n on do not count
 template <int N>
 __device__ __forceinline__ void lc_rows(float (&c)[N][4], const uint32_t (&ah)[4], const uint32_t (&al)[4], uint32_t hi, uint32_t lo, int row, int lane,
-                                        int nt_n, int first = 0) {
+                                        int nt_n) {
 #pragma unroll
   for (int nt = 0; nt < N; nt += 4)
-    if (first + nt < nt_n) {
+    if (nt < nt_n) {
       uint32_t bh[8], bl[8];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const uint32_t at = (uint32_t)((row + (lane & 15)) * 128 + (((first + nt + 2 * u + (lane >> 4)) ^ (lane & 7)) << 4));
+        const uint32_t at = (uint32_t)((row + (lane & 15)) * 128 + (((nt + 2 * u + (lane >> 4)) ^ (lane & 7)) << 4));
         lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bh + 4 * u), hi + at);
         lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bl + 4 * u), lo + at);
       }
@@ -162,8 +163,6 @@ __device__ __forceinline__ float lc_max(const float (&x)[M][8][4]) {
     for (int j = 0; j < 8; ++j) m = lc_max4<FINITE>(m, make_float4(x[i][j][0], x[i][j][1], x[i][j][2], x[i][j][3]));
   return m;
 }
-// All threads of the block, from whichever role's code.
-__device__ __forceinline__ void lc_barrier() { asm volatile("bar.sync 0, %0;" ::"n"(LC_THREADS) : "memory"); }
 #define LC_INF __int_as_float(0x7f800000)
 __device__ __forceinline__ void lc_put4(uint8_t* hi, uint8_t* lo, int row, int c, int pitch, float4 x, float s) {
   uint32_t h0, l0, h1, l1;
@@ -181,16 +180,17 @@ struct LcSmem {
                        S_HI = V_LO + LC * VP, S_LO = S_HI + DK * VP, BYTES = S_LO + DK * VP;
 };
 
-// Warps 0 to 3 compute the outputs of 16 tokens each, warps 4 to 7 keep the state, in their registers; all eight
-// load and split the tiles.  DK: 64 or 128, the largest dk the block can hold.  VEC: 128-bit global loads.
+// A warp computes the outputs of 16 tokens of a chunk and keeps a quarter of the state in its registers; all four load and
+// split the tiles.  DK: 64 or 128, the largest dk the block can hold.  VEC: 128-bit global loads.
 template <int DK, bool VEC>
-__global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs, int sms) {
+__global__ void __launch_bounds__(LC_THREADS, DK == 64 ? 3 : 2) la_chunk_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs, int sms) {
   using L = LcSmem<DK>;
-  constexpr int MT = DK / 64;                        // 16-row tiles of the state in a state warp
+  constexpr int MT = DK / 64;                        // 16-row tiles of the state in a warp
   constexpr int LPR = DK / 4, RPP = LC_THREADS / LPR;   // lanes per row of k, rows in a pass
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ float pw_pad[16 + LC + 1];              // powers of the decay, zeros before
-  __shared__ float red[3][8];
+  __shared__ float q_inv[LC];                        // 1 / scale of each row of q
+  __shared__ float red[3][4];
   const float* pw = pw_pad + 16;
 
   const LaChunkRun& cr = runs.run[blockIdx.y];
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
   const int v0 = slab * width, dv = min(width, p.dv - v0), dk = p.dk;
   const int nt_n = (dv + 7) >> 3;                                  // 8-column tiles in use
   const int ks_n = (dk + 15) >> 4;                                 // 16-deep steps over dk
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, w = warp & 3, g = lane >> 2, t2 = (lane & 3) * 2;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t2 = (lane & 3) * 2;
   const float l = c.decay[h];
   const int64_t states = (int64_t)dk * p.dv;
 
@@ -225,98 +225,156 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
   float* o_base = p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h + v0;
 
   if (tid < 16 + LC + 1) pw_pad[tid] = tid < 16 ? 0.f : (float)la_power(l, tid - 16);
-
-  constexpr int KN = LC / RPP, VN = LC * 16 / LC_THREADS;          // passes over k and v
-  constexpr int QP = 128 / LPR, QN = LC / QP;                      // rows of q in a pass of the output warps, passes
+  // Later tokens meet more keys: the blocks of an SM take the rows in opposite order, so that its four schedulers get
+  // about the same share.
+  const int r = (blockIdx.x / sms) & 1 ? 3 - w : w, i0 = 16 * r;      // this warp's tokens
+  constexpr int KN = LC / RPP, VN = LC * 16 / LC_THREADS;             // passes over k (and q) and v
   const int kc = (tid % LPR) * 4, vc = (tid & 15) * 4;
-  auto load_kv = [&](float4 (&kr)[KN], float4 (&vr)[VN], int64_t c0, int n) {
-    const float* kp = k + (c0 + tid / LPR) * k_t;
-    const float* vp = v + (c0 + (tid >> 4)) * v_t;
-#pragma unroll
-    for (int it = 0; it < KN; ++it, kp += RPP * k_t)
-      kr[it] = it * RPP + tid / LPR < n ? lc_row4<VEC>(kp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int it = 0; it < VN; ++it, vp += LC / VN * v_t)
-      vr[it] = it * (LC / VN) + (tid >> 4) < n ? lc_row4<VEC>(vp, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
-  };
-  // The largest magnitudes of the chunk's tiles and of the state; mx is this warp's of q (output warps) or of the state.
-  auto publish = [&](float mk, float mv, float mx) {
-    mk = warp_max(mk);
-    mv = warp_max(mv);
-    mx = warp_max(mx);
-    if (lane == 0) {
-      red[0][warp] = mk;
-      red[1][warp] = mv;
-      red[2][warp] = mx;
-    }
-    lc_barrier();
-  };
-  auto largest4 = [](const float* r) { return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])); };
-  struct Scales {
-    float k, v, q, s, w, k_inv, v_inv, q_inv, s_inv, w_inv;
-  };
-  auto collect = [&](Scales& x, int n) {       // false: an infinity must not decide a scale
-    const float mk = fmaxf(largest4(red[0]), largest4(red[0] + 4)), mv = fmaxf(largest4(red[1]), largest4(red[1] + 4));
-    const float mq = largest4(red[2]), ms = largest4(red[2] + 4);
-    if (fmaxf(fmaxf(mk, mv), fmaxf(mq, ms)) == LC_INF) return false;
-    x.k = lc_scale(mk, &x.k_inv);
-    x.v = lc_scale(mv, &x.v_inv);
-    x.q = lc_scale(mq, &x.q_inv);
-    x.s = lc_scale(ms, &x.s_inv);
-    x.w = x.w_inv = 1.f;
-    const float w_max = fabsf(pw[n - 1]);      // weights above one (a decay above one) are taken back below two
-    if (w_max > 1.f) {
-      x.w = lc_scale(w_max, &x.w_inv) * 0x1p-13f;
-      x.w_inv *= 0x1p13f;
-    }
-    return true;
-  };
-  auto put_kv = [&](const float4 (&kr)[KN], const float4 (&vr)[VN], const Scales& x, int n) {
-#pragma unroll
-    for (int it = 0; it < KN; ++it) {
-      const int i = it * RPP + tid / LPR;
-      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], x.k);
-    }
-#pragma unroll
-    for (int it = 0; it < VN; ++it) lc_put4(sm + L::V_HI, sm + L::V_LO, it * (LC / VN) + (tid >> 4), vc, L::VP, vr[it], x.v);
-  };
   auto prefetch = [&](const float* a, int64_t pitch, int d, int64_t c0) {      // a tile of the next chunk on its way into L2
-    const int x = (tid & 1) * 32, i = (tid & 127) >> 1;
+    const int x = (tid & 1) * 32, i = tid >> 1;
     if (c0 + LC + i < n_end)
       for (int e = x; e < d; e += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(a + (c0 + LC + i) * pitch + e));
   };
 
-  if (warp < 4) {
-    // ================ outputs: tokens 16 r .. 16 r + 15 of the chunk ================
-    // Later tokens meet more keys.  The two blocks of an SM take the rows in opposite order, so that its four schedulers
-    // get the same share.
-    const int r = (blockIdx.x / sms) & 1 ? 3 - w : w, i0 = 16 * r;
-    bool undecayed = p.reverse && seg == 0;            // the incoming state counts in full at the first token
-    for (int64_t c0 = first; c0 < n_end; c0 += LC) {
-      const int n = (int)min((int64_t)LC, n_end - c0);
-      float4 kr[KN], vr[VN], qr[QN];
-      load_kv(kr, vr, c0, n);
-      {
-        const float* qp = q + (c0 + tid / LPR) * q_t;
+  // the state: 16-row tiles w and w + 4 (rows 16 (w + 4 m) + g and + 8), columns 8 nt + t2, t2 + 1
+  auto row_of = [&](int m, int e) { return 16 * (w + 4 * m) + g + (e >> 1) * 8; };
+  auto col_of = [&](int nt, int e) { return 8 * nt + t2 + (e & 1); };
+  float S[MT][8][4];
 #pragma unroll
-        for (int it = 0; it < QN; ++it, qp += QP * q_t)
-          qr[it] = it * QP + tid / LPR < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      Scales x;
-      publish(lc_max<false>(kr), lc_max<false>(vr), lc_max<false>(qr));      // the tiles of the chunk before are free
-      if (!collect(x, n)) {
-        lc_barrier();
-        publish(lc_max<true>(kr), lc_max<true>(vr), lc_max<true>(qr));
-        collect(x, n);
-      }
-      put_kv(kr, vr, x, n);
-      {
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int it = 0; it < QN; ++it) lc_put4(sm + L::Q_HI, sm + L::Q_LO, it * QP + tid / LPR, kc, L::KP, qr[it], x.q);
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[m][nt][e] = 0.f;
+  {
+    const float* s0 = segments > 1 ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : p.s_in ? p.s_in + bh * states : nullptr;
+    const bool tr = segments > 1 ? cr.work_t : p.s_in_t;
+    if (s0 && tr) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = row_of(m, e), j = col_of(nt, e);
+            if (i < dk && j < dv) S[m][nt][e] = s0[(int64_t)(v0 + j) * dk + i];
+          }
+    } else if (s0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const int i = row_of(m, e), j = col_of(nt, e);
+            const float* at = s0 + (int64_t)i * p.dv + v0 + j;
+            if (VEC) {
+              if (i < dk && j < dv) {
+                const float2 x = *reinterpret_cast<const float2*>(at);
+                S[m][nt][e] = x.x;
+                S[m][nt][e + 1] = x.y;
+              }
+            } else {
+              if (i < dk && j < dv) S[m][nt][e] = at[0];
+              if (i < dk && j + 1 < dv) S[m][nt][e + 1] = at[1];
+            }
+          }
+    }
+  }
+  bool undecayed = p.reverse && seg == 0;            // the incoming state counts in full at the first token
+
+  for (int64_t c0 = first; c0 < n_end; c0 += LC) {
+    const int n = (int)min((int64_t)LC, n_end - c0);
+    float4 kr[KN], vr[VN];
+    {
+      const float* kp = k + (c0 + tid / LPR) * k_t;
+      const float* vp = v + (c0 + (tid >> 4)) * v_t;
+#pragma unroll
+      for (int it = 0; it < KN; ++it, kp += RPP * k_t)
+        kr[it] = it * RPP + tid / LPR < n ? lc_row4<VEC>(kp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int it = 0; it < VN; ++it, vp += LC / VN * v_t)
+        vr[it] = it * (LC / VN) + (tid >> 4) < n ? lc_row4<VEC>(vp, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // ---- with dk up to 64 the registers hold q as well; else it follows in halves
+    constexpr int QN = DK == 64 ? KN : KN / 2;
+    float4 qr[QN];
+    auto load_q = [&](int it0) {
+      const float* qp = q + (c0 + it0 * RPP + tid / LPR) * q_t;
+#pragma unroll
+      for (int it = 0; it < QN; ++it, qp += RPP * q_t)
+        qr[it] = (it0 + it) * RPP + tid / LPR < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    auto put_q = [&](int it0) {      // each row by its own scale: a row lies in LPR neighbouring lanes
+#pragma unroll
+      for (int it = 0; it < QN; ++it) {
+        const int i = (it0 + it) * RPP + tid / LPR;
+        float m = lc_max4<false>(0.f, qr[it]), inv;
+        if (__any_sync(0xffffffffu, m == LC_INF)) m = lc_max4<true>(0.f, qr[it]);
+#pragma unroll
+        for (int s = 1; s < LPR; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+        const float sc = lc_scale(m, &inv);
+        lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, kc, L::KP, qr[it], sc);
+        if (tid % LPR == 0) q_inv[i] = inv;
       }
-      lc_barrier();       // all tiles in place
-      prefetch(q, q_t, dk, c0);
-      if (i0 >= n) continue;
+    };
+    if (DK == 64) load_q(0);
+    auto publish = [&](float mk, float mv, float ms) {
+      mk = warp_max(mk);
+      mv = warp_max(mv);
+      ms = warp_max(ms);
+      if (lane == 0) {
+        red[0][w] = mk;
+        red[1][w] = mv;
+        red[2][w] = ms;
+      }
+      __syncthreads();
+    };
+    auto largest = [&](int i) { return fmaxf(fmaxf(red[i][0], red[i][1]), fmaxf(red[i][2], red[i][3])); };
+    publish(lc_max<false>(kr), lc_max<false>(vr), lc_max<false>(S));      // behind it the tiles of the chunk before are free
+    if (fmaxf(fmaxf(largest(0), largest(1)), largest(2)) == LC_INF) {      // an infinity must not decide a scale
+      __syncthreads();
+      publish(lc_max<true>(kr), lc_max<true>(vr), lc_max<true>(S));
+    }
+    struct {
+      float k, v, s, w, k_inv, v_inv, s_inv, w_inv;
+    } x;
+    x.k = lc_scale(largest(0), &x.k_inv);
+    x.v = lc_scale(largest(1), &x.v_inv);
+    x.s = lc_scale(largest(2), &x.s_inv);
+    x.w = x.w_inv = 1.f;
+    const float w_max = fabsf(pw[n - 1]);              // weights above one (a decay above one) are taken back below two
+    if (w_max > 1.f) {
+      x.w = lc_scale(w_max, &x.w_inv) * 0x1p-13f;
+      x.w_inv *= 0x1p13f;
+    }
+#pragma unroll
+    for (int it = 0; it < KN; ++it) lc_put4(sm + L::K_HI, sm + L::K_LO, it * RPP + tid / LPR, kc, L::KP, kr[it], x.k);
+#pragma unroll
+    for (int it = 0; it < VN; ++it) lc_put4(sm + L::V_HI, sm + L::V_LO, it * (LC / VN) + (tid >> 4), vc, L::VP, vr[it], x.v);
+    if (DK != 64) load_q(0);
+    put_q(0);
+    if (DK != 64) {
+      load_q(QN);
+      put_q(QN);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          uint32_t hi, lo;
+          lc_split(S[m][nt][e] * x.s, S[m][nt][e + 1] * x.s, hi, lo);
+          const uint32_t at = lc_at(row_of(m, e), nt, L::VP) + t2 * 2;
+          *reinterpret_cast<uint32_t*>(sm + L::S_HI + at) = hi;
+          *reinterpret_cast<uint32_t*>(sm + L::S_LO + at) = lo;
+        }
+    __syncthreads();      // all tiles in place
+    prefetch(k, k_t, dk, c0);
+    prefetch(q, q_t, dk, c0);
+    prefetch(v, v_t, dv, c0);
+    if (i0 < n) {
       // ---- scores of the tokens up to this warp's, and q S, in one walk over dk
       float P[8][4], acc_o[8][4];
 #pragma unroll
@@ -406,8 +464,8 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
         const int i = i0 + g + 8 * half;
         if (i < n) {
           // the factors one after the other where their product could leave the range of float32
-          const float f_o0 = x.s_inv * x.q_inv, f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
-          const float f_p0 = (half ? p_inv1 : p_inv0) * x.v_inv, f_p1 = x.q_inv * x.k_inv * (p.o_scale * p.k_scale);
+          const float f_o0 = x.s_inv * q_inv[i], f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
+          const float f_p0 = (half ? p_inv1 : p_inv0) * x.v_inv, f_p1 = q_inv[i] * x.k_inv * (p.o_scale * p.k_scale);
           float* row = o_base + (tok0 * p.os.t + (c0 + i) * o_t);
           if (VEC && !p.accumulate) {
 #pragma unroll
@@ -428,92 +486,8 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
           }
         }
       }
-      undecayed = false;
     }
-    if (!p.accumulate)       // tokens behind the end of the sequence
-      for (int64_t t = max((int64_t)n_all, first); t < limit; ++t)
-        for (int j = tid; j < dv; j += 128) o_base[t * p.os.t + j] = 0.f;
-    return;
-  }
-
-  // ================ the state: warp w, 16-row tiles w and w + 4 (rows 16 (w + 4 m) + g and + 8), columns 8 nt + t2, t2 + 1 ================
-  auto row_of = [&](int m, int e) { return 16 * (w + 4 * m) + g + (e >> 1) * 8; };
-  auto col_of = [&](int nt, int e) { return 8 * nt + t2 + (e & 1); };
-  float S[MT][8][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) S[m][nt][e] = 0.f;
-  {
-    const float* s0 = segments > 1 ? cr.work + ((int64_t)seg * c.B * c.H + bh) * states : p.s_in ? p.s_in + bh * states : nullptr;
-    const bool tr = segments > 1 ? cr.work_t : p.s_in_t;
-    if (s0 && tr) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = row_of(m, e), j = col_of(nt, e);
-            if (i < dk && j < dv) S[m][nt][e] = s0[(int64_t)(v0 + j) * dk + i];
-          }
-    } else if (s0) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const int i = row_of(m, e), j = col_of(nt, e);
-            const float* at = s0 + (int64_t)i * p.dv + v0 + j;
-            if (VEC) {
-              if (i < dk && j < dv) {
-                const float2 x = *reinterpret_cast<const float2*>(at);
-                S[m][nt][e] = x.x;
-                S[m][nt][e + 1] = x.y;
-              }
-            } else {
-              if (i < dk && j < dv) S[m][nt][e] = at[0];
-              if (i < dk && j + 1 < dv) S[m][nt][e + 1] = at[1];
-            }
-          }
-    }
-  }
-  bool undecayed = p.reverse && seg == 0;
-  for (int64_t c0 = first; c0 < n_end; c0 += LC) {
-    const int n = (int)min((int64_t)LC, n_end - c0);
-    Scales x;
-    {
-      float4 kr[KN], vr[VN];
-      load_kv(kr, vr, c0, n);
-      publish(lc_max<false>(kr), lc_max<false>(vr), lc_max<false>(S));
-      if (!collect(x, n)) {
-        lc_barrier();
-        publish(lc_max<true>(kr), lc_max<true>(vr), lc_max<true>(S));
-        collect(x, n);
-      }
-      put_kv(kr, vr, x, n);
-    }
-    {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            uint32_t hi, lo;
-            lc_split(S[m][nt][e] * x.s, S[m][nt][e + 1] * x.s, hi, lo);
-            const uint32_t at = lc_at(row_of(m, e), nt, L::VP) + t2 * 2;
-            *reinterpret_cast<uint32_t*>(sm + L::S_HI + at) = hi;
-            *reinterpret_cast<uint32_t*>(sm + L::S_LO + at) = lo;
-          }
-    }
-    lc_barrier();         // all tiles in place
-    prefetch(k, k_t, dk, c0);
-    prefetch(v, v_t, dv, c0);
-    // each element of k is met once here and takes its weight on the way
+    // ---- the state after the chunk; each element of k is met once here and takes its weight on the way
     const float keep = pw[n - (undecayed ? 1 : 0)];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -552,9 +526,11 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
           for (int e = 0; e < 4; ++e) S[m][nt][e] = keep * S[m][nt][e] + acc[nt][e] * f0 * f1;
       }
     }
-
     undecayed = false;
   }
+  if (!p.accumulate)       // tokens behind the end of the sequence
+    for (int64_t t = max((int64_t)n_all, first); t < limit; ++t)
+      for (int j = tid; j < dv; j += LC_THREADS) o_base[t * p.os.t + j] = 0.f;
   float* out = segments == 1 && p.s_out ? p.s_out + bh * states : nullptr;
   if (out) {
     const float f = (p.reverse && n_all > 0) ? l : 1.f;
@@ -579,9 +555,9 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_chunk_kernel(LaCommon c, LaC
 // The state pass: what a segment adds to the state, into work[segment].  Warp: 16-row tiles w and w + 4 of the state, 32 of
 // the 64 columns.  The next chunk's rows are already on their way into registers while the tensor pipe works.
 template <int DK, bool VEC>
-__global__ void __launch_bounds__(LC_THREADS, 2) la_state_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs) {
+__global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaChunkRuns runs, int segments, int seg_tokens, int max_slabs) {
   constexpr int KP = DK * 2, VP = LC_COLS * 2, K_LO = LC * KP, V_HI = 2 * LC * KP, V_LO = V_HI + LC * VP;
-  constexpr int MT = DK / 64, LPR = DK / 4, RPP = LC_THREADS / LPR, KN = LC / RPP, VN = LC * 16 / LC_THREADS;
+  constexpr int MT = DK / 64, LPR = DK / 4, RPP = LS_THREADS / LPR, KN = LC / RPP, VN = LC * 16 / LS_THREADS;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ float pw[LC + 1];
   __shared__ float red[2][8];
@@ -620,7 +596,7 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_state_kernel(LaCommon c, LaC
     for (int it = 0; it < VN; ++it, vp += LC / VN * v_t)
       vr[it] = it * (LC / VN) + (tid >> 4) < n ? lc_row4<VEC>(vp, vc, dv) : make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  float S[MT][4][4];
+  float S[MT][4][4], acc[MT][4][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -669,29 +645,40 @@ __global__ void __launch_bounds__(LC_THREADS, 2) la_state_kernel(LaCommon c, LaC
     __syncthreads();
     if (c0 + LC < n_end) load(c0 + LC);
     const float keep = pw[n], f0 = k_inv * w_inv, f1 = v_inv * p.k_scale;
+    if (nt0 < nt_n) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int r0 = 16 * (w + 4 * m);
-      if (r0 < dk && nt0 < nt_n) {
-        float acc[4][4];
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
+          for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.f;
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-          if (16 * kt < n) {
+      for (int kt = 0; kt < 4; ++kt)
+        if (16 * kt < n) {
+          uint32_t bh[8], bl[8];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t va = lc_at(16 * kt + (lane & 15), nt0 + 2 * u + (lane >> 4), VP);
+            lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bh + 4 * u), lc_smem(sm + V_HI) + va);
+            lc_ldmatrix_t(*reinterpret_cast<uint32_t(*)[4]>(bl + 4 * u), lc_smem(sm + V_LO) + va);
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const int r0 = 16 * (w + 4 * m);
+            if (r0 >= dk) continue;
             uint32_t ah[4], al[4];
             const uint32_t ka = lc_at(16 * kt + (lane & 7) + ((lane >> 4) << 3), (r0 >> 3) + ((lane >> 3) & 1), KP);
             lc_ldmatrix_t(ah, lc_smem(sm) + ka);
             lc_ldmatrix_t(al, lc_smem(sm + K_LO) + ka);
-            lc_rows(acc, ah, al, lc_smem(sm + V_HI), lc_smem(sm + V_LO), 16 * kt, lane, nt_n, nt0);
+            lc_mma3(acc[m][0], acc[m][1], acc[m][2], acc[m][3], ah, al, bh, bl);
           }
+        }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) S[m][nt][e] = keep * S[m][nt][e] + acc[nt][e] * f0 * f1;
-      }
+          for (int e = 0; e < 4; ++e) S[m][nt][e] = keep * S[m][nt][e] + acc[m][nt][e] * f0 * f1;
     }
   }
   float* out = cr.work + ((int64_t)seg * c.B * c.H + bh) * ((int64_t)dk * p.dv) + v0;
@@ -769,7 +756,7 @@ static LcPlan lc_plan(int64_t T, int64_t BH, int dk, int dv_max, int count) {
   LcPlan p;
   p.dk = dk <= 64 ? 64 : 128;
   p.slabs = (int)ceil_div(dv_max, LC_COLS);
-  p.segments = lc_segments(T, BH * p.slabs * count, state().sm_count * 2);
+  p.segments = lc_segments(T, BH * p.slabs * count, state().sm_count * (p.dk == 64 ? 3 : 2));
   p.seg_tokens = (int)(ceil_div(ceil_div(T, LC), p.segments) * LC);
   p.segments = (int)ceil_div(T, p.seg_tokens);
   return p;
@@ -792,7 +779,7 @@ static int lc_launch(const LaCommon& c, const LaChunkRuns& all, int count, const
     auto state_kernel = vec ? la_state_kernel<DK, true> : la_state_kernel<DK, false>;
     const size_t state_smem = (size_t)4 * LC * (DK + LC_COLS);       // both parts of k and v
     B200_CUDA(cudaFuncSetAttribute(state_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)state_smem));
-    state_kernel<<<dim3((unsigned)blocks, (unsigned)count), LC_THREADS, state_smem, st>>>(c, all, p.segments, p.seg_tokens, p.slabs);
+    state_kernel<<<dim3((unsigned)blocks, (unsigned)count), LS_THREADS, state_smem, st>>>(c, all, p.segments, p.seg_tokens, p.slabs);
     B200_LAUNCH_CHECK();
     const int64_t most = (int64_t)all.run[0].r.dk * all.run[0].r.dv;      // the same product for every run
     la_segments_kernel<<<dim3((unsigned)ceil_div(most, 256), (unsigned)((int64_t)c.B * c.H), (unsigned)count), 256, 0, st>>>(c, all, p.segments, p.seg_tokens);
