@@ -18,6 +18,8 @@
 //
 // Bound: HBM.  Forward moves 5 arrays, backward 8.
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 #include "common.cuh"
 
@@ -60,47 +62,77 @@ __device__ __forceinline__ float gn_act_deriv(int act, float a) {
   }
 }
 
-// A row is held by G threads (a power of two, 32 .. 1024), E floats each: VEC = 4: float4 number
-// i * G + t of the row, VEC = 1: float number i * G + t.
-template <int E, int VEC>
-__device__ __forceinline__ void gn_load(float (&v)[E], const float* row, int width, int G, int t) {
+// A row is held by G threads (a power of two, 32 .. 1024), E floats each.  MODE
+//   GN_SINGLE: float number i * G + t of the row, one at a time;
+//   GN_VEC:    float4 number i * G + t; all rows start on 16 bytes and hold a multiple of 4;
+//   GN_SHIFT:  any width and start, all arrays alike: float4 number i * G + t counted from the 16-byte boundary at or
+//              before the row, `off` floats (0 .. 3) ahead of it.  A thread meets rows of one `off` only (their distance is
+//              a multiple of 4 rows), so its columns stay the same: column c of slot (i, j) is 4 (i G + t) + j - off.
+enum { GN_SINGLE = 0, GN_VEC = 1, GN_SHIFT = 2 };
+template <int MODE>
+__device__ __forceinline__ int gn_column(int e, int G, int t, int off) {
+  return MODE == GN_SINGLE ? e * G + t : 4 * ((e / 4) * G + t) + e % 4 - (MODE == GN_SHIFT ? off : 0);
+}
+template <int E, int MODE>
+__device__ __forceinline__ void gn_load(float (&v)[E], const float* row, int width, int G, int t, int off) {
+  if (MODE == GN_SINGLE) {
 #pragma unroll
-  for (int i = 0; i < E / VEC; ++i) {
-    const int c = (i * G + t) * VEC;
-    if (VEC == 4) {
-      const float4 q = c < width ? *reinterpret_cast<const float4*>(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
-    } else {
-      v[i] = c < width ? row[c] : 0.f;
+    for (int e = 0; e < E; ++e) v[e] = e * G + t < width ? row[e * G + t] : 0.f;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < E / 4; ++i) {
+    const int c = gn_column<MODE>(4 * i, G, t, off);
+    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (MODE == GN_VEC ? c < width : c >= 0 && c + 4 <= width) {
+      q = *reinterpret_cast<const float4*>(row + c);
+    } else if (MODE == GN_SHIFT && c < width) {          // the ends of the row
+      if (c >= 0) q.x = row[c];
+      if (c + 1 >= 0 && c + 1 < width) q.y = row[c + 1];
+      if (c + 2 >= 0 && c + 2 < width) q.z = row[c + 2];
+      if (c + 3 >= 0 && c + 3 < width) q.w = row[c + 3];
+    }
+    v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+  }
+}
+template <int E, int MODE>
+__device__ __forceinline__ void gn_store(const float (&v)[E], float* row, int width, int G, int t, int off) {
+  if (MODE == GN_SINGLE) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e * G + t < width) row[e * G + t] = v[e];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < E / 4; ++i) {
+    const int c = gn_column<MODE>(4 * i, G, t, off);
+    if (MODE == GN_VEC ? c < width : c >= 0 && c + 4 <= width) {
+      *reinterpret_cast<float4*>(row + c) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else if (MODE == GN_SHIFT && c < width) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j >= 0 && c + j < width) row[c + j] = v[4 * i + j];
     }
   }
 }
-template <int E, int VEC>
-__device__ __forceinline__ void gn_store(const float (&v)[E], float* row, int width, int G, int t) {
+template <int E, int MODE>
+__device__ __forceinline__ void gn_add(float (&v)[E], const float* row, int width, int G, int t, int off) {
+  float o[E];
+  gn_load<E, MODE>(o, row, width, G, t, off);
 #pragma unroll
-  for (int i = 0; i < E / VEC; ++i) {
-    const int c = (i * G + t) * VEC;
-    if (c < width) {
-      if (VEC == 4) *reinterpret_cast<float4*>(row + c) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      else row[c] = v[i];
-    }
-  }
-}
-template <int E, int VEC>
-__device__ __forceinline__ void gn_add(float (&v)[E], const float* row, int width, int G, int t) {
-#pragma unroll
-  for (int i = 0; i < E / VEC; ++i) {
-    const int c = (i * G + t) * VEC;
-    if (c < width)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[VEC * i + j] = row[c + j] + v[VEC * i + j];
-  }
+  for (int e = 0; e < E; ++e) v[e] = o[e] + v[e];
 }
 // The weights of this thread's columns; ones where there is no vector.
-template <int E, int VEC>
-__device__ __forceinline__ void gn_weights(float (&v)[E], const float* w, int width, int G, int t) {
-  if (w) {
-    gn_load<E, VEC>(v, w, width, G, t);
+template <int E, int MODE>
+__device__ __forceinline__ void gn_weights(float (&v)[E], const float* w, int width, int G, int t, int off) {
+  if (w && MODE == GN_SHIFT) {         // the vectors do not start like the rows
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = gn_column<MODE>(e, G, t, off);
+      v[e] = c >= 0 && c < width ? __ldg(w + c) : 0.f;
+    }
+  } else if (w) {
+    gn_load<E, MODE>(v, w, width, G, t, 0);
   } else {
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 1.f;
@@ -154,11 +186,28 @@ __device__ __forceinline__ float gn_row_sum(float v, int G, float* smem) {
   return s;
 }
 
-template <int E, int VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_forward_kernel(GatedNorm p, int G) {
+template <int E, int MODE, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) gated_norm_forward_kernel(GatedNorm p, int G) {
+  constexpr bool KEEP = MODE == GN_SHIFT;      // the weights in registers: their loads are single
   __shared__ float red[32];
   const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
   const float inv_width = 1.f / (float)p.width;
+  const int64_t row_first = (int64_t)blockIdx.x * per_block + threadIdx.x / G;
+  const int off = MODE == GN_SHIFT ? (int)((reinterpret_cast<uintptr_t>(p.x + row_first * p.ld_x) >> 2) & 3) : 0;
+  float w_post[KEEP ? E : 1], w_scale[KEEP ? E : 1], w_pre[KEEP ? E : 1];
+  if constexpr (KEEP) {
+    gn_weights<E, MODE>(w_post, p.w_post, p.width, G, t, off);
+    gn_weights<E, MODE>(w_scale, p.scale, p.width, G, t, off);
+    gn_weights<E, MODE>(w_pre, p.w_pre, p.width, G, t, off);
+  }
+  auto weights = [&](float (&v)[E], const float* from, const float* kept) {
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = kept[e];
+    } else {
+      gn_weights<E, MODE>(v, from, p.width, G, t, off);
+    }
+  };
   for (int64_t row0 = (int64_t)blockIdx.x * per_block; row0 < p.rows; row0 += (int64_t)gridDim.x * per_block) {
     const int64_t row = row0 + threadIdx.x / G;
     const bool live = row < p.rows;
@@ -166,10 +215,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_fo
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = y[e] = g[e] = 0.f;
     if (live) {
-      gn_load<E, VEC>(x, p.x + row * p.ld_x, p.width, G, t);
+      gn_load<E, MODE>(x, p.x + row * p.ld_x, p.width, G, t, off);
       if (p.y) {
-        gn_load<E, VEC>(y, p.y + row * p.ld_y, p.width, G, t);
-        if (p.gate) gn_load<E, VEC>(g, p.gate + row * p.ld_gate, p.width, G, t);
+        gn_load<E, MODE>(y, p.y + row * p.ld_y, p.width, G, t, off);
+        if (p.gate) gn_load<E, MODE>(g, p.gate + row * p.ld_gate, p.width, G, t, off);
+      }
+      const int64_t next = row + (int64_t)gridDim.x * per_block;
+      if (next < p.rows) {
+        gn_prefetch(p.x + next * p.ld_x, p.width, G, t);
+        if (p.y) gn_prefetch(p.y + next * p.ld_y, p.width, G, t);
+        if (p.gate) gn_prefetch(p.gate + next * p.ld_gate, p.width, G, t);
       }
     }
     if (p.y) {
@@ -185,19 +240,19 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_fo
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] *= r;
       }
-      gn_weights<E, VEC>(g, p.w_post, p.width, G, t);
+      weights(g, p.w_post, w_post);
 #pragma unroll
       for (int e = 0; e < E; ++e) y[e] *= g[e];
-      gn_weights<E, VEC>(g, p.scale, p.width, G, t);
+      weights(g, p.scale, w_scale);
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] += y[e] * g[e];
       if (live) {
-        gn_store<E, VEC>(x, p.x_out + row * p.ld_x_out, p.width, G, t);
+        gn_store<E, MODE>(x, p.x_out + row * p.ld_x_out, p.width, G, t, off);
         if (t == 0 && p.r_post) p.r_post[row] = r;
       }
     }
     if (p.h_out) {
-      gn_weights<E, VEC>(g, p.w_pre, p.width, G, t);
+      weights(g, p.w_pre, w_pre);
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) s += x[e] * x[e];
@@ -205,7 +260,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_fo
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = x[e] * r * g[e];
       if (live) {
-        gn_store<E, VEC>(x, p.h_out + row * p.ld_h_out, p.width, G, t);
+        gn_store<E, MODE>(x, p.h_out + row * p.ld_h_out, p.width, G, t, off);
         if (t == 0 && p.r_pre) p.r_pre[row] = r;
       }
     }
@@ -213,8 +268,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) gated_norm_fo
 }
 
 // Shared memory: three vectors of column sums for each group of G threads (gn_sum_into).
-template <int E, int VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_backward_kernel(GatedNormGrad p, int G) {
+template <int E, int MODE, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 2 : 3) gated_norm_backward_kernel(GatedNormGrad p, int G) {
+  constexpr bool KEEP = MODE == GN_SHIFT;
   extern __shared__ float4 sums[];
   __shared__ float red[32];
   const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
@@ -224,6 +280,22 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
 #pragma unroll
   for (int i = 0; i < E / 4; ++i) s_post[i * blockDim.x] = s_scale[i * blockDim.x] = s_pre[i * blockDim.x] = make_float4(0.f, 0.f, 0.f, 0.f);
   const float inv_width = 1.f / (float)p.width;
+  const int64_t row_first = (int64_t)blockIdx.x * per_block + threadIdx.x / G;
+  const int off = MODE == GN_SHIFT ? (int)((reinterpret_cast<uintptr_t>(p.dx + row_first * p.ld_dx) >> 2) & 3) : 0;
+  float w_post[KEEP ? E : 1], w_scale[KEEP ? E : 1], w_pre[KEEP ? E : 1];
+  if constexpr (KEEP) {
+    gn_weights<E, MODE>(w_post, p.w_post, p.width, G, t, off);
+    gn_weights<E, MODE>(w_scale, p.scale, p.width, G, t, off);
+    gn_weights<E, MODE>(w_pre, p.w_pre, p.width, G, t, off);
+  }
+  auto weights = [&](float (&v)[E], const float* from, const float* kept) {
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = kept[e];
+    } else {
+      gn_weights<E, MODE>(v, from, p.width, G, t, off);
+    }
+  };
   for (int64_t row0 = (int64_t)blockIdx.x * per_block; row0 < p.rows; row0 += (int64_t)gridDim.x * per_block) {
     const int64_t row = row0 + threadIdx.x / G;
     const bool live = row < p.rows;
@@ -233,14 +305,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
     float r_pre = 0.f, r_post = 0.f;
     if (live) {
       if (p.dh) {
-        gn_load<E, VEC>(h, p.dh + row * p.ld_dh, p.width, G, t);
-        gn_load<E, VEC>(x, p.x_out + row * p.ld_x_out, p.width, G, t);
+        gn_load<E, MODE>(h, p.dh + row * p.ld_dh, p.width, G, t, off);
+        gn_load<E, MODE>(x, p.x_out + row * p.ld_x_out, p.width, G, t, off);
         r_pre = p.r_pre[row];
       }
-      if (p.dx_out) gn_load<E, VEC>(d, p.dx_out + row * p.ld_dx_out, p.width, G, t);
+      if (p.dx_out) gn_load<E, MODE>(d, p.dx_out + row * p.ld_dx_out, p.width, G, t, off);
       if (p.y) {
-        gn_load<E, VEC>(y, p.y + row * p.ld_y, p.width, G, t);
-        if (p.gate) gn_load<E, VEC>(g, p.gate + row * p.ld_gate, p.width, G, t);
+        gn_load<E, MODE>(y, p.y + row * p.ld_y, p.width, G, t, off);
+        if (p.gate) gn_load<E, MODE>(g, p.gate + row * p.ld_gate, p.width, G, t, off);
         r_post = p.r_post[row];
       }
       const int64_t next = row + (int64_t)gridDim.x * per_block;
@@ -262,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
         w[e] = h[e] * x[e];
       }
       gn_sum_into<E>(s_pre, w);
-      gn_weights<E, VEC>(w, p.w_pre, p.width, G, t);
+      weights(w, p.w_pre, w_pre);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         h[e] *= w[e];
@@ -277,10 +349,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
         float o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = d[e];
-        gn_add<E, VEC>(o, p.dx + row * p.ld_dx, p.width, G, t);
-        gn_store<E, VEC>(o, p.dx + row * p.ld_dx, p.width, G, t);
+        gn_add<E, MODE>(o, p.dx + row * p.ld_dx, p.width, G, t, off);
+        gn_store<E, MODE>(o, p.dx + row * p.ld_dx, p.width, G, t, off);
       } else {
-        gn_store<E, VEC>(d, p.dx + row * p.ld_dx, p.width, G, t);
+        gn_store<E, MODE>(d, p.dx + row * p.ld_dx, p.width, G, t, off);
       }
     }
     if (p.y) {
@@ -289,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = p.gate ? g[e] : 1.f;
       if (p.gate) gn_act_all<E>(p.act, x);
-      gn_weights<E, VEC>(w, p.w_post, p.width, G, t);
+      weights(w, p.w_post, w_post);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         y[e] *= r_post;
@@ -297,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
         g[e] = d[e] * x[e] * h[e];
       }
       gn_sum_into<E>(s_scale, g);
-      gn_weights<E, VEC>(g, p.scale, p.width, G, t);
+      weights(g, p.scale, w_scale);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         d[e] *= g[e];                                             // G scale
@@ -321,22 +393,35 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
 #pragma unroll
       for (int e = 0; e < E; ++e) d[e] = r_post * (d[e] - y[e] * m);
       if (live) {
-        if (p.accumulate) gn_add<E, VEC>(d, p.dy + row * p.ld_dy, p.width, G, t);
-        gn_store<E, VEC>(d, p.dy + row * p.ld_dy, p.width, G, t);
+        if (p.accumulate) gn_add<E, MODE>(d, p.dy + row * p.ld_dy, p.width, G, t, off);
+        gn_store<E, MODE>(d, p.dy + row * p.ld_dy, p.width, G, t, off);
         if (p.gate) {
-          if (p.accumulate) gn_add<E, VEC>(g, p.dgate + row * p.ld_dgate, p.width, G, t);
-          gn_store<E, VEC>(g, p.dgate + row * p.ld_dgate, p.width, G, t);
+          if (p.accumulate) gn_add<E, MODE>(g, p.dgate + row * p.ld_dgate, p.width, G, t, off);
+          gn_store<E, MODE>(g, p.dgate + row * p.ld_dgate, p.width, G, t, off);
         }
       }
     }
   }
   if (!p.partials) return;
+  if (MODE == GN_SHIFT) {       // each group's columns are its own: a row of partial sums for each
+    if (row_first >= p.rows) return;
+    float* out = p.partials + row_first * 3 * p.width;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = gn_column<MODE>(e, G, t, off);
+      if (c < 0 || c >= p.width) continue;
+      out[c] = reinterpret_cast<const float*>(s_post + e / 4 * blockDim.x)[e % 4];
+      out[p.width + c] = reinterpret_cast<const float*>(s_scale + e / 4 * blockDim.x)[e % 4];
+      out[2 * p.width + c] = reinterpret_cast<const float*>(s_pre + e / 4 * blockDim.x)[e % 4];
+    }
+    return;
+  }
   __syncthreads();
   if (threadIdx.x < G) {      // the groups of the block, in order
     float* out = p.partials + (int64_t)blockIdx.x * 3 * p.width;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = ((e / VEC) * G + t) * VEC + e % VEC;
+      const int c = gn_column<MODE>(e, G, t, 0);
       if (c >= p.width) continue;
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
@@ -350,23 +435,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) gated_norm_ba
 }
 
 // out[c] (+)= sum over the partial rows of column c, for the three vectors laid side by side.  32
-// columns x 8 slices of rows per block; the slices are added in order.
-__global__ void __launch_bounds__(256) gated_norm_sums_kernel(const float* partials, int blocks, int width, float* dw_post, float* dscale,
+// columns x 16 slices of rows per block; the slices are added in order.
+__global__ void __launch_bounds__(512) gated_norm_sums_kernel(const float* partials, int rows, int width, float* dw_post, float* dscale,
                                                               float* dw_pre, int accumulate) {
-  __shared__ float part[8][33];
+  __shared__ float part[16][33];
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   const int64_t cols = 3 * (int64_t)width;
   float s = 0.f;
   if (c < cols)
-#pragma unroll 4
-    for (int b = slice; b < blocks; b += 8) s += partials[(int64_t)b * cols + c];
+#pragma unroll 8
+    for (int b = slice; b < rows; b += 16) s += partials[(int64_t)b * cols + c];
   part[slice][lane] = s;
   __syncthreads();
   if (slice || c >= cols) return;
   s = part[0][lane];
 #pragma unroll
-  for (int k = 1; k < 8; ++k) s += part[k][lane];
+  for (int k = 1; k < 16; ++k) s += part[k][lane];
   const int which = (int)(c / width);
   float* out = which == 0 ? dw_post : which == 1 ? dscale : dw_pre;
   if (!out) return;
@@ -374,35 +459,63 @@ __global__ void __launch_bounds__(256) gated_norm_sums_kernel(const float* parti
   *out = accumulate ? *out + s : s;
 }
 
-// Threads per row and floats per thread for a width: the fewest threads (a warp at least) that hold the row
-// in 16 floats each, 8 where single loads with their bounds need the registers.
-static void gn_shape(int width, bool vec, int* G, int* E) {
-  int e = width <= 128 ? 4 : (width <= 256 || (!vec && width <= 8192)) ? 8 : 16, g = 32;
-  while (g * e < width) g *= 2;
-  *G = g;
-  *E = e;
+// How a call goes: the mode, threads per row (G) and floats per thread (E), the fewest threads (a warp at least) that
+// hold the row in 16 floats each, or 8 where registers are short (single loads with their bounds, kept weights); blocks.
+struct GnShape {
+  int mode, G, E, threads, per_block, blocks;
+};
+static GnShape gn_geometry(int64_t rows, int width, int mode, bool backward) {
+  GnShape s;
+  s.mode = mode;
+  const int span = width + (mode == GN_SHIFT ? 3 : 0);
+  s.E = span <= 128 ? 4 : (span <= 256 || (mode != GN_VEC && span <= 8192)) ? 8 : 16;
+  s.G = 32;
+  while (s.G * s.E < span) s.G *= 2;
+  s.threads = std::max(s.G, 256);
+  s.per_block = s.threads / s.G;
+  const int per_sm = s.threads > 256 ? 1 : backward ? (s.E == 16 ? 2 : 3) : (s.E == 16 ? 3 : 4);      // as the launch bounds
+  s.blocks = (int)std::min<int64_t>(ceil_div(rows, s.per_block), (int64_t)state().sm_count * per_sm);
+  // a thread's rows are blocks * per_block apart: in the shifted form a multiple of 4
+  if (mode == GN_SHIFT && s.blocks * (int64_t)s.per_block < rows)
+    while (s.blocks * s.per_block % 4) --s.blocks;
+  return s;
 }
-static int gn_blocks(int64_t rows, int G, int threads, int per_sm) {
-  return (int)std::min<int64_t>(ceil_div(rows, threads / G), (int64_t)state().sm_count * (threads > 256 ? 1 : per_sm));
+// Rows of partial sums that a backward call leaves.
+static int64_t gn_partial_rows(int64_t rows, const GnShape& s) {
+  return s.mode == GN_SHIFT ? std::min<int64_t>(rows, (int64_t)s.blocks * s.per_block) : s.blocks;
 }
-static bool gn_vec(int width, std::initializer_list<const void*> ptrs, std::initializer_list<int64_t> lds) {
-  if (width % 4) return false;
-  for (const void* p : ptrs) if (!aligned16(p)) return false;
-  for (int64_t l : lds) if (l % 4) return false;
-  return true;
+// arrays: row-pitched operands of the call (NULL left out), vectors: the weights
+static GnShape gn_shape(int64_t rows, int width, std::initializer_list<std::pair<const void*, int64_t>> arrays,
+                        std::initializer_list<const void*> vectors, bool backward) {
+  bool vec = width % 4 == 0, alike = true;
+  uintptr_t start = 4;
+  int64_t pitch = 0;
+  for (const auto& a : arrays) {
+    if (!a.first) continue;
+    const uintptr_t at = ((uintptr_t)a.first >> 2) & 3;
+    vec = vec && at == 0 && a.second % 4 == 0;
+    alike = alike && (start == 4 || (at == start && (a.second - pitch) % 4 == 0));
+    start = at;
+    pitch = a.second;
+  }
+  for (const void* v : vectors) vec = vec && aligned16(v);
+  // a row and its offset have to fit 512 x 8 in the shifted form
+  return gn_geometry(rows, width, vec ? GN_VEC : alike && width <= 4096 - 3 ? GN_SHIFT : GN_SINGLE, backward);
 }
 
 }  // namespace b200
 
 using namespace b200;
 
-// Rows of up to 4096 values: blocks of 256 threads; wider ones: one row for a block of 512 or 1024.
-#define GN_KERNELS(KERNEL)                                                                                                \
-  (threads == 1024 ? (vec ? KERNEL<16, 4, 1024> : E == 8 ? KERNEL<8, 1, 1024> : KERNEL<16, 1, 1024>)                       \
-   : threads == 512 ? (vec ? KERNEL<16, 4, 512> : E == 8 ? KERNEL<8, 1, 512> : KERNEL<16, 1, 512>)                         \
-   : E == 4 ? (vec ? KERNEL<4, 4, 256> : KERNEL<4, 1, 256>)                                                                \
-   : E == 8 ? (vec ? KERNEL<8, 4, 256> : KERNEL<8, 1, 256>)                                                                \
-            : (vec ? KERNEL<16, 4, 256> : KERNEL<16, 1, 256>))
+// Rows of up to 4096 values (2045 in the shifted form): blocks of 256 threads; wider ones: one row for a block of 512 or 1024.
+#define GN_KERNELS(KERNEL)                                                                                               \
+  (s.mode == GN_VEC ? (s.threads == 1024 ? KERNEL<16, GN_VEC, 1024> : s.threads == 512 ? KERNEL<16, GN_VEC, 512>         \
+                       : s.E == 4 ? KERNEL<4, GN_VEC, 256> : s.E == 8 ? KERNEL<8, GN_VEC, 256> : KERNEL<16, GN_VEC, 256>) \
+   : s.mode == GN_SHIFT ? (s.threads == 512 ? KERNEL<8, GN_SHIFT, 512>                                                   \
+                           : s.E == 4 ? KERNEL<4, GN_SHIFT, 256> : KERNEL<8, GN_SHIFT, 256>)                             \
+   : s.threads == 1024 ? (s.E == 8 ? KERNEL<8, GN_SINGLE, 1024> : KERNEL<16, GN_SINGLE, 1024>)                           \
+   : s.threads == 512 ? KERNEL<8, GN_SINGLE, 512>                                                                        \
+                      : (s.E == 4 ? KERNEL<4, GN_SINGLE, 256> : KERNEL<8, GN_SINGLE, 256>))
 
 B200_API int b200_gated_norm_forward(const float* x, const float* y, const float* gate, const float* w_post, const float* scale,
                                      const float* w_pre, float* x_out, float* h_out, float* r_post, float* r_pre, int64_t rows,
@@ -421,19 +534,19 @@ B200_API int b200_gated_norm_forward(const float* x, const float* y, const float
                "gated norm: leading dimension too small");
   GatedNorm p = {x, y, gate, w_post, scale, w_pre, x_out, h_out, r_post, r_pre, rows, ld_x, ld_y, ld_gate, ld_x_out, ld_h_out,
                  (int)width, act, eps};
-  const bool vec = gn_vec((int)width, {x, y, gate, y ? x_out : nullptr, h_out}, {ld_x, y ? ld_y : 0, gate ? ld_gate : 0, y ? ld_x_out : 0, h_out ? ld_h_out : 0}) &&
-                   aligned16(w_post) && aligned16(scale) && aligned16(w_pre);
-  int G, E;
-  gn_shape((int)width, vec, &G, &E);
-  const int threads = std::max(G, 256), blocks = gn_blocks(rows, G, threads, 3);
-  GN_KERNELS(gated_norm_forward_kernel)<<<blocks, threads, 0, state().stream>>>(p, G);
+  const GnShape s = gn_shape(rows, (int)width, {{x, ld_x}, {y, ld_y}, {gate, ld_gate}, {y ? x_out : nullptr, ld_x_out}, {h_out, ld_h_out}},
+                             {w_post, scale, w_pre}, false);
+  GN_KERNELS(gated_norm_forward_kernel)<<<s.blocks, s.threads, 0, state().stream>>>(p, s.G);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
 
 B200_API int64_t b200_gated_norm_scratch_floats(int64_t rows, int64_t width) {
   if (rows <= 0 || width <= 0 || width > GN_MAX_WIDTH) return 0;
-  return std::min<int64_t>(rows, (int64_t)state().sm_count * 2) * 3 * width;      // a row of sums for each block, at most
+  int64_t most = 0;       // the form depends on the pointers
+  for (int mode : {GN_SINGLE, GN_VEC, GN_SHIFT})
+    if (mode != GN_SHIFT || width <= 4096 - 3) most = std::max(most, gn_partial_rows(rows, gn_geometry(rows, (int)width, mode, true)));
+  return most * 3 * width;
 }
 
 B200_API int b200_gated_norm_backward(const float* x_out, const float* y, const float* gate, const float* w_post, const float* scale,
@@ -464,20 +577,19 @@ B200_API int b200_gated_norm_backward(const float* x_out, const float* y, const 
   B200_REQUIRE(!sums || (scratch && scratch_floats >= b200_gated_norm_scratch_floats(rows, width)), "gated norm: scratch too small");
   GatedNormGrad p = {x_out, y, gate, w_post, scale, w_pre, r_post, r_pre, dx_out, dh, dx, dy, dgate, sums ? scratch : nullptr, rows,
                      ld_x_out, ld_y, ld_gate, ld_dx_out, ld_dh, ld_dx, ld_dy, ld_dgate, (int)width, act, accumulate ? 1 : 0};
-  const bool vec = gn_vec((int)width, {dh ? x_out : nullptr, y, gate, dx_out, dh, dx, y ? dy : nullptr, gate ? dgate : nullptr},
-                          {dh ? ld_x_out : 0, y ? ld_y : 0, gate ? ld_gate : 0, dx_out ? ld_dx_out : 0, dh ? ld_dh : 0, ld_dx, y ? ld_dy : 0, gate ? ld_dgate : 0}) &&
-                   aligned16(w_post) && aligned16(scale) && aligned16(w_pre);
-  int G, E;
-  gn_shape((int)width, vec, &G, &E);
-  const int threads = std::max(G, 256), blocks = gn_blocks(rows, G, threads, 2);
-  const size_t smem = (size_t)3 * E * threads * sizeof(float);
+  const GnShape s = gn_shape(rows, (int)width,
+                             {{dh ? x_out : nullptr, ld_x_out}, {y, ld_y}, {gate, ld_gate}, {dx_out, ld_dx_out}, {dh, ld_dh}, {dx, ld_dx},
+                              {y ? dy : nullptr, ld_dy}, {gate ? dgate : nullptr, ld_dgate}},
+                             {w_post, scale, w_pre}, true);
+  const size_t smem = (size_t)3 * s.E * s.threads * sizeof(float);
   auto kernel = GN_KERNELS(gated_norm_backward_kernel);
   // 48 KiB and more of dynamic shared memory has to be asked for (the static part counts too)
   if (smem >= 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<blocks, threads, smem, state().stream>>>(p, G);
+  kernel<<<s.blocks, s.threads, smem, state().stream>>>(p, s.G);
   B200_LAUNCH_CHECK();
   if (sums) {
-    gated_norm_sums_kernel<<<(unsigned)ceil_div(3 * width, 32), 256, 0, state().stream>>>(scratch, blocks, (int)width, dw_post, dscale, dw_pre,
+    const int partial_rows = (int)gn_partial_rows(rows, s);
+    gated_norm_sums_kernel<<<(unsigned)ceil_div(3 * width, 32), 512, 0, state().stream>>>(scratch, partial_rows, (int)width, dw_post, dscale, dw_pre,
                                                                                           accumulate ? 1 : 0);
     B200_LAUNCH_CHECK();
   }

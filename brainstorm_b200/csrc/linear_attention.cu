@@ -24,7 +24,7 @@ constexpr int LR_COLS = 32, LR_THREADS = 128;
 // accesses but those of the outputs are of 128 (R = 2: 64) bits; else the columns are 8 apart (coalesced 32-bit
 // accesses).
 template <int R, bool VEC>
-__global__ void __launch_bounds__(LR_THREADS, R == 8 ? 5 : 8) la_recurrent_kernel(LaCommon c, LaRuns runs, int max_slabs) {
+__global__ void __launch_bounds__(LR_THREADS, R == 8 ? 7 : 8) la_recurrent_kernel(LaCommon c, LaRuns runs, int max_slabs) {
   __shared__ float part[2][4][LR_COLS];
   const LaRun& p = runs.run[blockIdx.y];
   const unsigned bh = blockIdx.x / (unsigned)max_slabs;
@@ -197,8 +197,11 @@ static int la_check(const char* what, int64_t T, int64_t B, int64_t H, int64_t k
                (long long)kv_heads);
   return B200_OK;
 }
-// strides: t, b, h of q, k, v and the outputs, in that order
-static LaStrides la_strides(const int64_t* s, int i, int64_t div) { return LaStrides{s[3 * i], s[3 * i + 1], s[3 * i + 2], (int)div}; }
+// t, b and head strides of array i; NULL: all arrays are contiguous
+static LaStrides la_strides(const int64_t* s, int i, int64_t div, int64_t B, int64_t heads, int64_t d) {
+  if (!s) return LaStrides{B * heads * d, heads * d, d, (int)div};
+  return LaStrides{s[3 * i], s[3 * i + 1], s[3 * i + 2], (int)div};
+}
 
 }  // namespace b200
 
@@ -216,12 +219,12 @@ B200_API int b200_linear_attention_forward(const float* q, const float* k, const
   if (int rc = la_check("linear attention", T, B, H, kv_heads, dk, dv)) return rc;
   if (B * H == 0) return B200_OK;
   B200_REQUIRE(scratch_floats >= b200_linear_attention_forward_scratch_floats(T, B, H, dk, dv), "linear attention: scratch too small");
-  B200_REQUIRE(decay && (T == 0 || (q && k && v && out && strides)), "linear attention: NULL operand");
+  B200_REQUIRE(decay && (T == 0 || (q && k && v && out)), "linear attention: NULL operand");
   const int64_t g = H / kv_heads;
-  const int64_t none[12] = {0};
-  const int64_t* s = strides ? strides : none;
+  const int64_t* s = strides;
   LaCommon c = {decay, lengths, (int)T, (int)B, (int)H};
-  LaRun r = {q, k, v, out, la_strides(s, 0, 1), la_strides(s, 1, g), la_strides(s, 2, g), la_strides(s, 3, 1), state, state_out, 0, 0,
+  LaRun r = {q, k, v, out, la_strides(s, 0, 1, B, H, dk), la_strides(s, 1, g, B, kv_heads, dk), la_strides(s, 2, g, B, kv_heads, dv),
+             la_strides(s, 3, 1, B, H, dv), state, state_out, 0, 0,
              0, (int)dk, (int)dv, 1.f, scale};
   return la_run(c, &r, 1, scratch);
 }
@@ -238,16 +241,17 @@ B200_API int b200_linear_attention_backward(const float* q, const float* k, cons
   if (int rc = require_ready()) return rc;
   if (int rc = la_check("linear attention", T, B, H, kv_heads, dk, dv)) return rc;
   if (B * H == 0) return B200_OK;
-  B200_REQUIRE(decay && (T == 0 || (q && k && v && dout && dq && dk_out && dv_out && strides)), "linear attention: NULL operand");
+  B200_REQUIRE(decay && (T == 0 || (q && k && v && dout && dq && dk_out && dv_out)), "linear attention: NULL operand");
   B200_REQUIRE(scratch_floats >= b200_linear_attention_backward_scratch_floats(T, B, H, kv_heads, dk, dv), "linear attention: scratch too small");
   B200_REQUIRE(!dstate || dstate != dstate_out, "linear attention: dstate overlaps dstate_out");   // two gradients read it
   const int64_t g = H / kv_heads;
-  const int64_t none[21] = {0};
-  const int64_t* s = strides ? strides : none;
+  const int64_t* s = strides;
   const int acc = accumulate ? 1 : 0;
   LaCommon c = {decay, lengths, (int)T, (int)B, (int)H};
-  const LaStrides qs = la_strides(s, 0, 1), ks = la_strides(s, 1, g), vs = la_strides(s, 2, g), dos = la_strides(s, 3, 1), dqs = la_strides(s, 4, 1);
-  LaStrides dks = la_strides(s, 5, 1), dvs = la_strides(s, 6, 1);
+  const LaStrides qs = la_strides(s, 0, 1, B, H, dk), ks = la_strides(s, 1, g, B, kv_heads, dk), vs = la_strides(s, 2, g, B, kv_heads, dv),
+                  dos = la_strides(s, 3, 1, B, H, dv), dqs = la_strides(s, 4, 1, B, H, dk);
+  const LaStrides shared[2] = {la_strides(s, 5, 1, B, kv_heads, dk), la_strides(s, 6, 1, B, kv_heads, dv)};
+  LaStrides dks = shared[0], dvs = shared[1];
   float *dk_w = dk_out, *dv_w = dv_out;
   if (g > 1) {     // one gradient for each head of q first, then the sum over the heads that share
     dk_w = scratch;
@@ -266,7 +270,7 @@ B200_API int b200_linear_attention_backward(const float* q, const float* k, cons
       const int d = (int)(i ? dv : dk);
       const int64_t total = T * B * kv_heads * d;
       const int64_t blocks = std::min<int64_t>(ceil_div(total, 256), (int64_t)b200::state().sm_count * 16);
-      la_share_kernel<<<(unsigned)blocks, 256, 0, b200::state().stream>>>(i ? dv_w : dk_w, i ? dv_out : dk_out, la_strides(s, i ? 6 : 5, 1), T * B,
+      la_share_kernel<<<(unsigned)blocks, 256, 0, b200::state().stream>>>(i ? dv_w : dk_w, i ? dv_out : dk_out, shared[i], T * B,
                                                                           (int)B, (int)kv_heads, (int)g, d, acc);
       B200_LAUNCH_CHECK();
     }

@@ -63,13 +63,11 @@ def _whole(a, shape, what):
     return a.ptr
 
 
-def _heads(a, ndim, what):
+def _heads(a, what):
     """(t, b, h) strides of a (T, B, heads, d) or (B, heads, d) array with contiguous d."""
-    if len(a.shape) != ndim:
-        raise ValueError('%s has shape %r, expected %d dimensions' % (what, a.shape, ndim))
     if a.shape[-1] > 1 and a.strides[-1] != 1:
         raise NotImplementedError('%s: the last dimension must be contiguous' % what)
-    return tuple(a.strides[:3]) if ndim == 4 else (0,) + tuple(a.strides[:2])
+    return tuple(a.strides[:3]) if len(a.shape) == 4 else (0,) + tuple(a.strides[:2])
 
 
 def _expect(a, shape, what):
@@ -84,17 +82,22 @@ def _span(a):
     return a.ptr, a.ptr + 4 * (sum((n - 1) * s for n, s in zip(a.shape, a.strides)) + 1)
 
 
-def _apart(outputs, inputs, allowed=()):
-    """Refuse an output that starts where another operand starts, and contiguous ones that overlap at all
-    (two row-pitched views may interleave in one buffer, as the columns of a hub do)."""
-    spans = sorted([_span(a) for _, a in outputs if a is not None and a.size] + [_span(a) for _, a in inputs if a is not None and a.size])
+def _meet(arrays):
+    """Whether the address ranges of any two of the arrays overlap."""
+    spans = [(a.ptr, a.ptr + 4 * a.size) if a._contig else _span(a) for a in arrays if a is not None and a.size]
+    spans.sort()
     end = 0
     for lo, hi in spans:
         if lo < end:
-            break
+            return True
         end = hi
-    else:
-        return              # no two operands meet anywhere
+    return False
+
+
+def _apart(outputs, inputs, allowed=()):
+    """Refuse an output that starts where another operand starts, and contiguous ones that overlap at all
+    (two row-pitched views may interleave in one buffer, as the columns of a hub do).  Called when operands
+    meet (``_meet``)."""
     seen = [(n, a) for n, a in inputs if a is not None and a.size]
     for name, a in outputs:
         if a is None or not a.size:
@@ -106,6 +109,9 @@ def _apart(outputs, inputs, allowed=()):
             if a.ptr == b.ptr or (a._contig or b._contig) and lo < _span(b)[1] and _span(b)[0] < hi:
                 raise ValueError('%s overlaps %s' % (name, other))
         seen.append((name, a))
+
+
+_Strides12, _Strides21 = ctypes.c_int64 * 12, ctypes.c_int64 * 21
 
 
 class SequenceOps(object):
@@ -130,13 +136,19 @@ class SequenceOps(object):
         63 tokens before it."""
         T, B, H, K, dk, dv = self._attention_shapes(q, k, v, 4)
         _expect(out, (T, B, H, dv), 'out')
-        strides = (ctypes.c_int64 * 12)(*(_heads(q, 4, 'q') + _heads(k, 4, 'k') + _heads(v, 4, 'v') + _heads(out, 4, 'out')))
-        _apart((('out', out), ('state_out', state_out)), (('q', q), ('k', k), ('v', v), ('decay', decay), ('state', state), ('lengths', lengths)),
-               (('state_out', 'state'),))
-        work, need = self._attention_work(lib.b200_linear_attention_forward_scratch_floats(T, B, H, dk, dv))
+        strides = 0
+        if not (q._contig and k._contig and v._contig and out._contig):
+            strides = _Strides12(*(_heads(q, 'q') + _heads(k, 'k') + _heads(v, 'v') + _heads(out, 'out')))
+        if _meet((q, k, v, out, decay, state, state_out, lengths)):
+            _apart((('out', out), ('state_out', state_out)), (('q', q), ('k', k), ('v', v), ('decay', decay), ('state', state), ('lengths', lengths)),
+                   (('state_out', 'state'),))
+        need = lib.b200_linear_attention_forward_scratch_floats(T, B, H, dk, dv)
+        # stream-ordered and released with the call: calls on two streams, and recorded graphs, have their own
+        work = B200Array.empty((need,), zero=False) if need else None
+        states = (B, H, dk, dv)
         check(lib.b200_linear_attention_forward(
-            q.ptr, k.ptr, v.ptr, _vector(decay, H, 'decay'), out.ptr, _whole(state, (B, H, dk, dv), 'state'),
-            _whole(state_out, (B, H, dk, dv), 'state_out'), _vector(lengths, B, 'lengths'), T, B, H, K, dk, dv, strides, scale, _ptr(work), need))
+            q.ptr, k.ptr, v.ptr, _vector(decay, H, 'decay'), out.ptr, _whole(state, states, 'state'), _whole(state_out, states, 'state_out'),
+            _vector(lengths, B, 'lengths'), T, B, H, K, dk, dv, strides, scale, _ptr(work), need))
 
     def linear_attention_backward(self, q, k, v, decay, dout, dq, dk, dv, scale=1.0, state=None, dstate_out=None, dstate=None, lengths=None,
                                   accumulate=True):
@@ -148,10 +160,15 @@ class SequenceOps(object):
         for a, shape, what in ((dout, (T, B, H, d_v), 'dout'), (dq, q.shape, 'dq'), (dk, k.shape, 'dk'), (dv, v.shape, 'dv')):
             _expect(a, shape, what)
         arrays = (('q', q), ('k', k), ('v', v), ('dout', dout), ('dq', dq), ('dk', dk), ('dv', dv))
-        strides = (ctypes.c_int64 * 21)(*[s for what, a in arrays for s in _heads(a, 4, what)])
-        _apart(arrays[4:] + (('dstate', dstate),), arrays[:4] + (('decay', decay), ('state', state), ('dstate_out', dstate_out), ('lengths', lengths)))
+        strides = 0
+        if not all(a._contig for _, a in arrays):
+            strides = _Strides21(*[s for what, a in arrays for s in _heads(a, what)])
+        if _meet((q, k, v, dout, dq, dk, dv, decay, state, dstate_out, dstate, lengths)):
+            _apart(arrays[4:] + (('dstate', dstate),),
+                   arrays[:4] + (('decay', decay), ('state', state), ('dstate_out', dstate_out), ('lengths', lengths)))
         states = (B, H, d_k, d_v)
-        work, need = self._attention_work(lib.b200_linear_attention_backward_scratch_floats(T, B, H, K, d_k, d_v))
+        need = lib.b200_linear_attention_backward_scratch_floats(T, B, H, K, d_k, d_v)
+        work = B200Array.empty((need,), zero=False) if need else None
         check(lib.b200_linear_attention_backward(
             q.ptr, k.ptr, v.ptr, _vector(decay, H, 'decay'), dout.ptr, dq.ptr, dk.ptr, dv.ptr, _whole(state, states, 'state'),
             _whole(dstate_out, states, 'dstate_out'), _whole(dstate, states, 'dstate'), _vector(lengths, B, 'lengths'), T, B, H, K, d_k, d_v,
@@ -160,10 +177,13 @@ class SequenceOps(object):
     def linear_attention_step(self, q, k, v, decay, state, out, scale=1.0):
         """One token for every sequence: q (B, H, dk), k (B, K, dk), v (B, K, dv), out (B, H, dv); ``state``
         (B, H, dk, dv) is updated in place.  The recurrence of ``linear_attention_forward``."""
-        _, B, H, K, dk, dv = self._attention_shapes(q, k, v, 3)
+        B, H, K, dk, dv = self._attention_shapes(q, k, v, 3)
         _expect(out, (B, H, dv), 'out')
-        strides = (ctypes.c_int64 * 12)(*(_heads(q, 3, 'q') + _heads(k, 3, 'k') + _heads(v, 3, 'v') + _heads(out, 3, 'out')))
-        _apart((('out', out), ('state', state)), (('q', q), ('k', k), ('v', v), ('decay', decay)))
+        strides = 0
+        if not (q._contig and k._contig and v._contig and out._contig):
+            strides = _Strides12(*(_heads(q, 'q') + _heads(k, 'k') + _heads(v, 'v') + _heads(out, 'out')))
+        if _meet((q, k, v, out, decay, state)):
+            _apart((('out', out), ('state', state)), (('q', q), ('k', k), ('v', v), ('decay', decay)))
         s = _whole(state, (B, H, dk, dv), 'state')
         check(lib.b200_linear_attention_forward(q.ptr, k.ptr, v.ptr, _vector(decay, H, 'decay'), out.ptr, s, s, 0, 1, B, H, K, dk, dv, strides, scale,
                                                 0, 0))
@@ -172,19 +192,13 @@ class SequenceOps(object):
     def _attention_shapes(q, k, v, ndim):
         if len(q.shape) != ndim or len(k.shape) != ndim or len(v.shape) != ndim:
             raise ValueError('q, k and v must have %d dimensions, got %r, %r, %r' % (ndim, q.shape, k.shape, v.shape))
-        lead, H, dk = q.shape[:-2], q.shape[-2], q.shape[-1]
+        *lead, H, dk = q.shape
         K, dv = k.shape[-2], v.shape[-1]
-        if k.shape != lead + (K, dk) or v.shape != lead + (K, dv):
+        if k.shape != (*lead, K, dk) or v.shape != (*lead, K, dv):
             raise ValueError('shapes %r, %r, %r of q, k, v do not agree' % (q.shape, k.shape, v.shape))
         if (K == 0) != (H == 0) or K and H % K:
             raise ValueError('%d heads cannot share %d key/value heads' % (H, K))
-        T, B = lead if ndim == 4 else (1, lead[0])
-        return T, B, H, K, dk, dv
-
-    @staticmethod
-    def _attention_work(floats):
-        # stream-ordered and released with the call: calls on two streams, and recorded graphs, have their own
-        return (B200Array.empty((floats,), zero=False), floats) if floats > 0 else (None, 0)
+        return (*lead, H, K, dk, dv)
 
     # ------------------------------------------------------- norms, gate and residual of a block
     def gated_norm_forward(self, x, y, gate, w_post, scale, w_pre, x_out, h_out, r_post, r_pre, epsilon=1e-6, activation='sigmoid'):
@@ -217,8 +231,9 @@ class SequenceOps(object):
         if y is None:
             x_out = None
         lds = [_rows(a, shape, what) for a, what in ((x, 'x'), (y, 'y'), (gate, 'gate'), (x_out, 'x_out'), (h_out, 'h_out'))]
-        _apart((('x_out', x_out), ('h_out', h_out), ('r_post', r_post), ('r_pre', r_pre)),
-               (('x', x), ('y', y), ('gate', gate), ('w_post', w_post), ('scale', scale), ('w_pre', w_pre)), (('x_out', 'x'), ('h_out', 'y')))
+        if _meet((x, y, gate, x_out, h_out, w_post, scale, w_pre, r_post, r_pre)):
+            _apart((('x_out', x_out), ('h_out', h_out), ('r_post', r_post), ('r_pre', r_pre)),
+                   (('x', x), ('y', y), ('gate', gate), ('w_post', w_post), ('scale', scale), ('w_pre', w_pre)), (('x_out', 'x'), ('h_out', 'y')))
         check(lib.b200_gated_norm_forward(
             x.ptr, _ptr(y), _ptr(gate), _vector(w_post, width, 'w_post'), _vector(scale, width, 'scale'), _vector(w_pre, width, 'w_pre'), _ptr(x_out),
             _ptr(h_out), _vector(r_post, rows, 'r_post') if y is not None else 0, _vector(r_pre, rows, 'r_pre') if h_out is not None else 0, rows,
@@ -254,8 +269,9 @@ class SequenceOps(object):
             dgate = None
         named = (('x_out', x_out), ('y', y), ('gate', gate), ('dx_out', dx_out), ('dh', dh), ('dx', dx), ('dy', dy), ('dgate', dgate))
         lds = [_rows(a, shape, what) for what, a in named]
-        _apart(named[5:] + (('dw_post', dw_post), ('dscale', dscale), ('dw_pre', dw_pre)),
-               named[:5] + (('w_post', w_post), ('scale', scale), ('w_pre', w_pre), ('r_post', r_post), ('r_pre', r_pre)), (('dx', 'dx_out'),))
+        if _meet((x_out, y, gate, dx_out, dh, dx, dy, dgate, dw_post, dscale, dw_pre, w_post, scale, w_pre, r_post, r_pre)):
+            _apart(named[5:] + (('dw_post', dw_post), ('dscale', dscale), ('dw_pre', dw_pre)),
+                   named[:5] + (('w_post', w_post), ('scale', scale), ('w_pre', w_pre), ('r_post', r_post), ('r_pre', r_pre)), (('dx', 'dx_out'),))
         need = lib.b200_gated_norm_scratch_floats(rows, width) if not (dw_post is None and dscale is None and dw_pre is None) else 0
         work = B200Array.empty((need,), zero=False) if need else None
         check(lib.b200_gated_norm_backward(
@@ -283,7 +299,8 @@ class SequenceOps(object):
         shape = param.shape
         arrays = (('param', param), ('grad', grad), ('momentum', momentum), ('update', update))
         ptrs = [_whole(a, shape, what) for what, a in arrays]
-        _apart((arrays[0],) + arrays[2:], arrays[1:2])
+        if _meet((param, grad, momentum, update)):
+            _apart((arrays[0],) + arrays[2:], arrays[1:2])
         n, rows, cols = shape if len(shape) == 3 else (1,) + shape
         need = lib.b200_muon_scratch_floats(n, rows, cols)
         work = B200Array.empty((need,), zero=False) if need else None

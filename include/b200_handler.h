@@ -392,7 +392,7 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      held to [0, T]; NULL: all T); out is zero behind them and the state keeps what it was
  *      at the end.  Arrays are (T, B, heads, d) with contiguous d; `strides` (host memory)
  *      gives the t, b and head strides in floats of q, k, v, out (forward) and of q, k, v,
- *      dout, dq, dk, dv (backward).  q, out have H heads, k and v kv_heads, H a multiple of
+ *      dout, dq, dk, dv (backward); NULL: all of them are contiguous.  q, out have H heads, k and v kv_heads, H a multiple of
  *      kv_heads: head h reads key/value head h / (H / kv_heads).  dk, dv: 1 .. 128.  state,
  *      state_out, dstate_out, dstate: contiguous (B, H, dk, dv), each may be NULL (zeros in,
  *      not wanted out); state_out may be state; no other output may overlap

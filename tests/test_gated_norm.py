@@ -103,7 +103,8 @@ def _check(h, d, act, post=True, pre=True, eps=1e-6):
 
 # one value, one row, widths at and off the vector and thread borders, the widest row, more rows than blocks
 SHAPES = [(1, 1), (3, 2), (1, 31), (7, 32), (5, 33), (4, 127), (9, 128), (2, 129), (300, 130), (3, 256), (3, 260), (17, 511), (700, 512), (11, 513), (33, 1000),
-          (5, 1024), (6, 1537), (400, 2048), (3, 4096), (2, 4097), (2, 8191), (3, 12000), (2, 16384), (310, 16383)]
+          (5, 1024), (6, 1537), (400, 2048), (3, 4096), (2, 4097), (2, 8191), (3, 12000), (2, 16384), (310, 16383),
+          (3000, 125), (3000, 126), (4000, 128), (5000, 33), (2500, 129), (2500, 253), (2500, 254), (1300, 509), (1300, 1021), (900, 1022), (900, 2045), (700, 2047), (700, 4093), (301, 4094)]
 
 
 @pytest.fixture(scope='module')
