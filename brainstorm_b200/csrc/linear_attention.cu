@@ -1,10 +1,9 @@
-// Decayed linear attention, recurrent form: 32 columns of the state of one (sequence, head) stay in the
-// registers of one block while the tokens pass by.  Columns of the state never meet, so blocks are
-// independent.  Serves single tokens (the step of a model that answers) and short sequences.
+// Decayed linear attention, recurrent form, for single tokens (the step of a model that answers) and short sequences:
+// the state stays on the SM while the tokens pass by.
 //
-// Bound for a single token: HBM, the state is read once and written once (8 dk dv bytes) and everything
-// else is small; the state, k, q and v are all asked for at once, and a block of 128 threads with up to 8
-// 128-bit loads each leaves room for many blocks on an SM.  For several tokens: latency, one barrier each.
+// Bound for a single token: HBM, the state is read once and written once (8 dk dv bytes) and everything else is small;
+// the state, k, q and v are all asked for at once, and the registers are held to what lets six blocks of 128 threads
+// share an SM (512 x 16 states of 128 x 128: 173 us, the floor being 166; five blocks 184, eight 189).  For several tokens: latency.
 #include <string.h>
 
 #include <algorithm>
@@ -20,26 +19,38 @@ struct LaRuns {
 
 constexpr int LR_COLS = 32, LR_THREADS = 128;
 
-// Thread: four columns cg (of 8 groups), rows R rl + r, r < R.  VEC: the four columns lie side by side, and all
-// accesses but those of the outputs are of 128 (R = 2: 64) bits; else the columns are 8 apart (coalesced 32-bit
-// accesses).
-template <int R, bool VEC>
-__global__ void __launch_bounds__(LR_THREADS, R == 8 ? 7 : 8) la_recurrent_kernel(LaCommon c, LaRuns runs, int max_slabs) {
+__device__ __forceinline__ int64_t la_offset(const LaStrides& x, int b, int h) {
+  return (int64_t)b * x.b + (int64_t)(x.div == 1 ? h : h / x.div) * x.h;
+}
+
+// 32 columns of the state of one (sequence, head), a slab, lie in the registers of `wps` warps (1, 2 or 4); columns never
+// meet, so slabs are independent.  Lane: four columns cg (of 8 groups), rows R rl + r, r < R; dv is a multiple of 4 and
+// states start on 16 bytes.  VEC: so do the rows of q, k and v, and dk is a multiple of 4.  ONE: a single token (the next
+// token's registers are not needed).
+template <int R, bool VEC, bool ONE>
+__global__ void __launch_bounds__(LR_THREADS, R == 8 ? (ONE ? 6 : 5) : 8) la_recurrent_kernel(LaCommon c, LaRuns runs, int max_slabs, int wps) {
   __shared__ float part[2][4][LR_COLS];
   const LaRun& p = runs.run[blockIdx.y];
-  const unsigned bh = blockIdx.x / (unsigned)max_slabs;
-  const int c0 = (int)(blockIdx.x - bh * max_slabs) * LR_COLS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned group = (unsigned)warp / wps, id = blockIdx.x * (4u / wps) + group;
+  const unsigned bh = id / (unsigned)max_slabs;
+  const int c0 = (int)(id - bh * max_slabs) * LR_COLS;
   const int dk = p.dk, dv = p.dv;
-  if (c0 >= dv) return;
+  if (bh >= (unsigned)c.B * (unsigned)c.H || c0 >= dv) return;
   const int b = (int)(bh / (unsigned)c.H), h = (int)bh - b * c.H;
   const int n = la_length(c, b);
   const float l = c.decay[h];
-  const int cg = threadIdx.x & 7, rl = threadIdx.x >> 3, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int cg = lane & 7, rl = (warp - group * wps) * 4 + (lane >> 3);
   const int64_t tok0 = p.reverse ? n - 1 : 0, dir = p.reverse ? -1 : 1;
-  auto at = [&](const LaStrides& x) { return (int64_t)b * x.b + (int64_t)(x.div == 1 ? h : h / x.div) * x.h; };
-  const float *q = p.q + at(p.qs) + tok0 * p.qs.t, *k = p.k + at(p.ks) + tok0 * p.ks.t, *v = p.v + at(p.vs) + tok0 * p.vs.t;
-  float* o = p.o + at(p.os);
-  auto col = [&](int j) { return c0 + (VEC ? 4 * cg + j : cg + 8 * j); };
+  const float *q = p.q + la_offset(p.qs, b, h) + tok0 * p.qs.t, *k = p.k + la_offset(p.ks, b, h) + tok0 * p.ks.t,
+              *v = p.v + la_offset(p.vs, b, h) + tok0 * p.vs.t;
+  float* o = p.o + la_offset(p.os, b, h);
+  const int col = c0 + 4 * cg;
+  auto meet = [&]() {       // the warps of this slab
+    if (wps == 1) __syncwarp();
+    else if (group == 0) asm volatile("bar.sync 1, %0;" ::"r"(32 * wps) : "memory");
+    else asm volatile("bar.sync 2, %0;" ::"r"(32 * wps) : "memory");
+  };
 
   float S[R][4], kk[R], qq[R], vv[4];
   const float* s_in = p.s_in ? p.s_in + (int64_t)bh * dk * dv : nullptr;
@@ -48,16 +59,13 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 7 : 8) la_recurrent_kerne
     const int i = R * rl + r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) S[r][j] = 0.f;
-    if (!s_in || i >= dk) continue;
-    if (VEC && !p.s_in_t) {
-      if (col(0) < dv) {
-        const float4 x = *reinterpret_cast<const float4*>(s_in + (int64_t)i * dv + col(0));
-        S[r][0] = x.x; S[r][1] = x.y; S[r][2] = x.z; S[r][3] = x.w;
-      }
+    if (!s_in || i >= dk || col >= dv) continue;
+    if (!p.s_in_t) {
+      const float4 x = *reinterpret_cast<const float4*>(s_in + (int64_t)i * dv + col);
+      S[r][0] = x.x; S[r][1] = x.y; S[r][2] = x.z; S[r][3] = x.w;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col(j) < dv) S[r][j] = p.s_in_t ? s_in[(int64_t)col(j) * dk + i] : s_in[(int64_t)i * dv + col(j)];
+      for (int j = 0; j < 4; ++j) S[r][j] = s_in[(int64_t)(col + j) * dk + i];
     }
   }
   auto fetch = [&](int step) {
@@ -77,7 +85,7 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 7 : 8) la_recurrent_kerne
         memcpy(kk + r, &x, sizeof(V));
       }
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (col(0) < dv) x = *reinterpret_cast<const float4*>(vt + col(0));
+      if (col < dv) x = *reinterpret_cast<const float4*>(vt + col);
       memcpy(vv, &x, sizeof(x));
     } else {
 #pragma unroll
@@ -86,29 +94,22 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 7 : 8) la_recurrent_kerne
         kk[r] = i + r < dk ? kt[i + r] : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) vv[j] = col(j) < dv ? vt[col(j)] : 0.f;
+      for (int j = 0; j < 4; ++j) vv[j] = col < dv ? vt[col + j] : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) vv[j] *= p.k_scale;
   };
   auto store_state = [&](float f) {
-    if (!p.s_out) return;
+    if (!p.s_out || col >= dv) return;
     float* s = p.s_out + (int64_t)bh * dk * dv;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int i = R * rl + r;
-      if (i >= dk) continue;
-      if (VEC) {
-        if (col(0) < dv) *reinterpret_cast<float4*>(s + (int64_t)i * dv + col(0)) = make_float4(f * S[r][0], f * S[r][1], f * S[r][2], f * S[r][3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col(j) < dv) s[(int64_t)i * dv + col(j)] = f * S[r][j];
-      }
+      if (i < dk) *reinterpret_cast<float4*>(s + (int64_t)i * dv + col) = make_float4(f * S[r][0], f * S[r][1], f * S[r][2], f * S[r][3]);
     }
   };
   if (n > 0) fetch(0);
-  for (int step = 0; step < n; ++step) {
+  for (int step = 0; step < (ONE ? min(n, 1) : n); ++step) {
     const float f = (p.reverse && step == 0) ? 1.f : l;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -118,48 +119,135 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? 7 : 8) la_recurrent_kerne
         S[r][j] = f * S[r][j] + kk[r] * vv[j];
         acc[j] += qq[r] * S[r][j];
       }
-    if (step + 1 < n) fetch(step + 1);
+    if (!ONE && step + 1 < n) fetch(step + 1);
     else store_state(p.reverse ? l : 1.f);
 #pragma unroll
     for (int m = 8; m < 32; m <<= 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], m);
-    if (lane < 8)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) part[step & 1][w][col(j) - c0] = acc[j];
-    __syncthreads();      // the sums of this step are in place; those of the step before have been read
-    if (threadIdx.x < LR_COLS && c0 + (int)threadIdx.x < dv) {
-      const float(*s)[LR_COLS] = part[step & 1];
-      const float x = p.o_scale * ((s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]));
-      float* dst = o + (tok0 + dir * step) * p.os.t + c0 + threadIdx.x;
+    if (lane < 8) *reinterpret_cast<float4*>(&part[step & 1][warp][4 * cg]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    meet();      // the sums of this step are in place; those of the step before have been read
+    if (warp == (int)group * wps && c0 + lane < dv) {
+      float x = part[step & 1][warp][lane];
+      for (int u = 1; u < wps; ++u) x += part[step & 1][warp + u][lane];
+      x *= p.o_scale;
+      float* dst = o + (tok0 + dir * step) * p.os.t + c0 + lane;
       *dst = p.accumulate ? *dst + x : x;
     }
   }
-  if (!p.accumulate && threadIdx.x < LR_COLS && c0 + (int)threadIdx.x < dv)      // tokens behind the end of the sequence
-    for (int64_t t = n; t < c.T; ++t) o[t * p.os.t + c0 + threadIdx.x] = 0.f;
+  if (!p.accumulate && warp == (int)group * wps && c0 + lane < dv)      // tokens behind the end of the sequence
+    for (int64_t t = n; t < c.T; ++t) o[t * p.os.t + c0 + lane] = 0.f;
   if (n == 0) store_state(1.f);
+}
+
+// Any dv and any alignment: a block for the state of one (sequence, head), 32 bits a lane.  Thread: column j, rows
+// rg + groups * r, r < R, in registers.
+template <int R>
+__global__ void __launch_bounds__(1024) la_recurrent_any_kernel(LaCommon c, LaRuns runs, int cols_log2) {
+  __shared__ float qkv[3 * LA_MAX_DIM];
+  extern __shared__ float part[];
+  const LaRun& p = runs.run[blockIdx.y];
+  const int bh = blockIdx.x, b = bh / c.H, h = bh - b * c.H;
+  const int n = la_length(c, b), dk = p.dk, dv = p.dv, tid = threadIdx.x, threads = blockDim.x;
+  const float l = c.decay[h];
+  const int64_t tok0 = p.reverse ? n - 1 : 0, dir = p.reverse ? -1 : 1;
+  const float *q = p.q + la_offset(p.qs, b, h) + tok0 * p.qs.t, *k = p.k + la_offset(p.ks, b, h) + tok0 * p.ks.t,
+              *v = p.v + la_offset(p.vs, b, h) + tok0 * p.vs.t;
+  float* o = p.o + la_offset(p.os, b, h);
+  const int cols = 1 << cols_log2, j = tid & (cols - 1), rg = tid >> cols_log2, groups = threads >> cols_log2;
+  const int64_t state = (int64_t)bh * dk * dv;
+  float S[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = rg + groups * r;
+    S[r] = 0.f;
+    if (p.s_in && i < dk && j < dv) S[r] = p.s_in_t ? p.s_in[state + j * dk + i] : p.s_in[state + i * dv + j];
+  }
+  for (int step = 0; step < n; ++step) {
+    const float *qt = q + dir * step * p.qs.t, *kt = k + dir * step * p.ks.t, *vt = v + dir * step * p.vs.t;
+    for (int i = tid; i < dk; i += threads) {
+      qkv[i] = qt[i];
+      qkv[LA_MAX_DIM + i] = kt[i] * p.k_scale;
+    }
+    for (int i = tid; i < dv; i += threads) qkv[2 * LA_MAX_DIM + i] = vt[i];
+    __syncthreads();
+    const float f = (p.reverse && step == 0) ? 1.f : l, vj = j < dv ? qkv[2 * LA_MAX_DIM + j] : 0.f;
+    float acc = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = min(rg + groups * r, LA_MAX_DIM - 1);
+      if (rg + groups * r < dk) {
+        S[r] = f * S[r] + qkv[LA_MAX_DIM + i] * vj;
+        acc += qkv[i] * S[r];
+      }
+    }
+    part[tid] = acc;
+    __syncthreads();
+    if (tid < dv) {
+      float x = part[tid];
+      for (int u = 1; u < groups; ++u) x += part[(u << cols_log2) + tid];
+      x *= p.o_scale;
+      float* dst = o + (tok0 + dir * step) * p.os.t + tid;
+      *dst = p.accumulate ? *dst + x : x;
+    }
+  }
+  if (!p.accumulate)       // tokens behind the end of the sequence
+    for (int64_t t = n; t < c.T; ++t)
+      for (int i = tid; i < dv; i += threads) o[t * p.os.t + i] = 0.f;
+  if (p.s_out) {
+    const float f = (p.reverse && n > 0) ? l : 1.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = rg + groups * r;
+      if (i < dk && j < dv) p.s_out[state + i * dv + j] = f * S[r];
+    }
+  }
 }
 
 // One launch for up to three runs over the same sequences.
 int la_recurrent(const LaCommon& c, const LaRun* runs, int count) {
   LaRuns all = {};
   int dk = 0, dv = 0;
-  bool vec = true;
+  bool whole = true, vec = true;
   for (int i = 0; i < count; ++i) {
     all.run[i] = runs[i];
     dk = std::max(dk, runs[i].dk);
     dv = std::max(dv, runs[i].dv);
-    vec = vec && runs[i].dk % 4 == 0 && runs[i].dv % 4 == 0 && aligned16(runs[i].s_in) && aligned16(runs[i].s_out);
+    whole = whole && runs[i].dv % 4 == 0 && aligned16(runs[i].s_in) && aligned16(runs[i].s_out);
+    vec = vec && runs[i].dk % 4 == 0;
     for (const float* a : {runs[i].q, runs[i].k, runs[i].v}) vec = vec && aligned16(a);
     for (const LaStrides* x : {&runs[i].qs, &runs[i].ks, &runs[i].vs}) vec = vec && x->t % 4 == 0 && x->b % 4 == 0 && x->h % 4 == 0;
   }
+  const int64_t BH = (int64_t)c.B * c.H;
+  const cudaStream_t st = state().stream;
+  if (!whole) {
+    int log2 = 3, threads = 128;
+    while ((1 << log2) < dv) ++log2;
+    while ((int64_t)dk << log2 > 16ll * threads) threads *= 2;      // 1024 at dk = dv = 128
+    const int rows = (int)ceil_div(dk, threads >> log2);
+    auto kernel = rows <= 4 ? la_recurrent_any_kernel<4> : rows <= 8 ? la_recurrent_any_kernel<8> : la_recurrent_any_kernel<16>;
+    kernel<<<dim3((unsigned)BH, (unsigned)count), threads, threads * sizeof(float), st>>>(c, all, log2);
+    B200_LAUNCH_CHECK();
+    return B200_OK;
+  }
   const int slabs = (int)ceil_div(dv, LR_COLS);
-  B200_REQUIRE((int64_t)c.B * c.H * slabs < (1ll << 31), "linear attention: extent too large");
-  const dim3 grid((unsigned)((int64_t)c.B * c.H * slabs), (unsigned)count);
-  auto kernel = dk <= 32 ? (vec ? la_recurrent_kernel<2, true> : la_recurrent_kernel<2, false>)
-                : dk <= 64 ? (vec ? la_recurrent_kernel<4, true> : la_recurrent_kernel<4, false>)
-                           : (vec ? la_recurrent_kernel<8, true> : la_recurrent_kernel<8, false>);
-  kernel<<<grid, LR_THREADS, 0, state().stream>>>(c, all, slabs);
+  B200_REQUIRE(BH * slabs < (1ll << 31), "linear attention: extent too large");
+  // Few slabs: four warps each, for the latency.  Many: as few as hold it with eight rows (dk up to 16: four) a lane, for
+  // the loads in flight.
+  int rows, wps;
+  if (BH * slabs * count <= 4ll * state().sm_count) {
+    wps = 4;
+    rows = dk <= 32 ? 2 : dk <= 64 ? 4 : 8;
+  } else {
+    rows = dk <= 16 ? 4 : 8;
+    wps = dk <= 32 ? 1 : dk <= 64 ? 2 : 4;
+  }
+#define LR_KERNELS(R)                                                                                  \
+  (c.T == 1 ? (vec ? la_recurrent_kernel<R, true, true> : la_recurrent_kernel<R, false, true>)         \
+            : (vec ? la_recurrent_kernel<R, true, false> : la_recurrent_kernel<R, false, false>))
+  auto kernel = rows == 2 ? LR_KERNELS(2) : rows == 4 ? LR_KERNELS(4) : LR_KERNELS(8);
+#undef LR_KERNELS
+  kernel<<<dim3((unsigned)ceil_div(BH * slabs, 4 / wps), (unsigned)count), LR_THREADS, 0, st>>>(c, all, slabs, wps);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }

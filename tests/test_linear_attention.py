@@ -82,7 +82,7 @@ def _run(h, d, scale=1.0, backward=True, use_state=True, accumulate=False, start
 
 # time, batch, heads, key/value heads, dk, dv: one token, chunk borders, lengths off every tile, many chunks, all head
 # sizes of the tiles and between them, shared heads, more blocks than the GPU holds at once
-SHAPES = [(1, 1, 1, 1, 1, 1), (1, 3, 4, 2, 64, 64), (2, 2, 2, 2, 8, 8), (15, 1, 2, 1, 16, 16), (16, 2, 2, 2, 32, 32), (17, 2, 3, 3, 33, 31),
+SHAPES = [(1, 1, 1, 1, 1, 1), (3, 300, 4, 2, 16, 96), (4, 300, 2, 1, 30, 64), (8, 400, 2, 2, 64, 40), (7, 200, 4, 2, 128, 124), (5, 90, 3, 3, 52, 15), (8, 3, 2, 2, 127, 126), (1, 3, 4, 2, 64, 64), (2, 2, 2, 2, 8, 8), (15, 1, 2, 1, 16, 16), (16, 2, 2, 2, 32, 32), (17, 2, 3, 3, 33, 31),
           (63, 2, 2, 2, 64, 64), (64, 2, 2, 2, 64, 64), (65, 2, 2, 2, 64, 64), (128, 3, 4, 4, 128, 128), (129, 2, 6, 2, 40, 72),
           (200, 3, 4, 1, 128, 17), (200, 3, 2, 2, 5, 128), (333, 2, 2, 2, 96, 64), (700, 1, 2, 2, 64, 128), (31, 40, 8, 8, 16, 16),
           (1100, 1, 1, 1, 48, 48), (2500, 1, 2, 1, 32, 64)]
@@ -176,7 +176,9 @@ def test_strided_views_and_row_order(handler, T):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize('shape', [(1, 1, 1, 1, 1), (1, 16, 16, 64, 64), (5, 6, 2, 33, 18), (300, 4, 4, 128, 128), (7, 8, 4, 16, 128), (64, 3, 1, 96, 50)])
+@pytest.mark.parametrize('shape', [(1, 1, 1, 1, 1), (1, 16, 16, 64, 64), (5, 6, 2, 33, 18), (300, 4, 4, 128, 128), (7, 8, 4, 16, 128), (64, 3, 1, 96, 50),
+                                   (700, 2, 2, 16, 96), (700, 3, 1, 12, 12), (350, 4, 2, 24, 64), (350, 2, 2, 30, 20), (400, 3, 3, 64, 32), (300, 4, 2, 57, 68),
+                                   (90, 8, 4, 52, 15), (5, 2, 2, 127, 127), (200, 4, 4, 97, 64)])
 def test_steps_are_the_recurrence(handler, shape):
     """Token by token with the state in place, against the whole sequence in 64 bits."""
     h, (B, H, K, dk, dv), T = handler, shape, 4
