@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(LR_THREADS, R == 8 ? (ONE ? 6 : 5) : 8) la_rec
 // Any dv and any alignment: a block for the state of one (sequence, head), 32 bits a lane.  Thread: column j, rows
 // rg + groups * r, r < R, in registers.
 template <int R>
-__global__ void __launch_bounds__(1024) la_recurrent_any_kernel(LaCommon c, LaRuns runs, int cols_log2) {
+__global__ void __launch_bounds__(1024, R <= 8 ? 2 : 1) la_recurrent_any_kernel(LaCommon c, LaRuns runs, int cols_log2) {
   __shared__ float qkv[3 * LA_MAX_DIM];
   extern __shared__ float part[];
   const LaRun& p = runs.run[blockIdx.y];
@@ -158,10 +158,13 @@ __global__ void __launch_bounds__(1024) la_recurrent_any_kernel(LaCommon c, LaRu
   const int64_t state = (int64_t)bh * dk * dv;
   float S[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = rg + groups * r;
-    S[r] = 0.f;
-    if (p.s_in && i < dk && j < dv) S[r] = p.s_in_t ? p.s_in[state + j * dk + i] : p.s_in[state + i * dv + j];
+  for (int r = 0; r < R; ++r) S[r] = 0.f;
+  if (p.s_in && j < dv) {
+    const float* s = p.s_in + state + (p.s_in_t ? j * dk + rg : rg * dv + j);
+    const int next = groups * (p.s_in_t ? 1 : dv);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (rg + groups * r < dk) S[r] = s[r * next];
   }
   for (int step = 0; step < n; ++step) {
     const float *qt = q + dir * step * p.qs.t, *kt = k + dir * step * p.ks.t, *vt = v + dir * step * p.vs.t;
@@ -194,13 +197,12 @@ __global__ void __launch_bounds__(1024) la_recurrent_any_kernel(LaCommon c, LaRu
   if (!p.accumulate)       // tokens behind the end of the sequence
     for (int64_t t = n; t < c.T; ++t)
       for (int i = tid; i < dv; i += threads) o[t * p.os.t + i] = 0.f;
-  if (p.s_out) {
+  if (p.s_out && j < dv) {
     const float f = (p.reverse && n > 0) ? l : 1.f;
+    float* s = p.s_out + state + rg * dv + j;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int i = rg + groups * r;
-      if (i < dk && j < dv) p.s_out[state + i * dv + j] = f * S[r];
-    }
+    for (int r = 0; r < R; ++r)
+      if (rg + groups * r < dk) s[r * groups * dv] = f * S[r];
   }
 }
 
