@@ -193,15 +193,20 @@ B200_API int b200_muon_update(float* param, const float* grad, float* momentum, 
   const dim3 tiles((unsigned)ceil_div(cols, 64), (unsigned)ceil_div(rows, 64), (unsigned)batch);
   muon_start_kernel<<<tiles, 256, 0, st>>>(grad, momentum, beta, nesterov, partial, (int)nb, X[0]);
   B200_LAUNCH_CHECK();
-  int now = 0;
-  for (int i = 0; i < steps; ++i, now ^= 1) {
-    const NsMatrix& x = X[now];
-    NsMatrix* y = &X[now ^ 1];
-    if (int rc = ns_gemm(x, tall, x, tall, &D, (int)batch, 1.f, NS_B / (2.f * NS_C), true)) return rc;       // from X X^T, or X^T X
-    if (int rc = ns_gemm(D, false, D, false, &P, (int)batch, NS_C, NS_A - NS_B * NS_B / (4.f * NS_C), true)) return rc;
-    const int rc = tall ? ns_gemm(x, false, P, false, y, (int)batch, 1.f, 0.f, false)              // X P, P symmetric
-                        : ns_gemm(P, false, x, true, y, (int)batch, 1.f, 0.f, false);              // P X
-    if (rc) return rc;
+  constexpr float d_diagonal = NS_B / (2.f * NS_C), p_diagonal = NS_A - NS_B * NS_B / (4.f * NS_C);
+  int now = steps & 1;
+  if (steps > 0 && ns_chain_fits(rows, cols, batch)) {
+    if (int rc = ns_chain(X, D, P, tall, (int)batch, steps, d_diagonal, NS_C, p_diagonal)) return rc;
+  } else {
+    for (int i = 0; i < steps; ++i) {
+      const NsMatrix& x = X[i & 1];
+      NsMatrix* y = &X[~i & 1];
+      if (int rc = ns_gemm(x, tall, x, tall, &D, (int)batch, 1.f, d_diagonal, true)) return rc;       // from X X^T, or X^T X
+      if (int rc = ns_gemm(D, false, D, false, &P, (int)batch, NS_C, p_diagonal, true)) return rc;
+      const int rc = tall ? ns_gemm(x, false, P, false, y, (int)batch, 1.f, 0.f, false)              // X P, P symmetric
+                          : ns_gemm(P, false, x, true, y, (int)batch, 1.f, 0.f, false);              // P X
+      if (rc) return rc;
+    }
   }
   const unsigned eb = (unsigned)std::min<int64_t>(ceil_div(size, 2048), (int64_t)state().sm_count * 8);
   const bool whole = cols % 8 == 0 && aligned16(update) && aligned16(param);

@@ -20,7 +20,9 @@
 //    4096 x 4096 update took 4.6 ms, with 128 it takes 3.7.
 //  * Roles (320 threads): warp 0 TMA, warp 1 MMA and tensor memory, warps 2 to 9 drain and epilogue (a lane owns
 //    a row; two groups of four warps own half the columns each).  One thread issues the MMAs; the descriptors
-//    of stages and steps are additions to one (with a descriptor built for each, issue took 180 clocks an MMA).
+//    of stages and steps are additions to one (with a descriptor built for each, issue took 180 clocks an MMA), and the
+//    thread is elected, not picked by lane == 0, so that they stay in uniform registers (twelve MMAs: 500 to 660 clocks
+//    to issue instead of 1000 to 1380; a 4096 x 4096 update 4.21 -> 3.88 ms).
 //  * A symmetric product computes and stores the blocks on and above the diagonal.  Where a product needs a block
 //    below it, the block above is loaded as an MN-major operand in its place: K-block by K-block, the
 //    instruction descriptor says which.  (Storing both halves made the epilogue cost 0.15 ms of a 0.51 ms update of four
@@ -104,7 +106,18 @@ static int ns_tiles(int tiles_m, int tiles_n, int bm, int bn, bool symmetric) {
   return n;
 }
 
-__device__ __forceinline__ uint32_t ns_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// two values as (hi, hi) and (lo, lo): lo = fp16(x - hi), the difference in one mixed-precision operation
+__device__ __forceinline__ void ns_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  asm("{\n\t.reg .f32 r0, r1;\n\t.reg .b16 h0, h1, m;\n\t"
+      "cvt.rn.f16x2.f32 %0, %3, %2;\n\t"
+      "mov.b32 {h0, h1}, %0;\n\t"
+      "mov.b16 m, 0xBC00;\n\t"                       // -1
+      "fma.rn.f32.f16 r0, h0, m, %2;\n\t"
+      "fma.rn.f32.f16 r1, h1, m, %3;\n\t"
+      "cvt.rn.f16x2.f32 %1, r1, r0;\n\t}"
+      : "=&r"(hi), "=r"(lo)
+      : "f"(x), "f"(y));
+}
 
 // W columns (64 or 32) of a warp's 32 rows: from acc (lane: row row0 + lane; columns col ..) to the planes.  Rows go
 // through shared memory (`buf`, this warp's: both planes, 32 rows of W halves and 16 bytes), so that whole rows of a
@@ -120,17 +133,11 @@ __device__ __forceinline__ void ns_store(const float* acc, uint8_t* buf, const N
 #pragma unroll
   for (int c8 = 0; c8 < W / 8; ++c8) {
     uint32_t hi[4], lo[4];
+    float x[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int c = 8 * c8 + 2 * u;
-      float x = alpha * acc[c], y = alpha * acc[c + 1];
-      if (on == c) x += diagonal;
-      if (on == c + 1) y += diagonal;
-      const __half2 h = __floats2half2_rn(x, y);
-      const float2 f = __half22float2(h);
-      hi[u] = ns_bits(h);
-      lo[u] = ns_bits(__floats2half2_rn(x - f.x, y - f.y));
-    }
+    for (int u = 0; u < 8; ++u) x[u] = alpha * acc[8 * c8 + u] + (on == 8 * c8 + u ? diagonal : 0.f);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) ns_split(x[2 * u], x[2 * u + 1], hi[u], lo[u]);
     *reinterpret_cast<uint4*>(mine + 16 * c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4*>(mine + PLANE + 16 * c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
@@ -221,6 +228,8 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   if (warp == 0 && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a_mn) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b_mn) : "memory");
   }
   if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
   tc_fence_before();
@@ -230,7 +239,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   pdl_wait();       // operands and outputs belong to the kernel before until here
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       asm volatile("fence.proxy.async;" ::: "memory");      // the planes were written by ordinary stores
       int issued = 0;
       for (int kb = 0; kb < num_kb; ++kb) {
@@ -249,7 +258,7 @@ ns_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       // D = F32, A = B = F16, N >> 3, M >> 4; the majors are set for each k-block
       const uint32_t idesc0 = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(NS_BM >> 4) << 24);
       // descriptors of stage 0; stages, planes and steps along K are additions to their address field (16-byte units)
@@ -365,6 +374,8 @@ ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   if (warp == 0 && lane == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a_mn) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b_mn) : "memory");
   }
   if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), Cfg::TMEM_COLS);
   tc_fence_before();
@@ -375,7 +386,7 @@ ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   pdl_wait();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       asm volatile("fence.proxy.async;" ::: "memory");
       int issued = 0;
       for (int kb = 0; kb < num_kb; ++kb) {
@@ -394,12 +405,13 @@ ns_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 1) {
+    const bool one = elect_one();
+    if (one && rank == 1) {
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!mbar_wait(full_bar(kb % S), (kb / S) & 1, abort_flag)) break;
         mbar_arrive_cluster(cluster_addr(peer_bar(kb % S), 0));
       }
-    } else if (lane == 0) {
+    } else if (one) {
       // D = F32, A = B = F16, N >> 3, M >> 4; the majors are set for each k-block
       const uint32_t idesc0 = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
       // descriptors of stage 0; stages, planes and steps along K are additions to their address field (16-byte units)
@@ -545,6 +557,241 @@ int ns_gemm(const NsMatrix& a, bool a_t, const NsMatrix& b, bool b_t, NsMatrix* 
   cfg.numAttrs = 1;
   B200_CUDA(cudaLaunchKernelEx(&cfg, best->kernel, ma, ma_mn, mb, mb_mn, e, M, N, K, batch, a.upper ? a.upper : (int)a_t, b.upper ? b.upper : (int)b_t,
                                symmetric ? 1 : 0, flag));
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
+// ---- the whole iteration in one launch, for matrices of a few tiles
+//
+// A product of such matrices is all latency: launched one by one, those of 205 x 256 take 6.2 us each (an update 107.7 us,
+// 96.3 in a recorded graph), of which the tensor pipe has work for one.  Here a cluster of up to eight CTAs computes all
+// of them for one matrix of the stack: the operands stay in L2, barriers and tensor memory are set up once, and between two
+// products stands a barrier of the cluster (with a fence between the stores of the one and the TMA loads of the next)
+// instead of a launch: 90.6 us, 88.1 recorded; 64 x 64: 65.8 -> 57.5, eight of 128 x 256: 95.4 -> 81.6.  Of a product's
+// 9000 clocks then 1500 are the way to the first MMA, 4000 the four K-blocks (loads and MMAs share the 128 bytes a clock
+// of shared memory), 2000 the epilogue, 1500 fence and barrier.
+// With two tiles a CTA it lost (256 x 500: 122.6 recorded against 116.0), as with more clusters than fit the GPU together
+// (sixteen of 256 x 256: 178 against 116): each CTA has one tile, and there are at most 64 tiles.
+constexpr int NC_CTAS = 8;
+
+struct NsChain {
+  __half* data[4];                                   // X, the other X, D, P
+  int ld[4];
+  int rows, cols, m, steps, tall, batch;
+  float d_diagonal, p_alpha, p_diagonal;
+};
+// ROWS rows of an operand as ns_load, with one map for both majors: the boxes are 64 x 64 either way.
+template <int ROWS>
+__device__ __forceinline__ void ns_chain_load(uint32_t at, const CUtensorMap* map, bool mn, int k0, int r0, int batch, int b, uint32_t bar) {
+#pragma unroll
+  for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+    for (int j = 0; j < ROWS / 64; ++j)
+      tma_load_3d(at + plane * ROWS * 128 + j * 8192, map, mn ? r0 + 64 * j : k0, mn ? k0 : r0 + 64 * j, plane * batch + b, bar);
+}
+
+struct NcConfig : NsConfig<64, false> {
+  static constexpr int STAGES = 3, OUT_BYTES = 8 * 2 * 32 * (W * 2 + 16);
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;
+};
+
+__global__ void __launch_bounds__(NS_THREADS, 1)
+ns_chain_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1, const __grid_constant__ CUtensorMap map2,
+                const __grid_constant__ CUtensorMap map3, const __grid_constant__ NsChain c, int* error_flag) {
+  using Cfg = NcConfig;
+  constexpr int S = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK;
+  static_assert(Cfg::CHUNK == 1 && BK == 64, "a stage is a chunk");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S * Cfg::STAGE_BYTES + Cfg::OUT_BYTES);
+  // bars[0..S) full, [S..2S) empty, [2S..2S+2) chunk ready, [2S+2..2S+4) chunk drained
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.y, rank = blockIdx.x;       // a cluster is a row of the grid
+  const uint32_t bar0 = smem_u32(bars), smem_base = smem_u32(smem);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (S + s); };
+  auto acc_full_bar = [&](int i) { return bar0 + 8u * (2 * S + i); };
+  auto acc_empty_bar = [&](int i) { return bar0 + 8u * (2 * S + 2 + i); };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full_bar(i), 1);
+      mbar_init(acc_empty_bar(i), 8);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map0) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map1) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map2) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map3) : "memory");
+  }
+  if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_d = *tmem_slot;
+
+  // Every role counts its stages (a stage is a chunk) through all products.
+  int s = 0, phase = 0, buf = 0, buf_phase = 0;
+  uint32_t issued = 0;
+  bool ok = true;
+  auto advance = [&]() {
+    if (++s == S) s = 0, phase ^= 1;
+    buf ^= 1;
+    if (buf == 0) buf_phase ^= 1;
+  };
+  // this CTA's tile of D and P, and of X: row tile << 16 | column tile, -1 for none
+  int mine[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int M = w == 0 ? c.m : c.rows, N = w == 0 ? c.m : c.cols;
+    int ti = 0, tj = 0;
+    const bool any = ns_tile(rank, (M + NS_BM - 1) / NS_BM, (N + BN - 1) / BN, NS_BM, BN, w == 0, &ti, &tj);
+    mine[w] = any ? ti << 16 | tj : -1;
+  }
+  pdl_wait();
+  asm volatile("fence.proxy.async;" ::: "memory");      // X was written by ordinary stores
+  for (int x = 0, step = 0; step < c.steps; ++step, x ^= 1) {
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+      // D = X X^T (X^T X) + .. I, P = c D D + .. I, X' = P X (X P)
+      const CUtensorMap* map_x = x ? &map1 : &map0;
+      const CUtensorMap* map_a = w == 0 ? map_x : w == 1 ? &map2 : c.tall ? map_x : &map3;
+      const CUtensorMap* map_b = w == 0 ? map_x : w == 1 ? &map2 : c.tall ? &map3 : map_x;
+      const int a_lies = w == 0 ? c.tall : w == 1 || !c.tall ? 128 : 0, b_lies = w == 0 ? c.tall : w == 1 || c.tall ? 128 : 1;
+      const int M = w < 2 ? c.m : c.rows, N = w < 2 ? c.m : c.cols, K = w > 0 ? c.m : c.tall ? c.rows : c.cols;
+      const int num_kb = (K + BK - 1) / BK;
+      const int t = mine[w == 2];
+      if (t >= 0 && ok) {
+        const int m0 = (t >> 16) * NS_BM, n0 = (t & 0xffff) * BN;
+        if (warp == 0) {
+          if (elect_one()) {
+            for (int kb = 0; kb < num_kb; ++kb) {
+              ok = mbar_wait(empty_bar(s), phase ^ 1, abort_flag);
+              if (!ok) break;
+              mbar_expect_tx(full_bar(s), Cfg::STAGE_BYTES);
+              const uint32_t at = smem_base + s * Cfg::STAGE_BYTES;
+              ns_chain_load<NS_BM>(at, map_a, ns_mn(a_lies, m0, kb * BK), kb * BK, m0, c.batch, b, full_bar(s));
+              ns_chain_load<BN>(at + 2 * Cfg::A_BYTES, map_b, ns_mn(b_lies, n0, kb * BK), kb * BK, n0, c.batch, b, full_bar(s));
+              ++issued;
+              advance();
+            }
+          }
+        } else if (warp == 1) {
+          if (elect_one()) {
+            const uint32_t idesc0 = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(NS_BM >> 4) << 24);
+            const uint64_t da_k = Cfg::desc_k(smem_base), da_mn = Cfg::desc_mn(smem_base);
+            const uint64_t db_k = Cfg::desc_k(smem_base + 2 * Cfg::A_BYTES), db_mn = Cfg::desc_mn(smem_base + 2 * Cfg::A_BYTES);
+            for (int kb = 0; kb < num_kb; ++kb) {
+              ok = mbar_wait(acc_empty_bar(buf), buf_phase ^ 1, abort_flag) && mbar_wait(full_bar(s), phase, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              const bool a_mn = ns_mn(a_lies, m0, kb * BK), b_mn = ns_mn(b_lies, n0, kb * BK);
+              const uint32_t idesc = idesc0 | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
+              const uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+              const uint32_t d = tmem_d + (uint32_t)(buf * BN);
+              const uint64_t ah = (a_mn ? da_mn : da_k) + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), al = ah + (Cfg::A_BYTES >> 4);
+              const uint64_t bh = (b_mn ? db_mn : db_k) + (uint64_t)(s * (Cfg::STAGE_BYTES >> 4)), bl = bh + (Cfg::B_BYTES >> 4);
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) {
+                mma_f16(d, al + a_step * k, bh + b_step * k, idesc, k > 0);
+                mma_f16(d, ah + a_step * k, bl + b_step * k, idesc, 1);
+              }
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) mma_f16(d, ah + a_step * k, bh + b_step * k, idesc, 1);
+              mma_commit(empty_bar(s));
+              mma_commit(acc_full_bar(buf));
+              advance();
+            }
+          }
+        } else {
+          const int q = warp & 3, group = (warp - 2) >> 2;
+          float acc[Cfg::ACC];
+#pragma unroll
+          for (int j = 0; j < Cfg::ACC; ++j) acc[j] = 0.f;
+          for (int kb = 0; kb < num_kb; ++kb) {
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full_bar(buf), buf_phase, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            drain_add<Cfg::ACC>(tmem_d + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + group * Cfg::ACC), acc);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty_bar(buf));
+            advance();
+          }
+          const int row0 = m0 + q * 32, col0 = n0 + group * Cfg::ACC;
+          if (ok && row0 < M && col0 < N) {
+            const int out = w < 2 ? 2 + w : x ^ 1, ld = c.ld[out];
+            const NsOut e = {c.data[out] + (int64_t)b * M * ld, ld, (w == 1 ? c.p_alpha : 1.f) * NS_GAIN, w == 0 ? c.d_diagonal : w == 1 ? c.p_diagonal : 0.f};
+            ns_store<Cfg::W>(acc, smem + S * Cfg::STAGE_BYTES + (warp - 2) * 2 * 32 * (Cfg::W * 2 + 16), e, (int64_t)c.batch * M * ld, row0, col0, M);
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      // the product is complete before anyone loads it: stores, fence, barrier, TMA
+      __syncwarp();
+      if (warp >= 2) asm volatile("fence.proxy.async;" ::: "memory");
+      cluster_sync_all();
+    }
+  }
+  if (warp == 0 && issued && *abort_flag) {      // copies already issued must land before shared memory is released
+    for (uint32_t k = issued > S ? issued - S : 0; k < issued; ++k)
+      for (uint32_t n = 0; n < TC_SPIN_LIMIT && !mbar_try_wait(full_bar(k % S), (k / S) & 1); ++n) __nanosleep(64);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_d, Cfg::TMEM_COLS);
+  }
+  if (threadIdx.x == 0 && *abort_flag && error_flag) *error_flag = 1;
+}
+
+static int ns_chain_tiles(int64_t rows, int64_t cols) { return (int)(ceil_div(rows, NS_BM) * ceil_div(cols, 64)); }
+
+bool ns_chain_fits(int64_t rows, int64_t cols, int64_t batch) {
+  return rows <= 4096 && cols <= 4096 && ns_chain_tiles(rows, cols) <= NC_CTAS && batch * ns_chain_tiles(rows, cols) <= 64;
+}
+
+int ns_chain(const NsMatrix* X, const NsMatrix& D, const NsMatrix& P, bool tall, int batch, int steps, float d_diagonal, float p_alpha, float p_diagonal) {
+  static bool ready = false;
+  if (!ready) {
+    B200_CUDA(cudaFuncSetAttribute(ns_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NcConfig::SMEM_BYTES));
+    ready = true;
+  }
+  int* flag = device_error_flag();
+  B200_REQUIRE(flag != nullptr, "the device error flag cannot be set up");
+  int ctas = 1;
+  const int full = ns_chain_tiles(X[0].rows, X[0].cols);
+  while (ctas < full && ctas < NC_CTAS) ctas *= 2;
+  const NsChain c = {{X[0].data, X[1].data, D.data, P.data}, {X[0].ld, X[1].ld, D.ld, P.ld}, X[0].rows, X[0].cols, D.rows, steps, tall ? 1 : 0, batch, d_diagonal, p_alpha, p_diagonal};
+  CUtensorMap maps[4];
+  const NsMatrix* all[4] = {&X[0], &X[1], &D, &P};
+  for (int i = 0; i < 4; ++i)
+    if (int rc = ns_map(*all[i], true, batch, 64, &maps[i])) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, (unsigned)batch);
+  cfg.blockDim = dim3(NS_THREADS);
+  cfg.dynamicSmemBytes = NcConfig::SMEM_BYTES;
+  cfg.stream = state().stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  B200_CUDA(cudaLaunchKernelEx(&cfg, ns_chain_kernel, maps[0], maps[1], maps[2], maps[3], c, flag));
   B200_LAUNCH_CHECK();
   return B200_OK;
 }

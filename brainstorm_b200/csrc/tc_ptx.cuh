@@ -13,6 +13,18 @@ constexpr uint32_t TC_SPIN_LIMIT = 1u << 22;
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
+// True for one lane of a converged warp, the same one every time.  Behind this branch, unlike behind lane == 0, the compiler
+// knows that one thread runs, and keeps coordinates, descriptors and barriers in the uniform registers that TMA and
+// tcgen05 instructions take them from.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one)::"memory");
+  return one != 0;
+}
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }

@@ -67,6 +67,13 @@ def test_update(handler, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(256, 256), (1000, 60), (60, 512), (128, 513), (1, 1), (129, 250), (8, 250, 65), (64, 17, 30), (65, 17, 30), (3, 40, 1)])
+def test_around_the_limits_of_a_single_launch(handler, shape):
+    """Up to eight tiles of 128 x 64 a matrix and 64 in all run as one launch, more product by product."""
+    _check(handler, _case(shape, seed=sum(shape)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('steps', [0, 1, 2, 3, 8])
 @pytest.mark.parametrize('shape', [(30, 50), (200, 150)])
 def test_steps(handler, shape, steps):
