@@ -31,6 +31,7 @@ def sources():
 
 def _newest_header():
     hs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(('.cuh', '.h'))]
+    hs.append(os.path.join(os.path.dirname(PKG), 'include', 'b200_handler.h'))      # argument structs
     return max([os.path.getmtime(h) for h in hs] + [os.path.getmtime(__file__)])
 
 

@@ -21,6 +21,7 @@
 #include <initializer_list>
 #include <utility>
 
+#include "../../include/b200_handler.h"
 #include "common.cuh"
 
 namespace b200 {
@@ -517,11 +518,10 @@ using namespace b200;
    : s.threads == 512 ? KERNEL<8, GN_SINGLE, 512>                                                                        \
                       : (s.E == 4 ? KERNEL<4, GN_SINGLE, 256> : KERNEL<8, GN_SINGLE, 256>))
 
-B200_API int b200_gated_norm_forward(const float* x, const float* y, const float* gate, const float* w_post, const float* scale,
-                                     const float* w_pre, float* x_out, float* h_out, float* r_post, float* r_pre, int64_t rows,
-                                     int64_t width, int64_t ld_x, int64_t ld_y, int64_t ld_gate, int64_t ld_x_out, int64_t ld_h_out,
-                                     float eps, int act) {
+B200_API int b200_gated_norm_forward(const b200_gated_norm_args* args) {
   if (int rc = require_ready()) return rc;
+  B200_REQUIRE(args, "gated norm: NULL arguments");
+  const auto& [x, y, gate, w_post, scale, w_pre, x_out, h_out, r_post, r_pre, rows, width, ld_x, ld_y, ld_gate, ld_x_out, ld_h_out, eps, act] = *args;
   B200_REQUIRE(rows >= 0 && width >= 0, "negative extent");
   B200_REQUIRE(width <= GN_MAX_WIDTH, "gated norm: rows of more than %d values are not supported", GN_MAX_WIDTH);
   B200_REQUIRE(act >= 0 && act <= 4, "unknown activation %d", act);

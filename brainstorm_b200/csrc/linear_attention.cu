@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "../../include/b200_handler.h"
 #include "linear_attention.cuh"
 
 namespace b200 {
@@ -302,10 +303,10 @@ B200_API int64_t b200_linear_attention_forward_scratch_floats(int64_t T, int64_t
   return la_chunked_work(T, B * H, (int)dk, (int)dv, false);
 }
 
-B200_API int b200_linear_attention_forward(const float* q, const float* k, const float* v, const float* decay, float* out, const float* state,
-                                           float* state_out, const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads,
-                                           int64_t dk, int64_t dv, const int64_t* strides, float scale, float* scratch, int64_t scratch_floats) {
+B200_API int b200_linear_attention_forward(const b200_linear_attention_args* args) {
   if (int rc = require_ready()) return rc;
+  B200_REQUIRE(args, "linear attention: NULL arguments");
+  const auto& [q, k, v, decay, out, state, state_out, lengths, strides, scratch, scratch_floats, T, B, H, kv_heads, dk, dv, scale] = *args;
   if (int rc = la_check("linear attention", T, B, H, kv_heads, dk, dv)) return rc;
   if (B * H == 0) return B200_OK;
   B200_REQUIRE(scratch_floats >= b200_linear_attention_forward_scratch_floats(T, B, H, dk, dv), "linear attention: scratch too small");

@@ -413,25 +413,41 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      may be dx_out.  scratch of b200_gated_norm_scratch_floats(rows, width) floats for the
  *      vectors' partial sums.
  *
+ *      The two forward calls, which also serve single tokens, take their arguments in one struct: a
+ *      caller that has to convert every argument of a call (ctypes) spent a third of a step on them.
+ *
  *      muon_update, for `batch` contiguous (rows, cols) matrices: momentum = beta momentum +
  *      grad; u = grad + beta momentum if nesterov, else momentum; X = u / (|u|_F + 1e-7);
  *      `steps` times X = a X + (b A + c A A) X with A = X X^T and (a, b, c) = (3.4445,
  *      -4.7750, 2.0315); update = X; param = (1 - learning_rate * weight_decay) param -
  *      learning_rate * X.  16-byte aligned scratch of b200_muon_scratch_floats floats.  The
  *      four arrays must not overlap. ---------------------------------------------------- */
-int b200_linear_attention_forward(const float* q, const float* k, const float* v, const float* decay, float* out, const float* state,
-                                  float* state_out, const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads,
-                                  int64_t dk, int64_t dv, const int64_t* strides, float scale, float* scratch, int64_t scratch_floats);
+typedef struct {
+  const float *q, *k, *v, *decay;
+  float* out;
+  const float* state;
+  float* state_out;
+  const float* lengths;
+  const int64_t* strides;
+  float* scratch;
+  int64_t scratch_floats, T, B, H, kv_heads, dk, dv;
+  float scale;
+} b200_linear_attention_args;
+int b200_linear_attention_forward(const b200_linear_attention_args* args);
 int64_t b200_linear_attention_forward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t dk, int64_t dv);
 int64_t b200_linear_attention_backward_scratch_floats(int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv);
 int b200_linear_attention_backward(const float* q, const float* k, const float* v, const float* decay, const float* dout, float* dq,
                                    float* dk_out, float* dv_out, const float* state, const float* dstate_out, float* dstate,
                                    const float* lengths, int64_t T, int64_t B, int64_t H, int64_t kv_heads, int64_t dk, int64_t dv,
                                    const int64_t* strides, float scale, int accumulate, float* scratch, int64_t scratch_floats);
-int b200_gated_norm_forward(const float* x, const float* y, const float* gate, const float* w_post, const float* scale,
-                            const float* w_pre, float* x_out, float* h_out, float* r_post, float* r_pre, int64_t rows,
-                            int64_t width, int64_t ld_x, int64_t ld_y, int64_t ld_gate, int64_t ld_x_out, int64_t ld_h_out,
-                            float eps, int act);
+typedef struct {
+  const float *x, *y, *gate, *w_post, *scale, *w_pre;
+  float *x_out, *h_out, *r_post, *r_pre;
+  int64_t rows, width, ld_x, ld_y, ld_gate, ld_x_out, ld_h_out;
+  float eps;
+  int act;
+} b200_gated_norm_args;
+int b200_gated_norm_forward(const b200_gated_norm_args* args);
 int64_t b200_gated_norm_scratch_floats(int64_t rows, int64_t width);
 int b200_gated_norm_backward(const float* x_out, const float* y, const float* gate, const float* w_post, const float* scale,
                              const float* w_pre, const float* r_post, const float* r_pre, const float* dx_out, const float* dh,
