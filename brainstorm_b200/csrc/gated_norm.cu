@@ -189,7 +189,8 @@ __device__ __forceinline__ float gn_row_sum(float v, int G, float* smem) {
 
 template <int E, int MODE, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) gated_norm_forward_kernel(GatedNorm p, int G) {
-  constexpr bool KEEP = MODE == GN_SHIFT;      // the weights in registers: their loads are single
+  // the weights in registers from the start: where their loads are single, or few rows leave their latency bare
+  constexpr bool KEEP = MODE == GN_SHIFT || E == 4;
   __shared__ float red[32];
   const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
   const float inv_width = 1.f / (float)p.width;
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) 
 // Shared memory: three vectors of column sums for each group of G threads (gn_sum_into).
 template <int E, int MODE, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 2 : 3) gated_norm_backward_kernel(GatedNormGrad p, int G) {
-  constexpr bool KEEP = MODE == GN_SHIFT;
+  constexpr bool KEEP = MODE == GN_SHIFT || E == 4;
   extern __shared__ float4 sums[];
   __shared__ float red[32];
   const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
@@ -470,6 +471,14 @@ static GnShape gn_geometry(int64_t rows, int width, int mode, bool backward) {
   s.mode = mode;
   const int span = width + (mode == GN_SHIFT ? 3 : 0);
   s.E = span <= 128 ? 4 : (span <= 256 || (mode != GN_VEC && span <= 8192)) ? 8 : 16;
+  // Few rows: a call is the latency of one row, which is shorter with 4 floats a thread, as long as all rows are resident
+  // at once (128 x 1000: forward 4.6 -> 3.3 us, backward 14.9 -> 7.0; 592 x 1000: 4.8 -> 4.5, 15.5 -> 12.7; forward of 400 x 2000
+  // 5.6 -> 8.2, of 64 x 4096 4.6 -> 5.5: fewer, wider blocks fit).
+  if (mode != GN_SINGLE && span <= (mode == GN_VEC && backward ? 4096 : 2048)) {
+    int G = 32;
+    while (G * 4 < span) G *= 2;
+    if (ceil_div(rows, std::max(1, 256 / G)) * (backward ? 1 : std::max(1, G / 256)) <= 4 * state().sm_count) s.E = 4;
+  }
   s.G = 32;
   while (s.G * s.E < span) s.G *= 2;
   s.threads = std::max(s.G, 256);
@@ -481,6 +490,9 @@ static GnShape gn_geometry(int64_t rows, int width, int mode, bool backward) {
     while (s.blocks * s.per_block % 4) --s.blocks;
   return s;
 }
+// Widths of the shifted form: a row and its offset fit 512 or 1024 threads with 8 floats each, and fill most of them
+// (2000 x 5001: forward 124 -> 91 us, backward 198 -> 129 against single loads; 500 x 4095: 19 -> 29, 36 -> 44).
+static bool gn_shiftable(int width) { return width + 3 <= 4096 || (width >= 4800 && width + 3 <= 8192); }
 // Rows of partial sums that a backward call leaves.
 static int64_t gn_partial_rows(int64_t rows, const GnShape& s) {
   return s.mode == GN_SHIFT ? std::min<int64_t>(rows, (int64_t)s.blocks * s.per_block) : s.blocks;
@@ -500,8 +512,7 @@ static GnShape gn_shape(int64_t rows, int width, std::initializer_list<std::pair
     pitch = a.second;
   }
   for (const void* v : vectors) vec = vec && aligned16(v);
-  // a row and its offset have to fit 512 x 8 in the shifted form
-  return gn_geometry(rows, width, vec ? GN_VEC : alike && width <= 4096 - 3 ? GN_SHIFT : GN_SINGLE, backward);
+  return gn_geometry(rows, width, vec ? GN_VEC : alike && gn_shiftable(width) ? GN_SHIFT : GN_SINGLE, backward);
 }
 
 }  // namespace b200
@@ -510,9 +521,10 @@ using namespace b200;
 
 // Rows of up to 4096 values (2045 in the shifted form): blocks of 256 threads; wider ones: one row for a block of 512 or 1024.
 #define GN_KERNELS(KERNEL)                                                                                               \
-  (s.mode == GN_VEC ? (s.threads == 1024 ? KERNEL<16, GN_VEC, 1024> : s.threads == 512 ? KERNEL<16, GN_VEC, 512>         \
+  (s.mode == GN_VEC ? (s.threads == 1024 ? (s.E == 4 ? KERNEL<4, GN_VEC, 1024> : KERNEL<16, GN_VEC, 1024>)               \
+                       : s.threads == 512 ? (s.E == 4 ? KERNEL<4, GN_VEC, 512> : KERNEL<16, GN_VEC, 512>)                 \
                        : s.E == 4 ? KERNEL<4, GN_VEC, 256> : s.E == 8 ? KERNEL<8, GN_VEC, 256> : KERNEL<16, GN_VEC, 256>) \
-   : s.mode == GN_SHIFT ? (s.threads == 512 ? KERNEL<8, GN_SHIFT, 512>                                                   \
+   : s.mode == GN_SHIFT ? (s.threads == 1024 ? KERNEL<8, GN_SHIFT, 1024> : s.threads == 512 ? (s.E == 4 ? KERNEL<4, GN_SHIFT, 512> : KERNEL<8, GN_SHIFT, 512>) \
                            : s.E == 4 ? KERNEL<4, GN_SHIFT, 256> : KERNEL<8, GN_SHIFT, 256>)                             \
    : s.threads == 1024 ? (s.E == 8 ? KERNEL<8, GN_SINGLE, 1024> : KERNEL<16, GN_SINGLE, 1024>)                           \
    : s.threads == 512 ? KERNEL<8, GN_SINGLE, 512>                                                                        \
@@ -545,7 +557,7 @@ B200_API int64_t b200_gated_norm_scratch_floats(int64_t rows, int64_t width) {
   if (rows <= 0 || width <= 0 || width > GN_MAX_WIDTH) return 0;
   int64_t most = 0;       // the form depends on the pointers
   for (int mode : {GN_SINGLE, GN_VEC, GN_SHIFT})
-    if (mode != GN_SHIFT || width <= 4096 - 3) most = std::max(most, gn_partial_rows(rows, gn_geometry(rows, (int)width, mode, true)));
+    if (mode != GN_SHIFT || gn_shiftable(width)) most = std::max(most, gn_partial_rows(rows, gn_geometry(rows, (int)width, mode, true)));
   return most * 3 * width;
 }
 
