@@ -15,12 +15,19 @@
 // between them; the split and the weights want the accumulators in the registers that compute them, where
 // mma.sync leaves them, and the masked half of the scores is skipped in steps of 16.  Measured here:
 // mma.sync fp16 555 TFLOP/s (185 of fp32 accuracy), tf32 277 (92 in three products).  With d = 64 a token
-// and head needs 13.3 k products, 40 clocks of an SM, against 44 clocks of HBM time for its 1 KiB.
+// and head needs 13.3 k products, 40 clocks of an SM, against 44 clocks of HBM time for its 1 KiB.  A form of
+// the outputs on tcgen05 (128 tokens a block, q and the scores in tensor memory, the states of all chunks from the
+// state pass) was right and slower: 8192 x 2 x 16 heads of 128 913 us against 626, since a block that fills
+// shared memory loads, splits, multiplies and stores in a row, and every chunk's state goes through HBM.
 //
 // Few sequences and heads: the time axis is cut into segments.  A first pass computes what each segment adds
 // to the state, a second one hands the state through, then all segments run side by side.
 //
-// Bound: HBM and the tensor pipe about evenly at d = 64, the tensor pipe at d = 128.
+// Bound: neither memory nor the tensor pipe (33 and 25 % of the clocks at d = 128 and 64) but the latency between
+// dependent instructions: registers and shared memory let two or three blocks onto an SM, two or three warps a
+// scheduler, which issue in 36 to 43 % of the clocks.  Measured: 8192 x 2 x 16 heads of 128 608 us (state pass 172, handing
+// through 20, outputs 420), HBM time 83; 100 x 128 x 16 heads of 64 with gradients 469 us, HBM time 114; 1999 x 6 x 12 heads
+// of 48 and 80 over 4, ragged, with gradients 567 us, HBM time 39.
 #include <cuda_fp16.h>
 
 #include <algorithm>

@@ -8,6 +8,10 @@
 // The iteration multiplies from the shorter side: with rows > cols, A = X^T X and X = X P.  P = a I + b A + c A A is
 // computed as c D D + (a - b^2 / 4c) I with D = A + b / 2c I: three plain products a step, whose only addition is
 // to a diagonal.
+//
+// Bound: the products (ns_gemm.cu).  4096 x 4096 takes 3.9 ms, of which they are 3.75 at 366 TFLOP/s of fp32 accuracy
+// (1100 of half precision, at the clocks that the power limit leaves); four of 1000 x 1000 0.40 ms, half of it the first
+// loads and the epilogues of fifteen products that each fill the GPU once; 205 x 256 91 us in one launch.
 #include <algorithm>
 
 #include "common.cuh"

@@ -137,8 +137,8 @@ class SequenceOps(object):
                 ``out`` is zero behind the end of a sequence and the state stays as it was there.  What the
                 inputs hold behind the end is not read.
 
-        dk, dv: 1 to 128.  A non-finite value of a token spreads to later tokens, and may spread to the up to
-        63 tokens before it."""
+        dk, dv: 1 to 128.  A non-finite value of a token spreads to later tokens of its sequence and head, and may
+        spread to up to 15 tokens before it."""
         T, B, H, K, dk, dv = self._attention_shapes(q, k, v, 4)
         _expect(out, (T, B, H, dv), 'out')
         strides = 0
