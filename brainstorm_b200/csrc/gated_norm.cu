@@ -45,6 +45,11 @@ struct GatedNormGrad {
   int width, act, accumulate;
 };
 
+// x^(-1/2): the approximation (two units in the last place) and a Newton step, which 0 and infinity do not take.
+__device__ __forceinline__ float gn_rsqrt(float x) {
+  const float r = rsqrtf(x), e = fmaf(-x * r, r, 1.f);
+  return e == e ? fmaf(0.5f * r, e, r) : r;
+}
 // The activations of the handler (0 sigmoid, 1 tanh, 2 rel, 3 el, 4 linear) and their derivatives as
 // functions of the output.
 __device__ __forceinline__ float gn_act(int act, float x) {
@@ -170,7 +175,8 @@ __device__ __forceinline__ void gn_sum_into(float4* s, const float (&v)[E]) {
   }
 }
 
-// A row on its way into L2: its 128-byte lines are asked for by the row's threads.
+// A row on its way into L2: its 128-byte lines are asked for by the row's threads.  Not with 4 floats a thread, where the
+// instructions of a row count.
 __device__ __forceinline__ void gn_prefetch(const float* row, int width, int G, int t) {
   for (int c = 32 * t; c < width; c += 32 * G) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
 }
@@ -226,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) 
         if (p.gate) gn_load<E, MODE>(g, p.gate + row * p.ld_gate, p.width, G, t, off);
       }
       const int64_t next = row + (int64_t)gridDim.x * per_block;
-      if (next < p.rows) {
+      if (E > 4 && next < p.rows) {
         gn_prefetch(p.x + next * p.ld_x, p.width, G, t);
         if (p.y) gn_prefetch(p.y + next * p.ld_y, p.width, G, t);
         if (p.gate) gn_prefetch(p.gate + next * p.ld_gate, p.width, G, t);
@@ -236,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) 
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) s += y[e] * y[e];
-      const float r = 1.f / sqrtf(gn_row_sum(s, G, red) * inv_width + p.eps);
+      const float r = gn_rsqrt(gn_row_sum(s, G, red) * inv_width + p.eps);
       if (p.gate) {
         gn_act_all<E>(p.act, g);
 #pragma unroll
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) 
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) s += x[e] * x[e];
-      const float r = 1.f / sqrtf(gn_row_sum(s, G, red) * inv_width + p.eps);
+      const float r = gn_rsqrt(gn_row_sum(s, G, red) * inv_width + p.eps);
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = x[e] * r * g[e];
       if (live) {
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 2 : 3) 
         r_post = p.r_post[row];
       }
       const int64_t next = row + (int64_t)gridDim.x * per_block;
-      if (next < p.rows) {
+      if (E > 4 && next < p.rows) {
         if (p.dh) {
           gn_prefetch(p.dh + next * p.ld_dh, p.width, G, t);
           gn_prefetch(p.x_out + next * p.ld_x_out, p.width, G, t);
@@ -493,9 +499,11 @@ static GnShape gn_geometry(int64_t rows, int width, int mode, bool backward) {
     while (s.blocks * s.per_block % 4) --s.blocks;
   return s;
 }
-// Widths of the shifted form: a row and its offset fit 512 or 1024 threads with 8 floats each, and fill most of them
-// (2000 x 5001: forward 124 -> 91 us, backward 198 -> 129 against single loads; 500 x 4095: 19 -> 29, 36 -> 44).
-static bool gn_shiftable(int width) { return width + 3 <= 4096 || (width >= 4800 && width + 3 <= 8192); }
+// Widths of the shifted form: not those that four single loads a lane hold (295099 x 83: forward 198 us shifted, 155 single,
+// backward 329 and 243: the ends of the rows cost more instructions than there are loads); a row and its offset fit 512 or
+// 1024 threads with 8 floats each, and fill most of them (2000 x 5001: forward 124 -> 91 us, backward 198 -> 129 against single
+// loads; 500 x 4095: 19 -> 29, 36 -> 44).
+static bool gn_shiftable(int width) { return width > 128 && (width + 3 <= 4096 || (width >= 4800 && width + 3 <= 8192)); }
 // Rows of partial sums that a backward call leaves.
 static int64_t gn_partial_rows(int64_t rows, const GnShape& s) {
   return s.mode == GN_SHIFT ? std::min<int64_t>(rows, (int64_t)s.blocks * s.per_block) : s.blocks;
