@@ -314,24 +314,39 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
       for (int it = 0; it < QN; ++it, qp += RPP * q_t)
         qr[it] = (it0 + it) * RPP + tid / LPR < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
-    auto put_q = [&](int it0) {      // each row by its own scale: a row lies in LPR neighbouring lanes
+    auto put_q = [&](int it0) {      // each row by its own scale: a row lies in LPR neighbouring lanes; all rows' shuffles together
+      float m[QN];
+      bool inf = false;
+#pragma unroll
+      for (int it = 0; it < QN; ++it) {
+        m[it] = lc_max4<false>(0.f, qr[it]);
+        inf = inf || m[it] == LC_INF;
+      }
+      if (__any_sync(0xffffffffu, inf)) {
+#pragma unroll
+        for (int it = 0; it < QN; ++it) m[it] = lc_max4<true>(0.f, qr[it]);
+      }
+#pragma unroll
+      for (int s = 1; s < LPR; s <<= 1)
+#pragma unroll
+        for (int it = 0; it < QN; ++it) m[it] = fmaxf(m[it], __shfl_xor_sync(0xffffffffu, m[it], s));
 #pragma unroll
       for (int it = 0; it < QN; ++it) {
         const int i = (it0 + it) * RPP + tid / LPR;
-        float m = lc_max4<false>(0.f, qr[it]), inv;
-        if (__any_sync(0xffffffffu, m == LC_INF)) m = lc_max4<true>(0.f, qr[it]);
-#pragma unroll
-        for (int s = 1; s < LPR; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-        const float sc = lc_scale(m, &inv);
+        float inv;
+        const float sc = lc_scale(m[it], &inv);
         lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, kc, L::KP, qr[it], sc);
         if (tid % LPR == 0) q_inv[i] = inv;
       }
     };
     if (QN == KN) load_q(0);
     auto publish = [&](float mk, float mv, float ms) {
-      mk = warp_max(mk);
-      mv = warp_max(mv);
-      ms = warp_max(ms);
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) {      // three chains of shuffles side by side
+        mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, s));
+        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, s));
+        ms = fmaxf(ms, __shfl_xor_sync(0xffffffffu, ms, s));
+      }
       if (lane == 0) {
         red[0][warp] = mk;
         red[1][warp] = mv;
@@ -512,7 +527,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[nt][e] = 0.f;
-#pragma unroll
+#pragma unroll(DK == 64 ? 1 : 4)      // code that follows itself soon stays in the instruction cache
         for (int kt = 0; kt < 4; ++kt)
           if (16 * kt < n) {
             uint32_t ah[4], al[4];
@@ -621,8 +636,11 @@ __global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaC
   for (int64_t c0 = first; c0 < n_end; c0 += LC) {
     const int n = (int)min((int64_t)LC, n_end - c0);
     auto publish = [&](float mk, float mv) {
-      mk = warp_max(mk);
-      mv = warp_max(mv);
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) {
+        mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, s));
+        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, s));
+      }
       if (lane == 0) {
         red[0][warp] = mk;
         red[1][warp] = mv;
@@ -666,7 +684,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaC
         for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.f;
-#pragma unroll
+#pragma unroll 1
       for (int kt = 0; kt < 4; ++kt)
         if (16 * kt < n) {
           uint32_t bh[8], bl[8];

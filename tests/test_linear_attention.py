@@ -409,3 +409,24 @@ def test_refusals_of_the_library(handler):
     for dk, dv in ((129, 8), (8, 200), (0, 8), (8, 0)):
         with pytest.raises(B200Error, match='values'):
             h.linear_attention_forward(z(2, 1, 1, dk), z(2, 1, 1, dk), z(2, 1, 1, dv), z(1), z(2, 1, 1, dv))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dv', [128, 127])
+def test_states_beyond_32_bit_offsets(handler, dv):
+    """8.7 GB of states, of which the last one is not zero: the address of a state does not fit 32 bits."""
+    h, (B, H, dk) = handler, (33300, 4, 128)
+    rng = np.random.RandomState(21)
+    q, k, v, s = rng.randn(dk), rng.randn(dk), rng.randn(dv), rng.randn(dk, dv)
+    up = {n: h.zeros(shape) for n, shape in (('q', (B, H, dk)), ('k', (B, H, dk)), ('v', (B, H, dv)), ('out', (B, H, dv)), ('state', (B, H, dk, dv)))}
+    assert up['state'].size > 2 ** 31
+    for n, x in (('q', q), ('k', k), ('v', v), ('state', s)):
+        h.set_from_numpy(up[n][B - 1, H - 1], x.astype(np.float32))
+    h.linear_attention_step(up['q'], up['k'], up['v'], h.create_from_numpy(np.full(H, 0.5, np.float32)), up['state'], up['out'])
+    q, k, v, s = (x.astype(np.float32).astype(np.float64) for x in (q, k, v, s))
+    want = 0.5 * s + np.outer(k, v)
+    # a state: two products and a sum, three half steps; an output: those, a product and a sum of 128 terms
+    assert (np.abs(h.get_numpy_copy(up['state'][B - 1, H - 1]) - want) <= 3 * U * (0.5 * np.abs(s) + np.abs(np.outer(k, v)))).all()
+    bound = 132 * U * (np.abs(q) @ (0.5 * np.abs(s) + np.abs(np.outer(k, v))))
+    assert (np.abs(h.get_numpy_copy(up['out'][B - 1, H - 1]) - q @ want) <= bound).all()
+    assert not h.get_numpy_copy(up['out'][:B - 1]).any() and not h.get_numpy_copy(up['state'][0]).any()
