@@ -430,3 +430,45 @@ def test_states_beyond_32_bit_offsets(handler, dv):
     bound = 132 * U * (np.abs(q) @ (0.5 * np.abs(s) + np.abs(np.outer(k, v))))
     assert (np.abs(h.get_numpy_copy(up['out'][B - 1, H - 1]) - q @ want) <= bound).all()
     assert not h.get_numpy_copy(up['out'][:B - 1]).any() and not h.get_numpy_copy(up['state'][0]).any()
+
+
+# more blocks than the GPU has SMs: four warps a block instead of eight
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape, ragged, decays', [((70, 40, 8, 4, 64, 64), True, None), ((129, 20, 8, 2, 48, 80), True, None), ((100, 20, 8, 8, 128, 128), False, None),
+                                                   ((65, 26, 6, 3, 33, 31), True, None), ((80, 40, 4, 4, 127, 126), True, None), ((150, 40, 4, 2, 96, 64), True, [1.0, 0.0, 0.5]),
+                                                   ((40, 100, 2, 2, 5, 128), True, [-0.75, 1.0]), ((9, 200, 1, 1, 17, 20), True, None), ((600, 38, 2, 1, 80, 48), True, None)])
+def test_many_sequences(handler, shape, ragged, decays):
+    d = _case(*shape, seed=sum(shape), ragged=ragged, decays=decays)
+    scale = shape[4] ** -0.5
+    got = _run(handler, d, scale)
+    out, state = ref.attention(d['q'], d['k'], d['v'], d['decay'], scale, d['state'], d['lengths'])
+    for name, want, bound in zip(('out', 'state_out'), (out, state), _bound(d, scale, False)):
+        _check(got[name], want, bound, name)
+    wants = ref.attention_backward(d['q'], d['k'], d['v'], d['decay'], d['dout'], scale, d['state'], d['dstate_out'], d['lengths'])
+    for name, want, bound in zip(('dq', 'dk', 'dv', 'dstate'), wants, _bound(d, scale, True)):
+        _check(got[name], want, bound, name)
+    more = _run(handler, d, scale, accumulate=True)       # onto ones
+    for name in ('dq', 'dk', 'dv'):
+        # rounding the sum with one, and the one or two sums in between
+        assert (np.abs(more[name] - (got[name].astype(np.float64) + 1)) <= 4 * U * (np.abs(got[name]) + 1)).all(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dk', [32, 96])
+@pytest.mark.parametrize('name', ['q', 'k', 'v'])
+@pytest.mark.parametrize('value', [np.nan, np.inf])
+def test_a_value_that_is_not_finite_among_many_sequences(handler, value, name, dk):
+    T, at = 140, 90
+    d = _case(T, 90, 2, 2, dk, 32, seed=17)
+    want = _run(handler, d, backward=False)
+    d[name][at, 50, 1, 5] = value
+    got = _run(handler, d, backward=False)['out']
+    same = np.ones(got.shape[1:3], bool)
+    same[50, 1] = False
+    assert np.array_equal(got[:, same], want['out'][:, same])
+    assert np.array_equal(got[:at - 15, 50, 1], want['out'][:at - 15, 50, 1])
+    assert not np.isfinite(got[at, 50, 1, 5])
+    if name == 'q':
+        assert np.array_equal(got[at + 1:, 50, 1], want['out'][at + 1:, 50, 1])
+    else:
+        assert not np.isfinite(got[at:, 50, 1, 5]).any()
