@@ -207,6 +207,125 @@ __global__ void __launch_bounds__(1024, R <= 8 ? 2 : 1) la_recurrent_any_kernel(
   }
 }
 
+// One token for many states of any dv and alignment.  The states of consecutive (sequence, head)s are one run of memory: a
+// block takes `per` of them into shared memory as they lie, 128 bits at a time counted from the boundary before the first,
+// works on them there column by column, and writes them back the same way.  k and q lie beside them, padded to four
+// rows, so that a thread reads four rows' factors at once.
+// Bound: HBM (512 x 16 states of 127 x 126: 380 us by 32-bit accesses from the columns in registers, 223 here, floor
+// 163; 4000 x 4 of 90 x 97: 642 and 238, floor 174; 2182 x 16 of 52 x 15: 97 and 67, floor 36).
+struct LaFlatState {
+  const float *q, *k, *v;
+  float* o;
+  float decay;
+  int live;
+};
+constexpr int LF_THREADS = 256, LF_MOST = 64;
+
+__host__ __device__ __forceinline__ int lf_rows(int dk) { return (dk + 3) & ~3; }
+
+__global__ void __launch_bounds__(LF_THREADS) la_flat_step_kernel(LaCommon c, LaRun p, int per, int cols_log2) {
+  extern __shared__ __align__(16) float lf_smem[];
+  __shared__ LaFlatState one[LF_MOST];
+  __shared__ float part[LF_THREADS];
+  const int dk = p.dk, dv = p.dv, N = dk * dv, dkp = lf_rows(dk), tid = threadIdx.x;
+  const int64_t BH = (int64_t)c.B * c.H, bh0 = (int64_t)blockIdx.x * per;
+  const int count = (int)min((int64_t)per, BH - bh0), total = count * N;
+  float* kq = lf_smem;                                       // k and q of each state
+  float* vs = kq + 2 * per * dkp;                            // v of each state
+  const float* s_in = p.s_in + bh0 * N;
+  float* s_out = p.s_out + bh0 * N;
+  const int off = (int)((reinterpret_cast<uintptr_t>(s_in) >> 2) & 3);
+  float* S = vs + ((per * dv + 3) & ~3) + off;               // element e of the run at S[e]
+  // ---- the states on their way
+  const int head = min(total, (4 - off) & 3), whole = (total - head) >> 2, tail = head + 4 * whole;
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(S);
+  for (int i = tid; i < whole; i += LF_THREADS)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * (head + 4 * i)), "l"(s_in + head + 4 * i) : "memory");
+  if (tid < head) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * tid), "l"(s_in + tid) : "memory");
+  if (tail + tid < total) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * (tail + tid)), "l"(s_in + tail + tid) : "memory");
+  // ---- the rest of them
+  if (tid < count) {
+    const int bh = (int)(bh0 + tid), b = bh / c.H, h = bh - b * c.H;
+    one[tid] = {p.q + la_offset(p.qs, b, h), p.k + la_offset(p.ks, b, h), p.v + la_offset(p.vs, b, h), p.o + la_offset(p.os, b, h), c.decay[h],
+                la_length(c, b) > 0};
+  }
+  __syncthreads();
+  for (int i = tid; i < count * dkp; i += LF_THREADS) {
+    const int g = i / dkp, row = i - g * dkp;
+    const bool in = row < dk && one[g].live;
+    kq[2 * g * dkp + row] = in ? one[g].k[row] * p.k_scale : 0.f;
+    kq[(2 * g + 1) * dkp + row] = in ? one[g].q[row] : 0.f;
+  }
+  for (int i = tid; i < count * dv; i += LF_THREADS) {
+    const int g = i / dv;
+    vs[i] = one[g].live ? one[g].v[i - g * dv] : 0.f;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  // ---- thread: a column of a state, a share of the rows
+  const int cols = 1 << cols_log2, groups = LF_THREADS >> cols_log2, rg = tid >> cols_log2;
+  const int rows = lf_rows((dk + groups - 1) / groups), first = rg * rows, last = min(dk, first + rows);
+  for (int c0 = 0; c0 < count * dv; c0 += cols) {            // one pass when there are groups
+    const int col = c0 + (tid & (cols - 1));
+    const int g = min(col / dv, count - 1), j = col - g * dv;
+    float acc = 0.f;
+    if (col < count * dv && one[g].live) {
+      const float l = one[g].decay, vj = vs[col];
+      const float4* kk = reinterpret_cast<const float4*>(kq + 2 * g * dkp);
+      const float4* qq = reinterpret_cast<const float4*>(kq + (2 * g + 1) * dkp);
+      float* s = S + g * N + j;
+      for (int i = first; i < last; i += 4) {
+        const float4 k4 = kk[i >> 2], q4 = qq[i >> 2];
+        const float kx[4] = {k4.x, k4.y, k4.z, k4.w}, qx[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (i + u < last) {
+            const float x = l * s[(i + u) * dv] + kx[u] * vj;
+            s[(i + u) * dv] = x;
+            acc += qx[u] * x;
+          }
+      }
+    }
+    if (groups > 1) {
+      part[tid] = acc;
+      __syncthreads();
+      if (rg == 0)
+        for (int u = 1; u < groups; ++u) acc += part[tid + (u << cols_log2)];
+    }
+    if (rg == 0 && col < count * dv) one[g].o[j] = one[g].live ? p.o_scale * acc : 0.f;
+  }
+  __syncthreads();
+  // ---- back
+  if (((reinterpret_cast<uintptr_t>(s_out) >> 2) & 3) == off) {
+    for (int i = tid; i < whole; i += LF_THREADS) *reinterpret_cast<float4*>(s_out + head + 4 * i) = *reinterpret_cast<const float4*>(S + head + 4 * i);
+    if (tid < head) s_out[tid] = S[tid];
+    if (tail + tid < total) s_out[tail + tid] = S[tail + tid];
+  } else {
+    for (int i = tid; i < total; i += LF_THREADS) s_out[i] = S[i];
+  }
+}
+
+// Floats of shared memory for `per` states.
+static int64_t lf_floats(int per, int dk, int dv) { return (int64_t)per * (2 * lf_rows(dk) + (int64_t)dk * dv) + (((int64_t)per * dv + 3) & ~3ll) + 4; }
+
+static int la_flat_step(const LaCommon& c, const LaRun& run) {
+  const int64_t BH = (int64_t)c.B * c.H;
+  // at most 40 KiB a block (or one state), at least eight blocks for each SM
+  int per = 1;
+  while (per < LF_MOST && lf_floats(per + 1, run.dk, run.dv) <= 10240 && ceil_div(BH, per + 1) >= 8ll * state().sm_count) ++per;
+  int log2 = 5;
+  while (log2 < 8 && (1 << log2) < per * run.dv) ++log2;
+  const int64_t smem = lf_floats(per, run.dk, run.dv) * 4;
+  static bool ready = false;
+  if (!ready) {
+    B200_CUDA(cudaFuncSetAttribute(la_flat_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lf_floats(1, LA_MAX_DIM, LA_MAX_DIM) * 4));
+    ready = true;
+  }
+  la_flat_step_kernel<<<(unsigned)ceil_div(BH, per), LF_THREADS, smem, state().stream>>>(c, run, per, log2);
+  B200_LAUNCH_CHECK();
+  return B200_OK;
+}
+
 // One launch for up to three runs over the same sequences.
 int la_recurrent(const LaCommon& c, const LaRun* runs, int count) {
   LaRuns all = {};
@@ -223,6 +342,7 @@ int la_recurrent(const LaCommon& c, const LaRun* runs, int count) {
   }
   const int64_t BH = (int64_t)c.B * c.H;
   const cudaStream_t st = state().stream;
+  if (!whole && c.T == 1 && count == 1 && runs[0].s_in && runs[0].s_out && BH >= 4ll * b200::state().sm_count) return la_flat_step(c, runs[0]);
   if (!whole) {
     int log2 = 3, threads = 128;
     while ((1 << log2) < dv) ++log2;

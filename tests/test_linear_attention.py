@@ -472,3 +472,34 @@ def test_a_value_that_is_not_finite_among_many_sequences(handler, value, name, d
         assert np.array_equal(got[at + 1:, 50, 1], want['out'][at + 1:, 50, 1])
     else:
         assert not np.isfinite(got[at:, 50, 1, 5]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('lengths', [False, True])
+@pytest.mark.parametrize('shift, shift_out', [(0, None), (1, None), (0, 2), (3, 3)])
+@pytest.mark.parametrize('dk, dv', [(52, 15), (127, 126), (16, 17), (5, 3), (90, 97), (64, 64), (1, 1), (1, 3), (128, 1), (3, 128), (30, 50)])
+def test_a_token_for_many_streams(handler, dk, dv, shift, shift_out, lengths):
+    """States that start `shift` floats behind a 16-byte boundary; in place, or into another array that starts elsewhere."""
+    h, (B, H, K) = handler, (307, 4, 2)
+    d = _case(1, B, H, K, dk, dv, seed=dk + dv)
+    if lengths:
+        d['lengths'] = (np.arange(B) % 3 > 0).astype(np.float32)
+    p = {n: None if a is None else h.create_from_numpy(a) for n, a in _poison(d).items()}
+    size = B * H * dk * dv
+
+    def at(offset):
+        flat = h.create_from_numpy(np.full(size + 8, 7.0, np.float32))
+        return flat, flat[offset:offset + size].reshape((B, H, dk, dv))
+    flat, state = at(shift)
+    flat_out, state_out = (flat, state) if shift_out is None else at(shift_out)
+    h.set_from_numpy(state, d['state'])
+    out = h.ones((1, B, H, dv))
+    h.linear_attention_forward(p['q'], p['k'], p['v'], p['decay'], out, scale=0.5, state=state, state_out=state_out, lengths=p['lengths'])
+    want, want_state = ref.attention(d['q'], d['k'], d['v'], d['decay'], 0.5, d['state'], d['lengths'])
+    for got, w, bound, what in zip((out, state_out), (want, want_state), _bound(d, 0.5, False), ('out', 'state')):
+        _check(h.get_numpy_copy(got), w, bound, what)
+    if lengths:
+        assert np.array_equal(h.get_numpy_copy(state_out)[::3], d['state'][::3]) and not h.get_numpy_copy(out)[0, ::3].any()
+    offset = shift if shift_out is None else shift_out
+    around = h.get_numpy_copy(flat_out)
+    assert (around[:offset] == 7).all() and (around[offset + size:] == 7).all()
