@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(1024, R <= 8 ? 2 : 1) la_recurrent_any_kernel(
 // works on them there column by column, and writes them back the same way.  k and q lie beside them, padded to four
 // rows, so that a thread reads four rows' factors at once.
 // Bound: HBM (512 x 16 states of 127 x 126: 380 us by 32-bit accesses from the columns in registers, 223 here, floor
-// 163; 4000 x 4 of 90 x 97: 642 and 238, floor 174; 2182 x 16 of 52 x 15: 97 and 67, floor 36).
+// 163; 4000 x 4 of 90 x 97: 642 and 238, floor 174; 2182 x 16 of 52 x 15: 97 and 64, floor 36).
 struct LaFlatState {
   const float *q, *k, *v;
   float* o;
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(LF_THREADS) la_flat_step_kernel(LaCommon c, La
   extern __shared__ __align__(16) float lf_smem[];
   __shared__ LaFlatState one[LF_MOST];
   __shared__ float part[LF_THREADS];
-  const int dk = p.dk, dv = p.dv, N = dk * dv, dkp = lf_rows(dk), tid = threadIdx.x;
+  const int dk = p.dk, dv = p.dv, N = dk * dv, dkp = lf_rows(dk), tid = threadIdx.x, threads = blockDim.x;
   const int64_t BH = (int64_t)c.B * c.H, bh0 = (int64_t)blockIdx.x * per;
   const int count = (int)min((int64_t)per, BH - bh0), total = count * N;
   float* kq = lf_smem;                                       // k and q of each state
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(LF_THREADS) la_flat_step_kernel(LaCommon c, La
   // ---- the states on their way
   const int head = min(total, (4 - off) & 3), whole = (total - head) >> 2, tail = head + 4 * whole;
   const uint32_t to = (uint32_t)__cvta_generic_to_shared(S);
-  for (int i = tid; i < whole; i += LF_THREADS)
+  for (int i = tid; i < whole; i += threads)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 4 * (head + 4 * i)), "l"(s_in + head + 4 * i) : "memory");
   if (tid < head) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * tid), "l"(s_in + tid) : "memory");
   if (tail + tid < total) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + 4 * (tail + tid)), "l"(s_in + tail + tid) : "memory");
@@ -250,20 +250,20 @@ __global__ void __launch_bounds__(LF_THREADS) la_flat_step_kernel(LaCommon c, La
                 la_length(c, b) > 0};
   }
   __syncthreads();
-  for (int i = tid; i < count * dkp; i += LF_THREADS) {
+  for (int i = tid; i < count * dkp; i += threads) {
     const int g = i / dkp, row = i - g * dkp;
     const bool in = row < dk && one[g].live;
     kq[2 * g * dkp + row] = in ? one[g].k[row] * p.k_scale : 0.f;
     kq[(2 * g + 1) * dkp + row] = in ? one[g].q[row] : 0.f;
   }
-  for (int i = tid; i < count * dv; i += LF_THREADS) {
+  for (int i = tid; i < count * dv; i += threads) {
     const int g = i / dv;
     vs[i] = one[g].live ? one[g].v[i - g * dv] : 0.f;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   // ---- thread: a column of a state, a share of the rows
-  const int cols = 1 << cols_log2, groups = LF_THREADS >> cols_log2, rg = tid >> cols_log2;
+  const int cols = 1 << cols_log2, groups = threads >> cols_log2, rg = tid >> cols_log2;
   const int rows = lf_rows((dk + groups - 1) / groups), first = rg * rows, last = min(dk, first + rows);
   for (int c0 = 0; c0 < count * dv; c0 += cols) {            // one pass when there are groups
     const int col = c0 + (tid & (cols - 1));
@@ -297,11 +297,11 @@ __global__ void __launch_bounds__(LF_THREADS) la_flat_step_kernel(LaCommon c, La
   __syncthreads();
   // ---- back
   if (((reinterpret_cast<uintptr_t>(s_out) >> 2) & 3) == off) {
-    for (int i = tid; i < whole; i += LF_THREADS) *reinterpret_cast<float4*>(s_out + head + 4 * i) = *reinterpret_cast<const float4*>(S + head + 4 * i);
+    for (int i = tid; i < whole; i += threads) *reinterpret_cast<float4*>(s_out + head + 4 * i) = *reinterpret_cast<const float4*>(S + head + 4 * i);
     if (tid < head) s_out[tid] = S[tid];
     if (tail + tid < total) s_out[tail + tid] = S[tail + tid];
   } else {
-    for (int i = tid; i < total; i += LF_THREADS) s_out[i] = S[i];
+    for (int i = tid; i < total; i += threads) s_out[i] = S[i];
   }
 }
 
@@ -310,18 +310,20 @@ static int64_t lf_floats(int per, int dk, int dv) { return (int64_t)per * (2 * l
 
 static int la_flat_step(const LaCommon& c, const LaRun& run) {
   const int64_t BH = (int64_t)c.B * c.H;
-  // at most 40 KiB a block (or one state), at least eight blocks for each SM
+  // 128 threads with at most 20 KiB (2000 x 8 states of 64 x 63: 104 us, 256 with 40 KiB 110) or, for states of more than 16 KiB, 256
+  // (512 x 16 of 127 x 126: 223 us, 128 threads 246); one state at least, eight blocks for each SM at least
+  const int threads = run.dk * run.dv <= 4096 ? 128 : LF_THREADS;
   int per = 1;
-  while (per < LF_MOST && lf_floats(per + 1, run.dk, run.dv) <= 10240 && ceil_div(BH, per + 1) >= 8ll * state().sm_count) ++per;
+  while (per < LF_MOST && lf_floats(per + 1, run.dk, run.dv) <= 40 * threads && ceil_div(BH, per + 1) >= 8ll * state().sm_count) ++per;
   int log2 = 5;
-  while (log2 < 8 && (1 << log2) < per * run.dv) ++log2;
+  while ((1 << log2) < threads && (1 << log2) < per * run.dv) ++log2;
   const int64_t smem = lf_floats(per, run.dk, run.dv) * 4;
   static bool ready = false;
   if (!ready) {
     B200_CUDA(cudaFuncSetAttribute(la_flat_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lf_floats(1, LA_MAX_DIM, LA_MAX_DIM) * 4));
     ready = true;
   }
-  la_flat_step_kernel<<<(unsigned)ceil_div(BH, per), LF_THREADS, smem, state().stream>>>(c, run, per, log2);
+  la_flat_step_kernel<<<(unsigned)ceil_div(BH, per), threads, smem, state().stream>>>(c, run, per, log2);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
