@@ -25,8 +25,8 @@
 //
 // Bound: neither memory nor the tensor pipe (33 and 25 % of the clocks at d = 128 and 64) but the latency between
 // dependent instructions: registers and shared memory let two or three blocks onto an SM, two or three warps a
-// scheduler, which issue in 36 to 43 % of the clocks.  Measured: 8192 x 2 x 16 heads of 128 608 us (state pass 172, handing
-// through 20, outputs 420), HBM time 83; 100 x 128 x 16 heads of 64 with gradients 469 us, HBM time 114; 1999 x 6 x 12 heads
+// scheduler, which issue in 36 to 43 % of the clocks.  Measured: 8192 x 2 x 16 heads of 128 598 us (state pass 160, handing
+// through 20, outputs 420), HBM time 83; 100 x 128 x 16 heads of 64 with gradients 454 us, HBM time 114; 1999 x 6 x 12 heads
 // of 48 and 80 over 4, ragged, with gradients 567 us, HBM time 39.
 #include <cuda_fp16.h>
 
@@ -806,7 +806,7 @@ static int lc_launch(const LaCommon& c, const LaChunkRuns& all, int count, const
   const int64_t blocks = (int64_t)c.B * c.H * p.segments * p.slabs;
   B200_REQUIRE(blocks < (1ll << 31), "linear attention: extent too large");
   // no more blocks than SMs: eight warps a block (24 tokens of 8 heads of 64: 10.2 -> 8.2 us; more blocks share the SMs better
-  // with four, 100 x 128 x 16 heads: 469 us against 518)
+  // with four, 100 x 128 x 16 heads: 469 us against 518 then)
   const bool few = blocks * count <= b200::state().sm_count;
   auto main_kernel = few ? (vec ? la_chunk_kernel<DK, 256, true> : la_chunk_kernel<DK, 256, false>)
                          : (vec ? la_chunk_kernel<DK, 128, true> : la_chunk_kernel<DK, 128, false>);
