@@ -164,14 +164,34 @@ __device__ __forceinline__ void gn_act_all(int act, float (&v)[E]) {
     for (int e = 0; e < E; ++e) v[e] = gn_act(3, v[e]);
   }
 }
-// Column sums in shared memory: float4 number i of thread t at i * threads + t.
+// Column sums in shared memory: vector (of 4 floats, or of E fewer) number i of thread t at i * threads + t.
 template <int E>
-__device__ __forceinline__ void gn_sum_into(float4* s, const float (&v)[E]) {
+struct GnVector {
+  using type = float4;
+};
+template <>
+struct GnVector<2> {
+  using type = float2;
+};
+template <>
+struct GnVector<1> {
+  using type = float;
+};
+template <int E>
+__device__ __forceinline__ void gn_sum_into(typename GnVector<E>::type* s, const float (&v)[E]) {
+  if constexpr (E == 1) {
+    *s += v[0];
+  } else if constexpr (E == 2) {
+    float2 q = *s;
+    q.x += v[0]; q.y += v[1];
+    *s = q;
+  } else {
 #pragma unroll
-  for (int i = 0; i < E / 4; ++i) {
-    float4 q = s[i * blockDim.x];
-    q.x += v[4 * i]; q.y += v[4 * i + 1]; q.z += v[4 * i + 2]; q.w += v[4 * i + 3];
-    s[i * blockDim.x] = q;
+    for (int i = 0; i < E / 4; ++i) {
+      float4 q = s[i * blockDim.x];
+      q.x += v[4 * i]; q.y += v[4 * i + 1]; q.z += v[4 * i + 2]; q.w += v[4 * i + 3];
+      s[i * blockDim.x] = q;
+    }
   }
 }
 
@@ -199,7 +219,7 @@ __device__ __forceinline__ float gn_row_sum(float v, int G, float* smem) {
 template <int E, int MODE, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) gated_norm_forward_kernel(GatedNorm p, int G) {
   // the weights in registers from the start: where their loads are single, or few rows leave their latency bare
-  constexpr bool KEEP = MODE == GN_SHIFT || E == 4;
+  constexpr bool KEEP = MODE == GN_SHIFT || E <= 4;
   __shared__ float red[32];
   const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
   const float inv_width = 1.f / (float)p.width;
@@ -281,15 +301,18 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 3 : 4) 
 // Shared memory: three vectors of column sums for each group of G threads (gn_sum_into).
 template <int E, int MODE, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 2 : 3) gated_norm_backward_kernel(GatedNormGrad p, int G) {
-  constexpr bool KEEP = MODE == GN_SHIFT || E == 4;
-  extern __shared__ float4 sums[];
+  constexpr bool KEEP = MODE == GN_SHIFT || E <= 4;
+  using Sum = typename GnVector<E>::type;
+  constexpr int W = E < 4 ? E : 4, N = E / W;      // floats of a vector, vectors of a thread
+  extern __shared__ float4 sum_space[];
+  Sum* sums = reinterpret_cast<Sum*>(sum_space);
   __shared__ float red[32];
   const int t = threadIdx.x & (G - 1), per_block = blockDim.x / G;
-  float4* s_post = sums + threadIdx.x;
-  float4* s_scale = s_post + E / 4 * blockDim.x;
-  float4* s_pre = s_scale + E / 4 * blockDim.x;
+  Sum* s_post = sums + threadIdx.x;
+  Sum* s_scale = s_post + N * blockDim.x;
+  Sum* s_pre = s_scale + N * blockDim.x;
 #pragma unroll
-  for (int i = 0; i < E / 4; ++i) s_post[i * blockDim.x] = s_scale[i * blockDim.x] = s_pre[i * blockDim.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < N; ++i) s_post[i * blockDim.x] = s_scale[i * blockDim.x] = s_pre[i * blockDim.x] = Sum();
   const float inv_width = 1.f / (float)p.width;
   const int64_t row_first = (int64_t)blockIdx.x * per_block + threadIdx.x / G;
   const int off = MODE == GN_SHIFT ? (int)((reinterpret_cast<uintptr_t>(p.dx + row_first * p.ld_dx) >> 2) & 3) : 0;
@@ -421,9 +444,9 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 2 : 3) 
     for (int e = 0; e < E; ++e) {
       const int c = gn_column<MODE>(e, G, t, off);
       if (c < 0 || c >= p.width) continue;
-      out[c] = reinterpret_cast<const float*>(s_post + e / 4 * blockDim.x)[e % 4];
-      out[p.width + c] = reinterpret_cast<const float*>(s_scale + e / 4 * blockDim.x)[e % 4];
-      out[2 * p.width + c] = reinterpret_cast<const float*>(s_pre + e / 4 * blockDim.x)[e % 4];
+      out[c] = reinterpret_cast<const float*>(s_post + e / W * blockDim.x)[e % W];
+      out[p.width + c] = reinterpret_cast<const float*>(s_scale + e / W * blockDim.x)[e % W];
+      out[2 * p.width + c] = reinterpret_cast<const float*>(s_pre + e / W * blockDim.x)[e % W];
     }
     return;
   }
@@ -436,9 +459,9 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 2 : 3) 
       if (c >= p.width) continue;
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        const float* col = reinterpret_cast<const float*>(sums + (int64_t)(k * (E / 4) + e / 4) * blockDim.x + t) + e % 4;
+        const float* col = reinterpret_cast<const float*>(sums + (int64_t)(k * N + e / W) * blockDim.x + t) + e % W;
         float s = 0.f;
-        for (int q = 0; q < per_block; ++q) s += col[4 * q * G];
+        for (int q = 0; q < per_block; ++q) s += col[W * q * G];
         out[(int64_t)k * p.width + c] = s;
       }
     }
@@ -479,7 +502,7 @@ static GnShape gn_geometry(int64_t rows, int width, int mode, bool backward) {
   GnShape s;
   s.mode = mode;
   const int span = width + (mode == GN_SHIFT ? 3 : 0);
-  s.E = span <= 128 ? 4 : (span <= 256 || (mode != GN_VEC && span <= 8192)) ? 8 : 16;
+  s.E = mode == GN_SINGLE && span <= 64 ? (span <= 32 ? 1 : 2) : span <= 128 ? 4 : (span <= 256 || (mode != GN_VEC && span <= 8192)) ? 8 : 16;
   // Few rows: a call is the latency of one row, which is shorter with 4 floats a thread, as long as all rows are resident
   // at once (128 x 1000: forward 4.6 -> 3.3 us, backward 14.9 -> 7.0; 592 x 1000: 4.8 -> 4.5, 15.5 -> 12.7; forward of 400 x 2000
   // 5.6 -> 8.2, of 64 x 4096 4.6 -> 5.5: fewer, wider blocks fit).
@@ -523,7 +546,9 @@ static GnShape gn_shape(int64_t rows, int width, std::initializer_list<std::pair
     pitch = a.second;
   }
   for (const void* v : vectors) vec = vec && aligned16(v);
-  return gn_geometry(rows, width, vec ? GN_VEC : alike && gn_shiftable(width) ? GN_SHIFT : GN_SINGLE, backward);
+  // up to 64 columns a float or two a lane, whatever the alignment (1000000 x 32: forward 358 -> 297 us, backward 566 -> 438;
+  // x 30: 445 -> 294, 690 -> 435; 254292 x 42: 125 -> 96, 194 -> 149, against four)
+  return gn_geometry(rows, width, width <= 64 ? GN_SINGLE : vec ? GN_VEC : alike && gn_shiftable(width) ? GN_SHIFT : GN_SINGLE, backward);
 }
 
 }  // namespace b200
@@ -539,7 +564,8 @@ using namespace b200;
                            : s.E == 4 ? KERNEL<4, GN_SHIFT, 256> : KERNEL<8, GN_SHIFT, 256>)                             \
    : s.threads == 1024 ? (s.E == 8 ? KERNEL<8, GN_SINGLE, 1024> : KERNEL<16, GN_SINGLE, 1024>)                           \
    : s.threads == 512 ? KERNEL<8, GN_SINGLE, 512>                                                                        \
-                      : (s.E == 4 ? KERNEL<4, GN_SINGLE, 256> : KERNEL<8, GN_SINGLE, 256>))
+                      : s.E == 1 ? KERNEL<1, GN_SINGLE, 256> : s.E == 2 ? KERNEL<2, GN_SINGLE, 256>                           \
+                      : s.E == 4 ? KERNEL<4, GN_SINGLE, 256> : KERNEL<8, GN_SINGLE, 256>)
 
 B200_API int b200_gated_norm_forward(const b200_gated_norm_args* args) {
   if (int rc = require_ready()) return rc;

@@ -121,7 +121,8 @@ def test_forward_and_gradients(handler, shape):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('shape', [(700, 1000), (593, 1000), (600, 1021), (1190, 510), (1300, 333), (610, 1537), (300, 2044), (300, 2045), (3, 2046), (3, 4093), (3, 4094), (3, 4799),
-                                   (3, 4801), (160, 5001), (2, 8189), (2, 8190), (3, 4096), (600, 4096), (2500, 129)])
+                                   (3, 4801), (160, 5001), (2, 8189), (2, 8190), (3, 4096), (600, 4096), (2500, 129), (3000, 17), (6000, 64), (2500, 50), (700, 32),
+                                   (4000, 1)])
 def test_around_the_limits_of_the_forms(handler, shape):
     """Few rows and many, widths that fill 256, 512 or 1024 threads."""
     _check(handler, _case(*shape, seed=shape[0]), 'sigmoid')
