@@ -556,15 +556,17 @@ static GnShape gn_shape(int64_t rows, int width, std::initializer_list<std::pair
 using namespace b200;
 
 // Rows of up to 4096 values (2045 in the shifted form): blocks of 256 threads; wider ones: one row for a block of 512 or 1024.
-#define GN_KERNELS(KERNEL)                                                                                               \
-  (s.mode == GN_VEC ? (s.threads == 1024 ? (s.E == 4 ? KERNEL<4, GN_VEC, 1024> : KERNEL<16, GN_VEC, 1024>)               \
-                       : s.threads == 512 ? (s.E == 4 ? KERNEL<4, GN_VEC, 512> : KERNEL<16, GN_VEC, 512>)                 \
+// Few rows of 2049 to 4096 values take `FEW` (4 floats a thread in the backward pass only).
+#define GN_KERNELS(KERNEL, FEW)                                                                                          \
+  (s.mode == GN_VEC ? (s.threads == 1024 ? (s.E == 4 ? FEW : KERNEL<16, GN_VEC, 1024>)                                   \
+                       : s.threads == 512 ? (s.E == 4 ? KERNEL<4, GN_VEC, 512> : KERNEL<16, GN_VEC, 512>)                \
                        : s.E == 4 ? KERNEL<4, GN_VEC, 256> : s.E == 8 ? KERNEL<8, GN_VEC, 256> : KERNEL<16, GN_VEC, 256>) \
-   : s.mode == GN_SHIFT ? (s.threads == 1024 ? KERNEL<8, GN_SHIFT, 1024> : s.threads == 512 ? (s.E == 4 ? KERNEL<4, GN_SHIFT, 512> : KERNEL<8, GN_SHIFT, 512>) \
+   : s.mode == GN_SHIFT ? (s.threads == 1024 ? KERNEL<8, GN_SHIFT, 1024>                                                 \
+                           : s.threads == 512 ? (s.E == 4 ? KERNEL<4, GN_SHIFT, 512> : KERNEL<8, GN_SHIFT, 512>)         \
                            : s.E == 4 ? KERNEL<4, GN_SHIFT, 256> : KERNEL<8, GN_SHIFT, 256>)                             \
    : s.threads == 1024 ? (s.E == 8 ? KERNEL<8, GN_SINGLE, 1024> : KERNEL<16, GN_SINGLE, 1024>)                           \
    : s.threads == 512 ? KERNEL<8, GN_SINGLE, 512>                                                                        \
-                      : s.E == 1 ? KERNEL<1, GN_SINGLE, 256> : s.E == 2 ? KERNEL<2, GN_SINGLE, 256>                           \
+                      : s.E == 1 ? KERNEL<1, GN_SINGLE, 256> : s.E == 2 ? KERNEL<2, GN_SINGLE, 256>                      \
                       : s.E == 4 ? KERNEL<4, GN_SINGLE, 256> : KERNEL<8, GN_SINGLE, 256>)
 
 B200_API int b200_gated_norm_forward(const b200_gated_norm_args* args) {
@@ -585,7 +587,7 @@ B200_API int b200_gated_norm_forward(const b200_gated_norm_args* args) {
                  (int)width, act, eps};
   const GnShape s = gn_shape(rows, (int)width, {{x, ld_x}, {y, ld_y}, {gate, ld_gate}, {y ? x_out : nullptr, ld_x_out}, {h_out, ld_h_out}},
                              {w_post, scale, w_pre}, false);
-  GN_KERNELS(gated_norm_forward_kernel)<<<s.blocks, s.threads, 0, state().stream>>>(p, s.G);
+  (GN_KERNELS(gated_norm_forward_kernel, (gated_norm_forward_kernel<16, GN_VEC, 1024>)))<<<s.blocks, s.threads, 0, state().stream>>>(p, s.G);
   B200_LAUNCH_CHECK();
   return B200_OK;
 }
@@ -631,7 +633,7 @@ B200_API int b200_gated_norm_backward(const float* x_out, const float* y, const 
                               {y ? dy : nullptr, ld_dy}, {gate ? dgate : nullptr, ld_dgate}},
                              {w_post, scale, w_pre}, true);
   const size_t smem = (size_t)3 * s.E * s.threads * sizeof(float);
-  auto kernel = GN_KERNELS(gated_norm_backward_kernel);
+  auto kernel = GN_KERNELS(gated_norm_backward_kernel, (gated_norm_backward_kernel<4, GN_VEC, 1024>));
   // 48 KiB and more of dynamic shared memory has to be asked for (the static part counts too)
   if (smem >= 48 * 1024) B200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<s.blocks, s.threads, smem, state().stream>>>(p, s.G);

@@ -4,7 +4,10 @@ Tolerance.  With U = 2^-24: a mean of D squares rounds each square once and adds
 steps, so 1 / rms is off by at most (E + 12) U of itself with E = 16 values for each thread; an output is a sum of
 products of at most six factors, each of which is rounded once (activations: at most 4 U and, through the argument of
 exp and the subtraction in 1 - a^2, 4 U of one), with at most four sums, and the two means enter once each.  So
-|error| <= 80 U (the same sum with absolute values).  A column sum over N rows adds to that at most N / blocks + blocks
+|error| <= 80 U (the same sum with absolute values).  r_pre is a function of the x_out that was formed: where x and the
+gated norm nearly cancel, x_out is off by far more than its own rounding, by e = 80 U (|x| + |x_out - x|) as any output
+is, and r(x_out) = (mean(x_out^2) + eps)^(-1/2) has the derivative -r^3 mean(x_out dx_out): r_pre is off by at most r^3
+mean((|x_out| + e) e) more (e^2 bounds the second order), and h_out by |x_out w_pre| times that.  A column sum over N rows adds to that at most N / blocks + blocks
 roundings: (80 + N) U of the sum of absolute values.
 """
 import numpy as np
@@ -81,11 +84,18 @@ def _check(h, d, act, post=True, pre=True, eps=1e-6):
     if post:
         size['x_out'] = size['x_out'] + np.abs(want['x_out'] - d['x'])
     if pre:
-        size['h_out'] = size['x_out'] * want['r_pre'][:, None] * (1 if d['w_pre'] is None else np.abs(d['w_pre']))
+        w, e = 1 if d['w_pre'] is None else np.abs(d['w_pre']), 80 * U * size['x_out']
+        size['h_out'] = size['x_out'] * want['r_pre'][:, None] * w
+    bound = {k: 80 * U * v for k, v in size.items()}
+    if pre and post:
+        x = np.abs(want['x_out'])
+        off = want['r_pre'] ** 3 * ((x + e) * e).mean(1)
+        bound['r_pre'] = bound['r_pre'] + off
+        bound['h_out'] = bound['h_out'] + x * w * off[:, None]
     for k in want:
         if k == 'x_out' and not post:
             continue
-        assert (np.abs(got[k] - want[k]) <= 80 * U * size[k] + 1e-37).all(), k
+        assert (np.abs(got[k] - want[k]) <= bound[k] + 1e-37).all(), k
     g = {k: h.get_numpy_copy(v).astype(np.float64) for k, v in _backward(h, up, o, act, post, pre).items()}
     # the backward formula at the forward pass's own float32 results
     f = {k: got[k] for k in ('x_out', 'r_post', 'r_pre')}
