@@ -11,7 +11,7 @@
 //
 // Bound: the products (ns_gemm.cu).  4096 x 4096 takes 3.9 ms, of which they are 3.75 at 366 TFLOP/s of fp32 accuracy
 // (1100 of half precision, at the clocks that the power limit leaves); four of 1000 x 1000 0.40 ms, half of it the first
-// loads and the epilogues of fifteen products that each fill the GPU once; 205 x 256 91 us in one launch.
+// loads and the epilogues of fifteen products that each fill the GPU once; 205 x 256 92 us in one launch.
 #include <algorithm>
 
 #include "common.cuh"

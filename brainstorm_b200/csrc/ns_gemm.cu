@@ -567,7 +567,7 @@ int ns_gemm(const NsMatrix& a, bool a_t, const NsMatrix& b, bool b_t, NsMatrix* 
 // 96.3 in a recorded graph), of which the tensor pipe has work for one.  Here a cluster of up to eight CTAs computes all
 // of them for one matrix of the stack: the operands stay in L2, barriers and tensor memory are set up once, and between two
 // products stands a barrier of the cluster (with a fence between the stores of the one and the TMA loads of the next)
-// instead of a launch: 90.6 us, 88.1 recorded; 64 x 64: 65.8 -> 57.5, eight of 128 x 256: 95.4 -> 81.6.  Of a product's
+// instead of a launch: 92 us, 89 recorded; 64 x 64: 65.8 -> 57.5, eight of 128 x 256: 95.4 -> 81.6.  Of a product's
 // 9000 clocks then 1500 are the way to the first MMA, 4000 the four K-blocks (loads and MMAs share the 128 bytes a clock
 // of shared memory), 2000 the epilogue, 1500 fence and barrier.
 // With two tiles a CTA it lost (256 x 500: 122.6 recorded against 116.0), as with more clusters than fit the GPU together
@@ -659,7 +659,6 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant_
     mine[w] = any ? ti << 16 | tj : -1;
   }
   pdl_wait();
-  asm volatile("fence.proxy.async;" ::: "memory");      // X was written by ordinary stores
   for (int x = 0, step = 0; step < c.steps; ++step, x ^= 1) {
 #pragma unroll
     for (int w = 0; w < 3; ++w) {
@@ -675,6 +674,7 @@ ns_chain_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant_
         const int m0 = (t >> 16) * NS_BM, n0 = (t & 0xffff) * BN;
         if (warp == 0) {
           if (elect_one()) {
+            asm volatile("fence.proxy.async;" ::: "memory");      // the operands were written by ordinary stores
             for (int kb = 0; kb < num_kb; ++kb) {
               ok = mbar_wait(empty_bar(s), phase ^ 1, abort_flag);
               if (!ok) break;
