@@ -30,7 +30,7 @@ __device__ __forceinline__ int64_t la_offset(const LaStrides& x, int b, int h) {
 // token's registers are not needed).
 template <int R, bool VEC, bool ONE>
 __global__ void __launch_bounds__(LR_THREADS, R == 8 ? (ONE ? 6 : 5) : 8) la_recurrent_kernel(LaCommon c, LaRuns runs, int max_slabs, int wps) {
-  __shared__ float part[2][4][LR_COLS];
+  __shared__ __align__(16) float part[2][4][LR_COLS];      // written as float4
   const LaRun& p = runs.run[blockIdx.y];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned group = (unsigned)warp / wps, id = blockIdx.x * (4u / wps) + group;
