@@ -583,6 +583,8 @@ B200_API int b200_gated_norm_forward(const b200_gated_norm_args* args) {
   B200_REQUIRE(y || !gate, "gated norm: a gate needs a block output");
   B200_REQUIRE(ld_x >= width && (!y || (ld_y >= width && ld_x_out >= width)) && (!gate || ld_gate >= width) && (!h_out || ld_h_out >= width),
                "gated norm: leading dimension too small");
+  B200_REQUIRE(rows == 1 || ((x_out != x || !y || ld_x_out == ld_x) && (h_out != y || !y || ld_h_out == ld_y)),
+               "gated norm: in place, both arrays have the same row pitch");
   GatedNorm p = {x, y, gate, w_post, scale, w_pre, x_out, h_out, r_post, r_pre, rows, ld_x, ld_y, ld_gate, ld_x_out, ld_h_out,
                  (int)width, act, eps};
   const GnShape s = gn_shape(rows, (int)width, {{x, ld_x}, {y, ld_y}, {gate, ld_gate}, {y ? x_out : nullptr, ld_x_out}, {h_out, ld_h_out}},
@@ -625,6 +627,7 @@ B200_API int b200_gated_norm_backward(const float* x_out, const float* y, const 
   B200_REQUIRE(ld_dx >= width && (!dh || (ld_dh >= width && ld_x_out >= width)) && (!dx_out || ld_dx_out >= width) &&
                    (!y || (ld_y >= width && ld_dy >= width)) && (!gate || (ld_gate >= width && ld_dgate >= width)),
                "gated norm: leading dimension too small");
+  B200_REQUIRE(rows == 1 || dx != dx_out || ld_dx == ld_dx_out, "gated norm: in place, both arrays have the same row pitch");
   B200_REQUIRE(!sums || (scratch && scratch_floats >= b200_gated_norm_scratch_floats(rows, width)), "gated norm: scratch too small");
   GatedNormGrad p = {x_out, y, gate, w_post, scale, w_pre, r_post, r_pre, dx_out, dh, dx, dy, dgate, sums ? scratch : nullptr, rows,
                      ld_x_out, ld_y, ld_gate, ld_dx_out, ld_dh, ld_dx, ld_dy, ld_dgate, (int)width, act, accumulate ? 1 : 0};

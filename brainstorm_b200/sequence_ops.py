@@ -95,17 +95,24 @@ def _meet(arrays):
     return any(map(gt, ends, starts[1:]))
 
 
+def _same(a, b):
+    """Whether two views have every element in the same place."""
+    return a.ptr == b.ptr and a.shape == b.shape and (a._contig and b._contig or
+                                                      all(s == t for n, s, t in zip(a.shape, a.strides, b.strides) if n > 1))
+
+
 def _apart(outputs, inputs, allowed=()):
     """Refuse an output that starts where another operand starts, and contiguous ones that overlap at all
-    (two row-pitched views may interleave in one buffer, as the columns of a hub do).  Called when operands
-    meet (``_meet``)."""
+    (two row-pitched views may interleave in one buffer, as the columns of a hub do).  An output that may be
+    an input has to be the same view: with another row pitch it would write rows that are still to be read.
+    Called when operands meet (``_meet``)."""
     seen = [(n, a) for n, a in inputs if a is not None and a.size]
     for name, a in outputs:
         if a is None or not a.size:
             continue
         lo, hi = _span(a)
         for other, b in seen:
-            if (name, other) in allowed and a.ptr == b.ptr:
+            if (name, other) in allowed and _same(a, b):
                 continue
             if a.ptr == b.ptr or (a._contig or b._contig) and lo < _span(b)[1] and _span(b)[0] < hi:
                 raise ValueError('%s overlaps %s' % (name, other))
@@ -222,7 +229,8 @@ class SequenceOps(object):
             epsilon: added to the mean squares.
             activation: 'sigmoid', 'tanh', 'rel', 'el' or 'linear'.
 
-        width: up to 16384.  ``x_out`` may be ``x`` and ``h_out`` may be ``y``."""
+        width: up to 16384.  ``x_out`` may be ``x`` and ``h_out`` may be ``y``, the same view; no other output may overlap
+        another operand."""
         act = _activation(activation)
         if len(x.shape) != 2:
             raise ValueError('expected 2-D arrays, got shape %r' % (x.shape,))

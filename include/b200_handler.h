@@ -407,10 +407,10 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      (y * r_post * w_post); without y x_out is x.  With h_out: r_pre = (mean(x_out^2) +
  *      eps)^-1/2, h_out = x_out * r_pre * w_pre.  w_post, scale, w_pre are vectors of `width`
  *      values or NULL (ones); gate NULL: no gate; act as in b200_bias_act.  Row pitches ld_*;
- *      width up to 16384.  x_out may be x, h_out may be y.  Backward takes the gradients
+ *      width up to 16384.  x_out may be x, h_out may be y, with the same pitch.  Backward takes the gradients
  *      dx_out (NULL: zero) and dh (NULL: no h_out was taken) and gives dx, dy, dgate and the
  *      vectors dw_post, dscale, dw_pre (each may be NULL); accumulate: all are ADDED to.  dx
- *      may be dx_out.  scratch of b200_gated_norm_scratch_floats(rows, width) floats for the
+ *      may be dx_out, with the same pitch.  scratch of b200_gated_norm_scratch_floats(rows, width) floats for the
  *      vectors' partial sums.
  *
  *      The two forward calls, which also serve single tokens, take their arguments in one struct: a
