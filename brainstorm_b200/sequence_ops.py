@@ -11,6 +11,7 @@ into pointers and extents; the kernels are in ``csrc/linear_attention*.cu``, ``g
 from __future__ import annotations
 
 import ctypes
+import functools
 import struct
 from operator import gt
 
@@ -101,22 +102,68 @@ def _same(a, b):
                                                       all(s == t for n, s, t in zip(a.shape, a.strides, b.strides) if n > 1))
 
 
+def _folded(shape, strides):
+    """A view's (stride, extent) pairs: adjacent dimensions that follow one another in memory as one."""
+    dims = []
+    for n, s in zip(reversed(shape), reversed(strides)):
+        if n > 1 and dims and s == dims[-1][0] * dims[-1][1]:
+            dims[-1] = (dims[-1][0], dims[-1][1] * n)
+        elif n > 1:
+            dims.append((s, n))
+    return dims
+
+
+@functools.lru_cache(maxsize=4096)
+def _overlap(delta, a_shape, a_strides, b_shape, b_strides):
+    """Whether two views, b starting ``delta`` elements behind a, have an element in common: whole numbers i within a's
+    extents and j within b's with sum i * a's strides - sum j * b's strides == delta.  Dimensions with the same
+    stride count together; going from the largest stride down, a number is tried only where the smaller strides
+    can still make up the rest, which leaves one or two for the views of a hub.  A search that does not end soon
+    counts as an overlap."""
+    reach = {}
+    for dims, sign in ((_folded(a_shape, a_strides), 1), (_folded(b_shape, b_strides), -1)):
+        for s, n in dims:
+            if s == 0:
+                continue
+            lo, hi = reach.get(abs(s), (0, 0))
+            step = sign * (n - 1) * (1 if s > 0 else -1)
+            reach[abs(s)] = (lo + min(step, 0), hi + max(step, 0))
+    terms = sorted(((s, lo, hi) for s, (lo, hi) in reach.items()), reverse=True)
+    below = [(0, 0)]                                   # what the strides behind a place in the order can make up
+    for s, lo, hi in reversed(terms):
+        below.insert(0, (below[0][0] + s * lo, below[0][1] + s * hi))
+    tries = 10000
+
+    def search(i, rest):
+        nonlocal tries
+        if i == len(terms):
+            return rest == 0
+        s, lo, hi = terms[i]
+        least, most = below[i + 1]
+        for x in range(max(lo, -((most - rest) // s)), min(hi, (rest - least) // s) + 1):
+            tries -= 1
+            if tries < 0 or search(i + 1, rest - s * x):
+                return True
+        return False
+    return search(0, delta)
+
+
 def _apart(outputs, inputs, allowed=()):
-    """Refuse an output that starts where another operand starts, and contiguous ones that overlap at all
-    (two row-pitched views may interleave in one buffer, as the columns of a hub do).  An output that may be
-    an input has to be the same view: with another row pitch it would write rows that are still to be read.
-    Called when operands meet (``_meet``)."""
-    seen = [(n, a) for n, a in inputs if a is not None and a.size]
+    """Refuse an output that has an element in common with another operand (row-pitched views may interleave in one
+    buffer, as the columns of a hub do).  An output that may be an input has to be the same view: with another row
+    pitch it would write rows that are still to be read.  Called when operands meet (``_meet``)."""
+    seen = [(n, a) + _span(a) for n, a in inputs if a is not None and a.size]
     for name, a in outputs:
         if a is None or not a.size:
             continue
         lo, hi = _span(a)
-        for other, b in seen:
-            if (name, other) in allowed and _same(a, b):
+        for other, b, b_lo, b_hi in seen:
+            if lo >= b_hi or b_lo >= hi or (name, other) in allowed and _same(a, b):
                 continue
-            if a.ptr == b.ptr or (a._contig or b._contig) and lo < _span(b)[1] and _span(b)[0] < hi:
+            delta = b_lo - lo
+            if delta % 4 or _overlap(delta // 4, a.shape, a.strides, b.shape, b.strides):
                 raise ValueError('%s overlaps %s' % (name, other))
-        seen.append((name, a))
+        seen.append((name, a, lo, hi))
 
 
 _Strides12, _Strides21 = ctypes.c_int64 * 12, ctypes.c_int64 * 21

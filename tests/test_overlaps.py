@@ -1,6 +1,7 @@
 """Calls of the sequence operators whose arrays share memory: in place where that is allowed, refused elsewhere.
 
 The checks come before any launch, so they are tested on views of addresses that nothing is read from."""
+import numpy as np
 import pytest
 
 
@@ -77,3 +78,69 @@ def test_the_library_takes_the_same_rows_in_place():
     backward(2 * W)
     with pytest.raises(B200Error, match='row pitch'):
         backward(W)
+
+
+# column ranges of one hub, as (first column, columns), and row ranges
+@pytest.mark.parametrize('x_out, overlaps', [((0, W), True), ((2, W), True), ((1 + W, W), False), ((1, W), False)])
+def test_column_ranges_of_a_hub(ops, x_out, overlaps):
+    hub = _array(0, ROWS, 2 * W + 1)
+    x, out = hub[:, 1:W + 1], hub[:, x_out[0]:sum(x_out)]
+    with pytest.raises(ValueError if overlaps else _Reached, match='x_out overlaps x' if overlaps else None):
+        _norm_forward(ops, x, _array(1, ROWS, W), out, _array(2, ROWS, W))
+    with pytest.raises(ValueError if overlaps else _Reached, match='dx overlaps dx_out' if overlaps else None):
+        _norm_backward(ops, x, out)
+
+
+@pytest.mark.parametrize('shift, overlaps', [(8, True), (-8, True), (31, True), (32, False), (96, False), (-32, False)])
+@pytest.mark.parametrize('T', [1, 4])
+def test_attention_outputs_in_a_hub(ops, T, shift, overlaps):
+    """q in columns 32 to 63 of a hub of 160, the output `shift` columns further on."""
+    hub, start = _array(0, T, 2, 160), 32
+    part = lambda c: hub[:, :, c:c + 32].reshape((T, 2, 4, 8))  # noqa: E731
+    q, out, k, v, decay = part(start), part(start + shift), _array(1, T, 2, 4, 8), _array(2, T, 2, 4, 8), _array(3, 4)
+    error, text = (ValueError, 'overlaps q') if overlaps else (_Reached, None)
+    with pytest.raises(error, match=text and 'out ' + text):
+        ops.linear_attention_forward(q, k, v, decay, out)
+    with pytest.raises(error, match=text and 'dq ' + text):
+        ops.linear_attention_backward(q, k, v, decay, _array(4, T, 2, 4, 8), out, _array(5, T, 2, 4, 8), _array(6, T, 2, 4, 8))
+    with pytest.raises(error, match=text and 'out ' + text):
+        ops.linear_attention_step(q[0], k[0], v[0], decay, _array(7, 2, 4, 8, 8), out[0])
+
+
+def test_rows_of_a_hub(ops):
+    """Alternate rows do not meet, nor do earlier and later ones; rows that both views hold do."""
+    hub = _array(0, 3 * ROWS, 2 * W)
+    y, h_out = _array(1, ROWS, W), _array(2, ROWS, W)
+    for x, x_out in ((hub[0:2 * ROWS:2, :W], hub[1:2 * ROWS + 1:2, :W]), (hub[:ROWS, :W], hub[ROWS:2 * ROWS, :W]), (hub[:ROWS, :W], hub[1:ROWS + 1, W:])):
+        with pytest.raises(_Reached):
+            _norm_forward(ops, x, y, x_out, h_out)
+    for x, x_out in ((hub[:ROWS, :W], hub[1:ROWS + 1, :W]), (hub[0:2 * ROWS:2, :W], hub[2:2 * ROWS + 2:2, :W]), (hub[:ROWS, :W], hub[1:2 * ROWS + 1:2, :W]),
+                     (hub[:ROWS, :W], hub[1:ROWS + 1, W - 1:2 * W - 1])):
+        with pytest.raises(ValueError, match='x_out overlaps x'):
+            _norm_forward(ops, x, y, x_out, h_out)
+
+
+def _places(offset, shape, strides):
+    return {offset + sum(i * s for i, s in zip(index, strides)) for index in np.ndindex(*shape)}
+
+
+def test_the_rule_against_enumeration():
+    """Small views of up to three dimensions, nested, interleaved and folded, against the sets of their elements."""
+    from brainstorm_b200.sequence_ops import _overlap
+    rs = np.random.RandomState(0)
+    met = 0
+    for _ in range(4000):
+        (a_shape, a_strides), (b_shape, b_strides) = [
+            (tuple(int(i) for i in rs.randint(1, 5, n)), tuple(int(i) for i in rs.choice([0, 1, 1, 2, 3, 4, 6, 7, 12, 24, 25], n))) for n in rs.randint(1, 4, 2)]
+        delta = int(rs.randint(-40, 41))
+        want = bool(_places(0, a_shape, a_strides) & _places(delta, b_shape, b_strides))
+        assert _overlap(delta, a_shape, a_strides, b_shape, b_strides) == want, (delta, a_shape, a_strides, b_shape, b_strides)
+        met += want
+    assert 500 < met < 3500
+
+
+def test_views_that_cannot_be_told_apart_in_time_are_refused():
+    """Strides without any nesting make the search long: it gives up and says that they may overlap."""
+    from brainstorm_b200.sequence_ops import _overlap
+    shape, strides = (997, 991, 983, 977), (9973, 9967, 9949, 9941)
+    assert _overlap(3, shape, strides, shape, tuple(s + 2 for s in strides))
