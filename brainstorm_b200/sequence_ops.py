@@ -73,6 +73,24 @@ def _heads(a, what):
     return tuple(a.strides[:3]) if len(a.shape) == 4 else (0,) + tuple(a.strides[:2])
 
 
+@functools.lru_cache(maxsize=4096)
+def _folds(shape, strides):
+    """Whether a view may hold one element twice: a stride that does not reach past the smaller ones together."""
+    past = 0
+    for s, n in sorted((s, n) for n, s in zip(shape, strides) if n > 1):
+        if s <= past:
+            return True
+        past += s * (n - 1)
+    return False
+
+
+def _result_heads(a, what):
+    """_heads of an array that is written."""
+    if a.size and _folds(a.shape, a.strides):
+        raise ValueError('%s overlaps itself' % what)
+    return _heads(a, what)
+
+
 def _expect(a, shape, what):
     if a.shape != shape:
         raise ValueError('%s has shape %r, expected %r' % (what, a.shape, shape))
@@ -183,7 +201,8 @@ class SequenceOps(object):
         Args:
             q, out: (T, B, H, dk) and (T, B, H, dv).
             k, v: (T, B, K, dk) and (T, B, K, dv); K divides H, head h of q reads head ``h // (H // K)``.
-                The last dimension of all four must be contiguous; the others may be strided.
+                The last dimension of all four must be contiguous; the others may be strided (for results: without an
+                element that lies in two places).
             decay: (H,), a constant factor for each head.
             state, state_out: (B, H, dk, dv) before the first and after the last token; ``state=None`` starts
                 from zero.  ``state_out`` may be ``state``.
@@ -197,7 +216,7 @@ class SequenceOps(object):
         _expect(out, (T, B, H, dv), 'out')
         strides = 0
         if not (q._contig and k._contig and v._contig and out._contig):
-            strides = _Strides12(*(_heads(q, 'q') + _heads(k, 'k') + _heads(v, 'v') + _heads(out, 'out')))
+            strides = _Strides12(*(_heads(q, 'q') + _heads(k, 'k') + _heads(v, 'v') + _result_heads(out, 'out')))
         if _meet((q, k, v, out, decay, state, state_out, lengths)):
             _apart((('out', out), ('state_out', state_out)), (('q', q), ('k', k), ('v', v), ('decay', decay), ('state', state), ('lengths', lengths)),
                    (('state_out', 'state'),))
@@ -221,7 +240,7 @@ class SequenceOps(object):
         arrays = (('q', q), ('k', k), ('v', v), ('dout', dout), ('dq', dq), ('dk', dk), ('dv', dv))
         strides = 0
         if not all(a._contig for _, a in arrays):
-            strides = _Strides21(*[s for what, a in arrays for s in _heads(a, what)])
+            strides = _Strides21(*[s for i, (what, a) in enumerate(arrays) for s in (_result_heads if i > 3 else _heads)(a, what)])
         if _meet((q, k, v, dout, dq, dk, dv, decay, state, dstate_out, dstate, lengths)):
             _apart(arrays[4:] + (('dstate', dstate),),
                    arrays[:4] + (('decay', decay), ('state', state), ('dstate_out', dstate_out), ('lengths', lengths)))
@@ -240,7 +259,7 @@ class SequenceOps(object):
         _expect(out, (B, H, dv), 'out')
         strides = 0
         if not (q._contig and k._contig and v._contig and out._contig):
-            strides = _Strides12(*(_heads(q, 'q') + _heads(k, 'k') + _heads(v, 'v') + _heads(out, 'out')))
+            strides = _Strides12(*(_heads(q, 'q') + _heads(k, 'k') + _heads(v, 'v') + _result_heads(out, 'out')))
         if _meet((q, k, v, out, decay, state)):
             _apart((('out', out), ('state', state)), (('q', q), ('k', k), ('v', v), ('decay', decay)))
         s = _whole(state, (B, H, dk, dv), 'state')

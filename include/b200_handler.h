@@ -395,7 +395,7 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      dout, dq, dk, dv (backward); NULL: all of them are contiguous.  q, out have H heads, k and v kv_heads, H a multiple of
  *      kv_heads: head h reads key/value head h / (H / kv_heads).  dk, dv: 1 .. 128.  state,
  *      state_out, dstate_out, dstate: contiguous (B, H, dk, dv), each may be NULL (zeros in,
- *      not wanted out); state_out may be state; no other output may overlap
+ *      not wanted out); state_out may be state; no other output may overlap itself,
  *      an input or another output.  decay is a constant of the layer, any finite
  *      values, not differentiated.  Backward: gradients of sum(out * dout) + sum(state_out *
  *      dstate_out), ADDED to dq, dk, dv (not to dstate) when accumulate is set; they are

@@ -144,3 +144,28 @@ def test_views_that_cannot_be_told_apart_in_time_are_refused():
     from brainstorm_b200.sequence_ops import _overlap
     shape, strides = (997, 991, 983, 977), (9973, 9967, 9949, 9941)
     assert _overlap(3, shape, strides, shape, tuple(s + 2 for s in strides))
+
+
+def test_outputs_that_fold_onto_themselves(ops):
+    """Views built with a stride of zero, or rows that run into one another: read, but not written."""
+    from brainstorm_b200 import B200Array
+    T, B, H, d = 4, 2, 3, 8
+    a = lambda i, heads=H: _array(i, T, B, heads, d)  # noqa: E731
+    shared = lambda i: B200Array(None, (i + 1) << 20, (T, B, H, d), (B * d, d, 0, 1))  # noqa: E731
+    close = lambda i: B200Array(None, (i + 1) << 20, (T, B, H, d), (B * (H * d - 1), H * d - 1, d, 1))  # noqa: E731
+    turned = B200Array(None, 9 << 20, (T, B, H, d), (d, T * d, B * T * d, 1))      # batch and heads before time
+    decay = _array(20, H)
+    for out in (shared(1), close(1)):
+        with pytest.raises(ValueError, match='out overlaps itself'):
+            ops.linear_attention_forward(a(2), a(3), a(4), decay, out)
+        with pytest.raises(ValueError, match='out overlaps itself'):
+            ops.linear_attention_step(a(2)[0], a(3)[0], a(4)[0], decay, _array(5, B, H, d, d), out[0])
+        for i, name in enumerate(('dq', 'dk', 'dv')):
+            grads = [a(6), a(7), a(8)]
+            grads[i] = out
+            with pytest.raises(ValueError, match=name + ' overlaps itself'):
+                ops.linear_attention_backward(a(2), a(3), a(4), decay, a(5), *grads)
+    with pytest.raises(_Reached):
+        ops.linear_attention_forward(shared(1), close(2), shared(3), decay, turned)
+    with pytest.raises(_Reached):
+        ops.linear_attention_backward(shared(1), close(2), shared(3), decay, shared(4), turned, a(10), a(11))
