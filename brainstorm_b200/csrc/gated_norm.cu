@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 256 ? 1 : E == 16 ? 2 : 3) 
       for (int e = 0; e < E; ++e) d[e] += r_pre * (h[e] - x[e] * m);
     }
     if (live) {
-      if (p.accumulate) {
+      if (p.accumulate && p.dx != p.dx_out) {      // in the place of dx_out, what is there is in d already
         float o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = d[e];

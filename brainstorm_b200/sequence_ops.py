@@ -324,7 +324,8 @@ class SequenceOps(object):
         """Gradients of ``gated_norm_forward`` from those of ``x_out`` (``dx_out``, None: zero) and ``h_out`` (``dh``,
         None: it was not taken).  ``y``, ``gate`` and the weights are None where they were in the forward pass; a
         vector gradient that is None is not computed.  Adds to all gradients, or overwrites them without
-        ``accumulate``.  Without a block output ``x_out`` is the forward pass's ``x``.  ``dx`` may be ``dx_out``."""
+        ``accumulate``.  Without a block output ``x_out`` is the forward pass's ``x``.  ``dx`` may be ``dx_out``, the same view:
+        it becomes the gradient of ``x``, in which ``dx_out`` counts once, with ``accumulate`` or without."""
         act = _activation(activation)
         if len(dx.shape) != 2:
             raise ValueError('expected 2-D arrays, got shape %r' % (dx.shape,))

@@ -410,7 +410,7 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      width up to 16384.  x_out may be x, h_out may be y, with the same pitch.  Backward takes the gradients
  *      dx_out (NULL: zero) and dh (NULL: no h_out was taken) and gives dx, dy, dgate and the
  *      vectors dw_post, dscale, dw_pre (each may be NULL); accumulate: all are ADDED to.  dx
- *      may be dx_out, with the same pitch.  scratch of b200_gated_norm_scratch_floats(rows, width) floats for the
+ *      may be dx_out, with the same pitch: it is then overwritten, dx_out counts once.  scratch of b200_gated_norm_scratch_floats(rows, width) floats for the
  *      vectors' partial sums.
  *
  *      The two forward calls, which also serve single tokens, take their arguments in one struct: a
