@@ -6,10 +6,12 @@
 //
 // One block of four warps walks the chunks of one (sequence, head), or of a segment of them, for up to 64
 // columns of v, with the state in registers.  All four products run on mma.sync.m16n8k16 in fp32 accuracy:
-// every operand x is scaled by a power of two (per tile, per row for q and the scores) and split into two
-// half-precision parts, hi = fp16(x), lo = fp16(x - hi), 22 bits together, and a product is hi.hi + hi.lo +
-// lo.hi.  A value more than 2^17 below the largest of its tile begins to lose bits (the error stays below
-// 2^-39 of that largest value).
+// every operand x is scaled by a power of two and split into two half-precision parts, hi = fp16(x), lo = fp16(x - hi), 22
+// bits together, and a product is hi.hi + hi.lo + lo.hi.  A scale belongs to one token's row of q, k or v, to one row of
+// scores, or to the state: what a token's output does not depend on, a later token above all, does not decide a scale
+// that it is computed with.  The scales of k and v are taken back where the scores get their decay, and enter the weights
+// with which a chunk's keys and values are added to the state.  A value more than 2^17 below the largest of its row, or of
+// the state, begins to lose bits (the error stays below 2^-38 of that largest value).
 //
 // Why mma.sync and not tcgen05: a chunk's products are 64 x 64 x d with a mask, weights and a new split
 // between them; the split and the weights want the accumulators in the registers that compute them, where
@@ -130,12 +132,15 @@ __device__ __forceinline__ float lc_size(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;
 }
-// The power of two that takes a largest value m into [2^13, 2^14); *inv its reciprocal.
+// 2^k, k from -126 to 127
+__device__ __forceinline__ float lc_pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+// k of the power of two that takes a largest value m = 1.. * 2^(biased - 127) into [2^13, 2^14)
+__device__ __forceinline__ int lc_scale_exponent(int biased) { return min(140 - biased, 126); }      // 2^126 and its reciprocal are both normal numbers
+// That power of two; *inv its reciprocal.
 __device__ __forceinline__ float lc_scale(float m, float* inv) {
-  const int e = (int)(__float_as_uint(m) >> 23) - 127;
-  const int k = min(13 - e, 126);         // 2^126 and its reciprocal are both normal numbers
-  *inv = __uint_as_float((uint32_t)(127 - k) << 23);
-  return __uint_as_float((uint32_t)(127 + k) << 23);
+  const int k = lc_scale_exponent((int)(__float_as_uint(m) >> 23));
+  *inv = lc_pow2(-k);
+  return lc_pow2(k);
 }
 // Byte offset of 16-byte group `g` of row `row` in a tile of halves with `pitch` bytes a row: groups are
 // permuted within their 128 bytes by the row, so that eight rows of one column meet eight bank groups.
@@ -170,6 +175,44 @@ __device__ __forceinline__ float lc_max(const float (&x)[M][N][4]) {
   return m;
 }
 #define LC_INF __int_as_float(0x7f800000)
+// Biased exponents of the largest finite magnitude of each row of a tile, two rows in a word: a row lies in LANES
+// neighbouring lanes, one float4 each; all rows' shuffles together.  All lanes of the warp call it.
+template <int LANES, int N>
+__device__ __forceinline__ void lc_row_exponents(uint32_t (&e)[N / 2], const float4 (&x)[N]) {
+  float m[N];
+  bool inf = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    m[i] = lc_max4<false>(0.f, x[i]);
+    inf = inf || m[i] == LC_INF;
+  }
+  if (__any_sync(0xffffffffu, inf)) {      // an infinity must not decide a scale
+#pragma unroll
+    for (int i = 0; i < N; ++i) m[i] = lc_max4<true>(0.f, x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) e[i] = __float_as_uint(m[2 * i]) >> 23 | __float_as_uint(m[2 * i + 1]) >> 23 << 16;
+#pragma unroll
+  for (int s = 1; s < LANES; s <<= 1)
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) e[i] = __vmaxu2(e[i], __shfl_xor_sync(0xffffffffu, e[i], s));
+}
+template <int N>
+__device__ __forceinline__ int lc_row_scale(const uint32_t (&e)[N], int i) { return lc_scale_exponent((int)(e[i / 2] >> (i & 1) * 16 & 0xffff)); }
+// The weights of a chunk's n tokens in the state after it, l^(n-1-j) k_inv[j] v_inv[j], as u0 (token `lane`), u1 (token 32 + `lane`),
+// all below 2, times 2^(*f0's and *f1's exponents): taken together a weight may be outside the range of float32, and the
+// largest decides the scale, so that a token that the decay has removed does not count.
+__device__ __forceinline__ void lc_weights(float& u0, float& u1, float& f0, float& f1, const float* pw, const float* k_inv, const float* v_inv, int n, int lane) {
+  auto exponent = [](float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; };
+  const float p0 = lane < n ? pw[n - 1 - lane] : 0.f, p1 = lane + 32 < n ? pw[n - 33 - lane] : 0.f;
+  const int e0 = exponent(k_inv[lane]) + exponent(v_inv[lane]), e1 = exponent(k_inv[lane + 32]) + exponent(v_inv[lane + 32]);
+  const int top = __reduce_max_sync(0xffffffffu, max(p0 != 0.f ? e0 + exponent(p0) : -1000, p1 != 0.f ? e1 + exponent(p1) : -1000));
+  u0 = scalbnf(p0, e0 - top);
+  u1 = scalbnf(p1, e1 - top);
+  const int half = top / 2;
+  f0 = lc_pow2(max(-126, min(127, half)));
+  f1 = lc_pow2(max(-126, min(127, top - half)));
+}
 __device__ __forceinline__ void lc_put4(uint8_t* hi, uint8_t* lo, int row, int c, int pitch, float4 x, float s) {
   uint32_t h0, l0, h1, l1;
   lc_split(x.x * s, x.y * s, h0, l0);
@@ -197,8 +240,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
   constexpr int LPR = DK / 4, RPP = THREADS / LPR;   // lanes per row of k, rows in a pass
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ float pw_pad[16 + LC + 1];              // powers of the decay, zeros before
-  __shared__ float q_inv[LC];                        // 1 / scale of each row of q
-  __shared__ float red[3][THREADS / 32];
+  __shared__ __align__(8) float k_inv[LC], v_inv[LC];      // 1 / scale of each row
+  __shared__ int8_t q_exp[LC];                       // exponent of the scale of each row of q (a float each would not leave room for two blocks)
+  __shared__ float red[THREADS / 32];
   const float* pw = pw_pad + 16;
 
   const LaChunkRun& cr = runs.run[blockIdx.y];
@@ -314,73 +358,49 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
       for (int it = 0; it < QN; ++it, qp += RPP * q_t)
         qr[it] = (it0 + it) * RPP + tid / LPR < n ? lc_row4<VEC>(qp, kc, dk) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
-    auto put_q = [&](int it0) {      // each row by its own scale: a row lies in LPR neighbouring lanes; all rows' shuffles together
-      float m[QN];
-      bool inf = false;
+    auto put_q = [&](int it0) {
+      uint32_t e[QN / 2];
+      lc_row_exponents<LPR>(e, qr);
 #pragma unroll
       for (int it = 0; it < QN; ++it) {
-        m[it] = lc_max4<false>(0.f, qr[it]);
-        inf = inf || m[it] == LC_INF;
-      }
-      if (__any_sync(0xffffffffu, inf)) {
-#pragma unroll
-        for (int it = 0; it < QN; ++it) m[it] = lc_max4<true>(0.f, qr[it]);
-      }
-#pragma unroll
-      for (int s = 1; s < LPR; s <<= 1)
-#pragma unroll
-        for (int it = 0; it < QN; ++it) m[it] = fmaxf(m[it], __shfl_xor_sync(0xffffffffu, m[it], s));
-#pragma unroll
-      for (int it = 0; it < QN; ++it) {
-        const int i = (it0 + it) * RPP + tid / LPR;
-        float inv;
-        const float sc = lc_scale(m[it], &inv);
-        lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, kc, L::KP, qr[it], sc);
-        if (tid % LPR == 0) q_inv[i] = inv;
+        const int i = (it0 + it) * RPP + tid / LPR, x = lc_row_scale(e, it);
+        lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, kc, L::KP, qr[it], lc_pow2(x));
+        if (tid % LPR == 0) q_exp[i] = (int8_t)x;
       }
     };
     if (QN == KN) load_q(0);
-    auto publish = [&](float mk, float mv, float ms) {
+    uint32_t ke[KN / 2], ve[VN / 2];
+    lc_row_exponents<LPR>(ke, kr);
+    lc_row_exponents<16>(ve, vr);
+    auto publish = [&](float m) {
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) {      // three chains of shuffles side by side
-        mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, s));
-        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, s));
-        ms = fmaxf(ms, __shfl_xor_sync(0xffffffffu, ms, s));
-      }
-      if (lane == 0) {
-        red[0][warp] = mk;
-        red[1][warp] = mv;
-        red[2][warp] = ms;
-      }
+      for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+      if (lane == 0) red[warp] = m;
       __syncthreads();
-    };
-    auto largest = [&](int i) {
-      float m = red[i][0];
+      m = red[0];
 #pragma unroll
-      for (int u = 1; u < THREADS / 32; ++u) m = fmaxf(m, red[i][u]);
+      for (int u = 1; u < THREADS / 32; ++u) m = fmaxf(m, red[u]);
       return m;
     };
-    publish(lc_max<false>(kr), lc_max<false>(vr), lc_max<false>(S));      // behind it the tiles of the chunk before are free
-    if (fmaxf(fmaxf(largest(0), largest(1)), largest(2)) == LC_INF) {      // an infinity must not decide a scale
+    float s_max = publish(lc_max<false>(S));           // behind it the tiles of the chunk before are free
+    if (s_max == LC_INF) {
       __syncthreads();
-      publish(lc_max<true>(kr), lc_max<true>(vr), lc_max<true>(S));
+      s_max = publish(lc_max<true>(S));
     }
-    struct {
-      float k, v, s, w, k_inv, v_inv, s_inv, w_inv;
-    } x;
-    x.k = lc_scale(largest(0), &x.k_inv);
-    x.v = lc_scale(largest(1), &x.v_inv);
-    x.s = lc_scale(largest(2), &x.s_inv);
-    x.w = x.w_inv = 1.f;
-    const float w_max = fabsf(pw[n - 1]);              // weights above one (a decay above one) are taken back below two
-    if (w_max > 1.f) {
-      x.w = lc_scale(w_max, &x.w_inv) * 0x1p-13f;
-      x.w_inv *= 0x1p13f;
+    float s_inv;
+    const float s_scale = lc_scale(s_max, &s_inv);
+#pragma unroll
+    for (int it = 0; it < KN; ++it) {
+      const int i = it * RPP + tid / LPR, x = lc_row_scale(ke, it);
+      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], lc_pow2(x));
+      if (tid % LPR == 0) k_inv[i] = lc_pow2(-x);
     }
 #pragma unroll
-    for (int it = 0; it < KN; ++it) lc_put4(sm + L::K_HI, sm + L::K_LO, it * RPP + tid / LPR, kc, L::KP, kr[it], x.k);
-#pragma unroll
-    for (int it = 0; it < VN; ++it) lc_put4(sm + L::V_HI, sm + L::V_LO, it * (LC / VN) + (tid >> 4), vc, L::VP, vr[it], x.v);
+    for (int it = 0; it < VN; ++it) {
+      const int i = it * (LC / VN) + (tid >> 4), x = lc_row_scale(ve, it);
+      lc_put4(sm + L::V_HI, sm + L::V_LO, i, vc, L::VP, vr[it], lc_pow2(x));
+      if ((tid & 15) == 0) v_inv[i] = lc_pow2(-x);
+    }
     if (QN != KN) load_q(0);
     put_q(0);
     if (QN != KN) {
@@ -394,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           uint32_t hi, lo;
-          lc_split(S[m][nt][e] * x.s, S[m][nt][e + 1] * x.s, hi, lo);
+          lc_split(S[m][nt][e] * s_scale, S[m][nt][e + 1] * s_scale, hi, lo);
           const uint32_t at = lc_at(row_of(m, e), nt0 + nt, L::VP) + t2 * 2;
           *reinterpret_cast<uint32_t*>(sm + L::S_HI + at) = hi;
           *reinterpret_cast<uint32_t*>(sm + L::S_LO + at) = lo;
@@ -433,18 +453,21 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
           }
         lc_rows(acc_o, qh, ql, lc_smem(sm + L::S_HI), lc_smem(sm + L::S_LO), 16 * ks, lane, nt0, nt_n);
       }
-      // ---- weights and mask, then the scores' own scale for each row.  Element (nt, half, e) is apart by
-      // base - 8 (nt - half) - e tokens: the weight of half 1 is the one half 0 had a tile before.
+      // ---- weights, the scales of q, k and v taken back, and mask, then the scores' own scale for each row.  Element
+      // (nt, half, e) is apart by base - 8 (nt - half) - e tokens: the weight of half 1 is the one half 0 had a tile before.
+      // The factors one after the other: two of them together could leave the range of float32.
       const float* pb = pw + (i0 + g - t2);
+      const float q_inv0 = lc_pow2(-q_exp[i0 + g]), q_inv1 = lc_pow2(-q_exp[i0 + g + 8]);
       float m0 = 0.f, m1 = 0.f, b0 = pb[8], b1 = pb[7];
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
         if (nt < 2 * r + 2) {
           const float a0 = pb[-8 * nt], a1 = pb[-8 * nt - 1];
-          P[nt][0] *= a0;
-          P[nt][1] *= a1;
-          P[nt][2] *= b0;
-          P[nt][3] *= b1;
+          const float2 k2 = *reinterpret_cast<const float2*>(k_inv + 8 * nt + t2), v2 = *reinterpret_cast<const float2*>(v_inv + 8 * nt + t2);
+          P[nt][0] = P[nt][0] * q_inv0 * a0 * k2.x * v2.x;
+          P[nt][1] = P[nt][1] * q_inv0 * a1 * k2.y * v2.y;
+          P[nt][2] = P[nt][2] * q_inv1 * b0 * k2.x * v2.x;
+          P[nt][3] = P[nt][3] * q_inv1 * b1 * k2.y * v2.y;
           if (nt >= 2 * r) {                            // the tiles on the diagonal
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -493,8 +516,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
         const int i = i0 + g + 8 * half;
         if (i < n) {
           // the factors one after the other where their product could leave the range of float32
-          const float f_o0 = x.s_inv * q_inv[i], f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
-          const float f_p0 = (half ? p_inv1 : p_inv0) * x.v_inv, f_p1 = q_inv[i] * x.k_inv * (p.o_scale * p.k_scale);
+          const float f_o0 = s_inv * (half ? q_inv1 : q_inv0), f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
+          const float f_p0 = half ? p_inv1 : p_inv0, f_p1 = p.o_scale * p.k_scale;
           float* row = o_base + (tok0 * p.os.t + (c0 + i) * o_t);
           if (VEC && !p.accumulate) {
 #pragma unroll
@@ -518,6 +541,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
     }
     // ---- the state after the chunk; each element of k is met once here and takes its weight on the way
     const float keep = pw[n - (undecayed ? 1 : 0)];
+    float u0, u1, f0, f1;
+    lc_weights(u0, u1, f0, f1, pw, k_inv, v_inv, n, lane);
+    f1 *= p.k_scale;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       const int r0 = 16 * (w + 4 * m);
@@ -537,8 +563,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
             {
 #pragma unroll
               for (int e = 0; e < 2; ++e) {             // tokens 16 kt + 8 e + t2 and the next
-                const int i = n - 1 - (16 * kt + 8 * e + t2);
-                const float w0 = (i >= 0 ? pw[i] : 0.f) * x.w, w1 = (i >= 1 ? pw[i - 1] : 0.f) * x.w;
+                const int from = (16 * kt + 8 * e + t2) & 31;
+                const float w0 = __shfl_sync(0xffffffffu, kt < 2 ? u0 : u1, from), w1 = __shfl_sync(0xffffffffu, kt < 2 ? u0 : u1, from + 1);
 #pragma unroll
                 for (int r = 2 * e; r < 2 * e + 2; ++r) {
                   const float2 y = lc_join(ah[r], al[r]);
@@ -548,7 +574,6 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
             }
             lc_rows(acc, ah, al, lc_smem(sm + L::V_HI), lc_smem(sm + L::V_LO), 16 * kt, lane, nt0, nt_n);
           }
-        const float f0 = x.k_inv * x.w_inv, f1 = x.v_inv * p.k_scale;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -588,8 +613,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaC
   constexpr int KP = DK * 2, VP = LC_COLS * 2, K_LO = LC * KP, V_HI = 2 * LC * KP, V_LO = V_HI + LC * VP;
   constexpr int MT = DK / 64, LPR = DK / 4, RPP = LS_THREADS / LPR, KN = LC / RPP, VN = LC * 16 / LS_THREADS;
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ float pw[LC + 1];
-  __shared__ float red[2][8];
+  __shared__ float pw[LC + 1], k_inv[LC], v_inv[LC];
 
   const LaChunkRun& cr = runs.run[blockIdx.y];
   const LaRun& p = cr.r;
@@ -635,48 +659,30 @@ __global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaC
   load(first);
   for (int64_t c0 = first; c0 < n_end; c0 += LC) {
     const int n = (int)min((int64_t)LC, n_end - c0);
-    auto publish = [&](float mk, float mv) {
+    uint32_t ke[KN / 2], ve[VN / 2];
+    lc_row_exponents<LPR>(ke, kr);
+    lc_row_exponents<16>(ve, vr);
 #pragma unroll
-      for (int s = 16; s > 0; s >>= 1) {
-        mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, s));
-        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, s));
-      }
-      if (lane == 0) {
-        red[0][warp] = mk;
-        red[1][warp] = mv;
-      }
-      __syncthreads();
-    };
-    auto largest = [&](int i) {
-      float m = red[i][0];
+    for (int it = 0; it < KN; ++it)
+      if (tid % LPR == 0) k_inv[it * RPP + tid / LPR] = lc_pow2(-lc_row_scale(ke, it));
 #pragma unroll
-      for (int u = 1; u < 8; ++u) m = fmaxf(m, red[i][u]);
-      return m;
-    };
-    publish(lc_max<false>(kr), lc_max<false>(vr));
-    float mk = largest(0), mv = largest(1);
-    if (fmaxf(mk, mv) == LC_INF) {
-      __syncthreads();
-      publish(lc_max<true>(kr), lc_max<true>(vr));
-      mk = largest(0);
-      mv = largest(1);
-    }
-    float k_inv, v_inv, w_inv = 1.f, w_s = 1.f;
-    const float k_s = lc_scale(mk, &k_inv), v_s = lc_scale(mv, &v_inv), w_max = fabsf(pw[n - 1]);
-    if (w_max > 1.f) {
-      w_s = lc_scale(w_max, &w_inv) * 0x1p-13f;
-      w_inv *= 0x1p13f;
-    }
+    for (int it = 0; it < VN; ++it)
+      if ((tid & 15) == 0) v_inv[it * (LC / VN) + (tid >> 4)] = lc_pow2(-lc_row_scale(ve, it));
+    __syncthreads();      // the scales are in place, and the tiles of the chunk before are free
+    float u0, u1, f0, f1;
+    lc_weights(u0, u1, f0, f1, pw, k_inv, v_inv, n, lane);
 #pragma unroll
     for (int it = 0; it < KN; ++it) {
       const int i = it * RPP + tid / LPR;
-      lc_put4(sm, sm + K_LO, i, kc, KP, kr[it], i < n ? k_s * (pw[n - 1 - i] * w_s) : 0.f);
+      const float u = __shfl_sync(0xffffffffu, it * RPP < 32 ? u0 : u1, i & 31);
+      lc_put4(sm, sm + K_LO, i, kc, KP, kr[it], lc_pow2(lc_row_scale(ke, it)) * u);
     }
 #pragma unroll
-    for (int it = 0; it < VN; ++it) lc_put4(sm + V_HI, sm + V_LO, it * (LC / VN) + (tid >> 4), vc, VP, vr[it], v_s);
+    for (int it = 0; it < VN; ++it) lc_put4(sm + V_HI, sm + V_LO, it * (LC / VN) + (tid >> 4), vc, VP, vr[it], lc_pow2(lc_row_scale(ve, it)));
     __syncthreads();
     if (c0 + LC < n_end) load(c0 + LC);
-    const float keep = pw[n], f0 = k_inv * w_inv, f1 = v_inv * p.k_scale;
+    const float keep = pw[n];
+    f1 *= p.k_scale;
     if (nt0 < nt_n) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)

@@ -211,7 +211,9 @@ class SequenceOps(object):
                 inputs hold behind the end is not read.
 
         dk, dv: 1 to 128.  A non-finite value of a token spreads to later tokens of its sequence and head, and may
-        spread to up to 15 tokens before it."""
+        spread to up to 15 tokens before it.  Products are as exact as in float32 (22 bits of each operand, sums in float32).
+        From 9 tokens on, a value more than 2^17 below the largest of its row (one token and head of ``q``, ``k``, ``v`` or
+        ``dout``, and the state) keeps fewer bits: it is held to 2^-38 of that largest value.  Other tokens do not matter."""
         T, B, H, K, dk, dv = self._attention_shapes(q, k, v, 4)
         _expect(out, (T, B, H, dv), 'out')
         strides = 0

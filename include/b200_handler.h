@@ -400,6 +400,8 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      values, not differentiated.  Backward: gradients of sum(out * dout) + sum(state_out *
  *      dstate_out), ADDED to dq, dk, dv (not to dstate) when accumulate is set; they are
  *      zero behind the end of a sequence.  Sums run in a fixed order, no atomics.
+ *      From 9 tokens on operands have 22 bits; a value more than 2^17 below the largest of its row (one token and head; the
+ *      whole state) is held to 2^-38 of that largest value.
  *      16-byte aligned scratch of the given number of floats (0: NULL will do; it depends on the
  *      extents and on the number of SMs).
  *
