@@ -55,6 +55,11 @@ __device__ __forceinline__ double la_power(double l, int e) {
   return f;
 }
 
+// x, or the largest number in the place of an infinity: a factor beyond the range of float32 may meet zeros (tokens without
+// a key, a state that is zero still), which an infinity would turn into NaN.
+__device__ __forceinline__ float la_finite(float x) { return fabsf(x) > 3.402823466e38f ? copysignf(3.402823466e38f, x) : x; }
+__device__ __forceinline__ float la_power32(double l, int e) { return la_finite((float)la_power(l, e)); }
+
 int la_recurrent(const LaCommon& c, const LaRun* runs, int count);                      // linear_attention.cu
 int la_chunked(const LaCommon& c, const LaRun* runs, int count, float* work);           // linear_attention_chunks.cu
 int64_t la_chunked_work(int64_t T, int64_t BH, int dk, int dv, bool backward);          // floats

@@ -134,11 +134,10 @@ __device__ __forceinline__ float lc_size(float x) {
 }
 // 2^k, k from -126 to 127
 __device__ __forceinline__ float lc_pow2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
-// k of the power of two that takes a largest value m = 1.. * 2^(biased - 127) into [2^13, 2^14)
-__device__ __forceinline__ int lc_scale_exponent(int biased) { return min(140 - biased, 126); }      // 2^126 and its reciprocal are both normal numbers
-// That power of two; *inv its reciprocal.
+// The power of two that takes a largest value m into [2^13, 2^14); *inv its reciprocal.
 __device__ __forceinline__ float lc_scale(float m, float* inv) {
-  const int k = lc_scale_exponent((int)(__float_as_uint(m) >> 23));
+  const int e = (int)(__float_as_uint(m) >> 23) - 127;
+  const int k = min(13 - e, 126);         // 2^126 and its reciprocal are both normal numbers
   *inv = lc_pow2(-k);
   return lc_pow2(k);
 }
@@ -175,10 +174,11 @@ __device__ __forceinline__ float lc_max(const float (&x)[M][N][4]) {
   return m;
 }
 #define LC_INF __int_as_float(0x7f800000)
-// Biased exponents of the largest finite magnitude of each row of a tile, two rows in a word: a row lies in LANES
-// neighbouring lanes, one float4 each; all rows' shuffles together.  All lanes of the warp call it.
+// The scales of the rows of a tile, two rows in a word: biased exponents of the powers of two that take a row's largest finite
+// magnitude into (2^13, 2^14], 2^126 at most; 254 for a row of zeros.  A row lies in LANES neighbouring lanes, one
+// float4 each; all rows' shuffles together.  All lanes of the warp call it.
 template <int LANES, int N>
-__device__ __forceinline__ void lc_row_exponents(uint32_t (&e)[N / 2], const float4 (&x)[N]) {
+__device__ __forceinline__ void lc_row_scales(uint32_t (&e)[N / 2], const float4 (&x)[N]) {
   float m[N];
   bool inf = false;
 #pragma unroll
@@ -190,28 +190,39 @@ __device__ __forceinline__ void lc_row_exponents(uint32_t (&e)[N / 2], const flo
 #pragma unroll
     for (int i = 0; i < N; ++i) m[i] = lc_max4<true>(0.f, x[i]);
   }
+  // exponents rounded up, from 1 on for all but zero
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) e[i] = __float_as_uint(m[2 * i]) >> 23 | __float_as_uint(m[2 * i + 1]) >> 23 << 16;
+  for (int i = 0; i < N / 2; ++i) e[i] = __byte_perm(__float_as_uint(m[2 * i]) + 0x7fffffu >> 7, __float_as_uint(m[2 * i + 1]) + 0x7fffffu >> 7, 0x7632) & 0x01ff01ffu;
 #pragma unroll
   for (int s = 1; s < LANES; s <<= 1)
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) e[i] = __vmaxu2(e[i], __shfl_xor_sync(0xffffffffu, e[i], s));
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) e[i] = __vminu2(0x010c010cu - e[i], 0x00fd00fdu) + __vseteq2(e[i], 0);      // 268 - e is 141 - (e - 127) biased
 }
 template <int N>
-__device__ __forceinline__ int lc_row_scale(const uint32_t (&e)[N], int i) { return lc_scale_exponent((int)(e[i / 2] >> (i & 1) * 16 & 0xffff)); }
+__device__ __forceinline__ uint32_t lc_row(const uint32_t (&e)[N], int i) { return i & 1 ? e[i / 2] >> 16 : e[i / 2] & 0xffff; }
+__device__ __forceinline__ float lc_biased(uint32_t b) { return __uint_as_float(b << 23); }
+// 1 / scale, 0 for a row of zeros
+__device__ __forceinline__ float lc_inverse(uint32_t b) { return lc_biased(254 - b); }
 // The weights of a chunk's n tokens in the state after it, l^(n-1-j) k_inv[j] v_inv[j], as u0 (token `lane`), u1 (token 32 + `lane`),
 // all below 2, times 2^(*f0's and *f1's exponents): taken together a weight may be outside the range of float32, and the
-// largest decides the scale, so that a token that the decay has removed does not count.
+// largest decides the scale, so that a token that the decay has removed does not count, nor one without a key or a value.
 __device__ __forceinline__ void lc_weights(float& u0, float& u1, float& f0, float& f1, const float* pw, const float* k_inv, const float* v_inv, int n, int lane) {
   auto exponent = [](float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; };
-  const float p0 = lane < n ? pw[n - 1 - lane] : 0.f, p1 = lane + 32 < n ? pw[n - 33 - lane] : 0.f;
-  const int e0 = exponent(k_inv[lane]) + exponent(v_inv[lane]), e1 = exponent(k_inv[lane + 32]) + exponent(v_inv[lane + 32]);
+  const float k0 = k_inv[lane], k1 = k_inv[lane + 32], v0 = v_inv[lane], v1 = v_inv[lane + 32];
+  const float p0 = lane < n && k0 != 0.f && v0 != 0.f ? pw[n - 1 - lane] : 0.f, p1 = lane + 32 < n && k1 != 0.f && v1 != 0.f ? pw[n - 33 - lane] : 0.f;
+  const int e0 = exponent(k0) + exponent(v0), e1 = exponent(k1) + exponent(v1);
   const int top = __reduce_max_sync(0xffffffffu, max(p0 != 0.f ? e0 + exponent(p0) : -1000, p1 != 0.f ? e1 + exponent(p1) : -1000));
-  u0 = scalbnf(p0, e0 - top);
-  u1 = scalbnf(p1, e1 - top);
-  const int half = top / 2;
-  f0 = lc_pow2(max(-126, min(127, half)));
-  f1 = lc_pow2(max(-126, min(127, top - half)));
+  // in two factors: where a power of the decay is far below one, the other exponents may be far above the largest sum
+  auto scaled = [](float p, int e) {
+    const int half = e >> 1;
+    return p * lc_pow2(max(-126, min(127, half))) * lc_pow2(max(-126, min(127, e - half)));
+  };
+  u0 = scaled(p0, e0 - top);
+  u1 = scaled(p1, e1 - top);
+  f0 = lc_pow2(max(-126, min(127, top >> 1)));
+  f1 = lc_pow2(max(-126, min(127, top - (top >> 1))));
 }
 __device__ __forceinline__ void lc_put4(uint8_t* hi, uint8_t* lo, int row, int c, int pitch, float4 x, float s) {
   uint32_t h0, l0, h1, l1;
@@ -241,7 +252,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ float pw_pad[16 + LC + 1];              // powers of the decay, zeros before
   __shared__ __align__(8) float k_inv[LC], v_inv[LC];      // 1 / scale of each row
-  __shared__ int8_t q_exp[LC];                       // exponent of the scale of each row of q (a float each would not leave room for two blocks)
+  __shared__ uint8_t q_scale[LC];                    // biased exponents of the scales of q (a float each would not leave room for two blocks)
   __shared__ float red[THREADS / 32];
   const float* pw = pw_pad + 16;
 
@@ -276,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
   const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + v0 + tok0 * p.vs.t;
   float* o_base = p.o + (int64_t)b * p.os.b + (int64_t)(h / p.os.div) * p.os.h + v0;
 
-  if (tid < 16 + LC + 1) pw_pad[tid] = tid < 16 ? 0.f : (float)la_power(l, tid - 16);
+  if (tid < 16 + LC + 1) pw_pad[tid] = tid < 16 ? 0.f : la_power32(l, tid - 16);
   // Later tokens meet more keys: the blocks of an SM take the rows in opposite order, so that its four schedulers get
   // about the same share.
   const int r = ((NT == 8 ? blockIdx.x / sms : warp >> 2) & 1) ? 3 - w : w, i0 = 16 * r;      // this warp's tokens
@@ -360,18 +371,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
     };
     auto put_q = [&](int it0) {
       uint32_t e[QN / 2];
-      lc_row_exponents<LPR>(e, qr);
+      lc_row_scales<LPR>(e, qr);
 #pragma unroll
       for (int it = 0; it < QN; ++it) {
-        const int i = (it0 + it) * RPP + tid / LPR, x = lc_row_scale(e, it);
-        lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, kc, L::KP, qr[it], lc_pow2(x));
-        if (tid % LPR == 0) q_exp[i] = (int8_t)x;
+        const int i = (it0 + it) * RPP + tid / LPR;
+        lc_put4(sm + L::Q_HI, sm + L::Q_LO, i, kc, L::KP, qr[it], lc_biased(lc_row(e, it)));
+        if (tid % LPR == 0) q_scale[i] = (uint8_t)lc_row(e, it);
       }
     };
     if (QN == KN) load_q(0);
     uint32_t ke[KN / 2], ve[VN / 2];
-    lc_row_exponents<LPR>(ke, kr);
-    lc_row_exponents<16>(ve, vr);
+    lc_row_scales<LPR>(ke, kr);
+    lc_row_scales<16>(ve, vr);
     auto publish = [&](float m) {
 #pragma unroll
       for (int s = 16; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
@@ -391,15 +402,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
     const float s_scale = lc_scale(s_max, &s_inv);
 #pragma unroll
     for (int it = 0; it < KN; ++it) {
-      const int i = it * RPP + tid / LPR, x = lc_row_scale(ke, it);
-      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], lc_pow2(x));
-      if (tid % LPR == 0) k_inv[i] = lc_pow2(-x);
+      const int i = it * RPP + tid / LPR;
+      lc_put4(sm + L::K_HI, sm + L::K_LO, i, kc, L::KP, kr[it], lc_biased(lc_row(ke, it)));
+      if (tid % LPR == 0) k_inv[i] = lc_inverse(lc_row(ke, it));
     }
 #pragma unroll
     for (int it = 0; it < VN; ++it) {
-      const int i = it * (LC / VN) + (tid >> 4), x = lc_row_scale(ve, it);
-      lc_put4(sm + L::V_HI, sm + L::V_LO, i, vc, L::VP, vr[it], lc_pow2(x));
-      if ((tid & 15) == 0) v_inv[i] = lc_pow2(-x);
+      const int i = it * (LC / VN) + (tid >> 4);
+      lc_put4(sm + L::V_HI, sm + L::V_LO, i, vc, L::VP, vr[it], lc_biased(lc_row(ve, it)));
+      if ((tid & 15) == 0) v_inv[i] = lc_inverse(lc_row(ve, it));
     }
     if (QN != KN) load_q(0);
     put_q(0);
@@ -457,17 +468,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
       // (nt, half, e) is apart by base - 8 (nt - half) - e tokens: the weight of half 1 is the one half 0 had a tile before.
       // The factors one after the other: two of them together could leave the range of float32.
       const float* pb = pw + (i0 + g - t2);
-      const float q_inv0 = lc_pow2(-q_exp[i0 + g]), q_inv1 = lc_pow2(-q_exp[i0 + g + 8]);
+      const float q_inv0 = lc_inverse(q_scale[i0 + g]), q_inv1 = lc_inverse(q_scale[i0 + g + 8]);
       float m0 = 0.f, m1 = 0.f, b0 = pb[8], b1 = pb[7];
 #pragma unroll
       for (int nt = 0; nt < 8; ++nt)
         if (nt < 2 * r + 2) {
           const float a0 = pb[-8 * nt], a1 = pb[-8 * nt - 1];
-          const float2 k2 = *reinterpret_cast<const float2*>(k_inv + 8 * nt + t2), v2 = *reinterpret_cast<const float2*>(v_inv + 8 * nt + t2);
-          P[nt][0] = P[nt][0] * q_inv0 * a0 * k2.x * v2.x;
-          P[nt][1] = P[nt][1] * q_inv0 * a1 * k2.y * v2.y;
-          P[nt][2] = P[nt][2] * q_inv1 * b0 * k2.x * v2.x;
-          P[nt][3] = P[nt][3] * q_inv1 * b1 * k2.y * v2.y;
+          float2 k2 = *reinterpret_cast<const float2*>(k_inv + 8 * nt + t2);
+          const float2 v2 = *reinterpret_cast<const float2*>(v_inv + 8 * nt + t2);
+          if (v2.x == 0.f) k2.x = 0.f;                 // a token without a value: its score counts nothing, however large its weight
+          if (v2.y == 0.f) k2.y = 0.f;
+          P[nt][0] = P[nt][0] * q_inv0 * k2.x * a0 * v2.x;
+          P[nt][1] = P[nt][1] * q_inv0 * k2.y * a1 * v2.y;
+          P[nt][2] = P[nt][2] * q_inv1 * k2.x * b0 * v2.x;
+          P[nt][3] = P[nt][3] * q_inv1 * k2.y * b1 * v2.y;
           if (nt >= 2 * r) {                            // the tiles on the diagonal
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -516,7 +530,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
         const int i = i0 + g + 8 * half;
         if (i < n) {
           // the factors one after the other where their product could leave the range of float32
-          const float f_o0 = s_inv * (half ? q_inv1 : q_inv0), f_o1 = p.o_scale * pw[i + (undecayed ? 0 : 1)];
+          const float f_o0 = s_inv * (half ? q_inv1 : q_inv0), f_o1 = la_finite(p.o_scale * pw[i + (undecayed ? 0 : 1)]);
           const float f_p0 = half ? p_inv1 : p_inv0, f_p1 = p.o_scale * p.k_scale;
           float* row = o_base + (tok0 * p.os.t + (c0 + i) * o_t);
           if (VEC && !p.accumulate) {
@@ -635,7 +649,7 @@ __global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaC
   const int kc = (tid % LPR) * 4, vc = (tid & 15) * 4;
   const float* k = p.k + (int64_t)b * p.ks.b + (int64_t)(h / p.ks.div) * p.ks.h + (tok0 * p.ks.t + (first + tid / LPR) * k_t);
   const float* v = p.v + (int64_t)b * p.vs.b + (int64_t)(h / p.vs.div) * p.vs.h + v0 + (tok0 * p.vs.t + (first + (tid >> 4)) * v_t);
-  if (tid <= LC) pw[tid] = (float)la_power(c.decay[h], tid);
+  if (tid <= LC) pw[tid] = la_power32(c.decay[h], tid);
 
   float4 kr[KN], vr[VN];
   auto load = [&](int64_t c0) {       // rows of the chunk at c0 (a step of this segment); zero behind the end
@@ -660,14 +674,14 @@ __global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaC
   for (int64_t c0 = first; c0 < n_end; c0 += LC) {
     const int n = (int)min((int64_t)LC, n_end - c0);
     uint32_t ke[KN / 2], ve[VN / 2];
-    lc_row_exponents<LPR>(ke, kr);
-    lc_row_exponents<16>(ve, vr);
+    lc_row_scales<LPR>(ke, kr);
+    lc_row_scales<16>(ve, vr);
 #pragma unroll
     for (int it = 0; it < KN; ++it)
-      if (tid % LPR == 0) k_inv[it * RPP + tid / LPR] = lc_pow2(-lc_row_scale(ke, it));
+      if (tid % LPR == 0) k_inv[it * RPP + tid / LPR] = lc_inverse(lc_row(ke, it));
 #pragma unroll
     for (int it = 0; it < VN; ++it)
-      if ((tid & 15) == 0) v_inv[it * (LC / VN) + (tid >> 4)] = lc_pow2(-lc_row_scale(ve, it));
+      if ((tid & 15) == 0) v_inv[it * (LC / VN) + (tid >> 4)] = lc_inverse(lc_row(ve, it));
     __syncthreads();      // the scales are in place, and the tiles of the chunk before are free
     float u0, u1, f0, f1;
     lc_weights(u0, u1, f0, f1, pw, k_inv, v_inv, n, lane);
@@ -675,10 +689,10 @@ __global__ void __launch_bounds__(LS_THREADS, 2) la_state_kernel(LaCommon c, LaC
     for (int it = 0; it < KN; ++it) {
       const int i = it * RPP + tid / LPR;
       const float u = __shfl_sync(0xffffffffu, it * RPP < 32 ? u0 : u1, i & 31);
-      lc_put4(sm, sm + K_LO, i, kc, KP, kr[it], lc_pow2(lc_row_scale(ke, it)) * u);
+      lc_put4(sm, sm + K_LO, i, kc, KP, kr[it], lc_biased(lc_row(ke, it)) * u);
     }
 #pragma unroll
-    for (int it = 0; it < VN; ++it) lc_put4(sm + V_HI, sm + V_LO, it * (LC / VN) + (tid >> 4), vc, VP, vr[it], lc_pow2(lc_row_scale(ve, it)));
+    for (int it = 0; it < VN; ++it) lc_put4(sm + V_HI, sm + V_LO, it * (LC / VN) + (tid >> 4), vc, VP, vr[it], lc_biased(lc_row(ve, it)));
     __syncthreads();
     if (c0 + LC < n_end) load(c0 + LC);
     const float keep = pw[n];
@@ -743,7 +757,7 @@ __global__ void __launch_bounds__(256) la_segments_kernel(LaCommon c, LaChunkRun
   const double l = c.decay[h];
   float S = 0.f;
   if (p.s_in) S = p.s_in[bh * states + (p.s_in_t ? (e % p.dv) * p.dk + e / p.dv : e)];
-  const float full = (float)la_power(l, seg_tokens);
+  const float full = la_power32(l, seg_tokens);
   for (int s0 = 0; s0 < segments; s0 += 4) {
     float add[4];
     float* at = cr.work + ((int64_t)s0 * c.B * c.H + bh) * states + e;
@@ -758,7 +772,7 @@ __global__ void __launch_bounds__(256) la_segments_kernel(LaCommon c, LaChunkRun
       const int64_t left = (int64_t)n - (int64_t)s * seg_tokens;
       const int count = (int)(left < 0 ? 0 : left < seg_tokens ? left : seg_tokens);
       const int times = (p.reverse && s == 0 && count > 0) ? count - 1 : count;
-      const float f = times == 0 ? 1.f : times == seg_tokens ? full : (float)la_power(l, times);
+      const float f = times == 0 ? 1.f : times == seg_tokens ? full : la_power32(l, times);
       if (count > 0) S = f * S + add[i];
     }
   }

@@ -108,3 +108,27 @@ def test_a_prompt_agrees_with_answering_token_by_token(handler, T):
     bound = _bounds(d, 1.0)
     for name, a in (('out', out), ('state_out', p['state'])):
         _check(whole[name], h.get_numpy_copy(a).astype(np.float64), 2 * bound[name], 'two forms')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('scale', [1.0, 4.0])
+@pytest.mark.parametrize('decay', [30.0, -1e6])
+@pytest.mark.parametrize('T, B', [(8, 2), (60, 2), (200, 40), (700, 1)])
+def test_powers_of_a_large_decay_beyond_float32_meet_zeros(handler, T, B, decay, scale):
+    """Keys before the last four tokens, or gradients behind the first four, are zero: powers of the decay that leave the range
+    of float32 multiply nothing else."""
+    d = _case(T, B, 2, 2, 32, 40, seed=4, decays=[decay, 0.5])
+    d['k'][:T - 4], d['state'][:] = 0, 0
+    with np.errstate(all='ignore'):
+        got, want, bound = _run(handler, d, scale, backward=False), _all(d, scale), _bounds(d, scale)
+    for name in ('out', 'state_out'):
+        _check(got[name], want[name], bound[name], name)
+    d = _case(T, B, 2, 2, 32, 40, seed=5, decays=[decay, 0.5])
+    for name in ('dout', 'k', 'v'):
+        d[name][4:] = 0
+    d['state'][:], d['dstate_out'][:] = 0, 0
+    with np.errstate(all='ignore'):                       # the states behind the first tokens do overflow
+        got, want, bound = _run(handler, d, scale), _all(d, scale), _bounds(d, scale)
+    for name in ('dk', 'dv', 'dstate', 'dq'):
+        n = 4 if name == 'dq' else None
+        _check(got[name][:n], want[name][:n], bound[name][:n], name)
