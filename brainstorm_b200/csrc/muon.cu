@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const float* grad, f
   }
 }
 
-__device__ __forceinline__ float muon_inverse_norm(const double* partial, int count, double* red) {
+// The factor that makes planes of u / (|u| + 1e-7).  Formed in 64 bits: the inverse of a norm above 2^126 alone would lose bits in 32.
+__device__ __forceinline__ float muon_plane_factor(const double* partial, int count, double* red) {
   double s = 0.;
   for (int i = threadIdx.x; i < count; i += blockDim.x) s += partial[i];
 #pragma unroll
@@ -72,7 +73,7 @@ __device__ __forceinline__ float muon_inverse_norm(const double* partial, int co
   __syncthreads();
   double t = 0.;
   for (int w = 0; w < (int)(blockDim.x >> 5); ++w) t += red[w];
-  return (float)(1. / (sqrt(t) + 1e-7));
+  return (float)((double)NS_SCALE / (sqrt(t) + 1e-7));
 }
 
 __device__ __forceinline__ void muon_split(float x, float y, __half2& hi, __half2& lo) {
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(256) muon_start_kernel(const float* grad, cons
       }
     }
   }
-  const float inv = NS_SCALE * muon_inverse_norm(partial + blockIdx.z * partials, partials, red);
+  const float inv = muon_plane_factor(partial + blockIdx.z * partials, partials, red);
   __half2 hi, lo;
 #pragma unroll
   for (int y = 0; y < 8; ++y) {

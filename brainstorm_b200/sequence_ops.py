@@ -374,7 +374,8 @@ class SequenceOps(object):
 
         ``orthogonalised(u)`` is ``steps`` Newton-Schulz iterations ``X = 3.4445 X + (-4.7750 A + 2.0315 A A) X`` with
         ``A = X X^T`` from ``u / (|u| + 1e-7)``: the singular values of ``u`` are all brought near one, each matrix of
-        a stack on its own.  A zero direction gives a zero update."""
+        a stack on its own.  A zero direction gives a zero update.  Values of ``X`` have 22 bits and are held to 2^-37 at
+        least: where ``|u|`` is below 1e-7 so is the update's precision, relative to its then small size."""
         if len(param.shape) not in (2, 3):
             raise ValueError('expected matrices, got shape %r' % (param.shape,))
         if not 0 <= steps <= 100 or int(steps) != steps:

@@ -422,7 +422,7 @@ int b200_bias_act(float* out, const float* bias, int64_t rows, int64_t cols, int
  *      grad; u = grad + beta momentum if nesterov, else momentum; X = u / (|u|_F + 1e-7);
  *      `steps` times X = a X + (b A + c A A) X with A = X X^T and (a, b, c) = (3.4445,
  *      -4.7750, 2.0315); update = X; param = (1 - learning_rate * weight_decay) param -
- *      learning_rate * X.  16-byte aligned scratch of b200_muon_scratch_floats floats.  The
+ *      learning_rate * X.  Values of X have 22 bits and are held to 2^-37 at least.  16-byte aligned scratch of b200_muon_scratch_floats floats.  The
  *      four arrays must not overlap. ---------------------------------------------------- */
 typedef struct {
   const float *q, *k, *v, *decay;
