@@ -19,7 +19,9 @@
 // Bound: HBM where rows fill the vectors.  Forward moves 5 arrays, backward 8: 8192 x 4096 in 117 and 197 us, 5.7 and
 // 5.5 TB/s.  Rows that start anywhere (3001 x 1537): 31 and 52 us, 3.0 and 2.9 TB/s, the latency of a row's two sums in the
 // blocks that registers allow; the next row through shared memory instead of L2 gave 30 and 61.  Few rows: the
-// latency of one (128 x 1000: 3.3 and 7.0 us).
+// latency of one (128 x 1000: 3.3 and 7.0 us).  Rows of 8193 to 16384 values hold 16 floats a thread on 1024 threads, whose 64
+// registers are too few for a backward pass: 1500 x 16384 127 and 394 us (floors 75 and 120), 1500 x 16383, by single loads, 278 and 832.
+// Added gradients read what was there: 8192 x 4096 294 us (floor 226), 3001 x 1537 67 (31), 1000000 x 32 809 (215).
 #include <algorithm>
 #include <initializer_list>
 #include <utility>

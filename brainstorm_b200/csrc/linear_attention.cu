@@ -3,7 +3,8 @@
 //
 // Bound for a single token: HBM, the state is read once and written once (8 dk dv bytes) and everything else is small;
 // the state, k, q and v are all asked for at once, and the registers are held to what lets six blocks of 128 threads
-// share an SM (512 x 16 states of 128 x 128: 173 us, the floor being 166; five blocks 184, eight 189).  For several tokens: latency.
+// share an SM (512 x 16 states of 128 x 128: 173 us on the device under the profiler, where five blocks took 184 and eight
+// 189; a whole call 188 to 190; floor 166).  For several tokens: latency.
 #include <string.h>
 
 #include <algorithm>
@@ -396,7 +397,13 @@ __global__ void __launch_bounds__(256) la_share_kernel(const float* src, float* 
   }
 }
 
-constexpr int LA_RECURRENT_TOKENS = 8;      // sequences of up to this many tokens take the recurrent form
+// Sequences of up to this many tokens take the recurrent form.  Its time grows with the tokens, that of a chunk hardly does; they meet
+// at 6 to 11 tokens (forward / gradients in us on the device, recurrent against chunked):
+//   tokens, 8 heads of 64            4: 5.3 / 5.2, 6.4 / 6.3       8: 8.1 / 8.1, 6.5 / 6.3        12: 10.9 / 10.8, 6.7 / 6.5
+//   128 x 16 heads of 64             4: 22 / 68, 46 / 126          8: 38 / 110, 47 / 127          12: 54 / 154, 49 / 133
+//   64 x 16 heads of 128             4: 51 / 133, 93 / 262         8: 79 / 212, 94 / 267          12: 108 / 292, 97 / 276
+//   64 x 8 heads over 2, 40 and 75   4: 19 / 112, 27 / 87          8: 31 / 185, 27 / 87           12: 44 / 260, 29 / 93
+constexpr int LA_RECURRENT_TOKENS = 8;
 
 static int la_run(const LaCommon& c, const LaRun* runs, int count, float* work) {
   return c.T <= LA_RECURRENT_TOKENS ? la_recurrent(c, runs, count) : la_chunked(c, runs, count, work);

@@ -25,11 +25,15 @@
 // Few sequences and heads: the time axis is cut into segments.  A first pass computes what each segment adds
 // to the state, a second one hands the state through, then all segments run side by side.
 //
-// Bound: neither memory nor the tensor pipe (33 and 25 % of the clocks at d = 128 and 64) but the latency between
+// Bound: neither memory nor the tensor pipe (33 and 26 % of the clocks at d = 128 and 64) but the latency between
 // dependent instructions: registers and shared memory let two or three blocks onto an SM, two or three warps a
-// scheduler, which issue in 36 to 43 % of the clocks.  Measured: 8192 x 2 x 16 heads of 128 598 us (state pass 160, handing
-// through 20, outputs 420), HBM time 83; 100 x 128 x 16 heads of 64 with gradients 454 us, HBM time 114; 1999 x 6 x 12 heads
-// of 48 and 80 over 4, ragged, with gradients 567 us, HBM time 39.
+// scheduler, which issue in 38 to 46 % of the clocks.  Measured: 8192 x 2 x 16 heads of 128 623 us (state pass 165, handing
+// through 20, outputs 435), HBM time 83; 100 x 128 x 16 heads of 64 with gradients 508 us, HBM time 114; 1999 x 6 x 12 heads
+// of 48 and 80 over 4, ragged, with gradients 605 us, HBM time 39.  (With one scale for all of a chunk's keys, and one for
+// its values, 598, 454 and 570 us, but a token then lost bits to later ones.)
+//
+// Errors against 64 bits, of |out| and of the gradients together: 4 to 7e-7, two to three times those of sums in float32:
+// sums on the tensor core truncate.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -780,8 +784,14 @@ __global__ void __launch_bounds__(256) la_segments_kernel(LaCommon c, LaChunkRun
 }
 
 // Segments for `blocks` blocks of one segment: as many as use the resident blocks of the GPU best, where
-// the main pass costs its chunks, the state pass 0.4 of that, and a segment's state about three chunks to
-// write, hand through and read.
+// the main pass costs its chunks, the state pass 0.4 of that (165 us beside 435), and a segment's state about three chunks to
+// write, hand through and read.  Measured with the number of segments forced, forward / gradients in us:
+//   8192 x 2 x 16 heads of 128    1: 1101 / 1718    2: 785 / 2041    4: 617 / 1646    8: 641 / 1660     taken: 617 / 1552
+//   8192 x 8 heads of 64          1: 723 / 727      4: 241 / 251     12: 90 / 149     16: 69 / 132      taken: 68 / 133
+//   2000 x 4 heads of 128         1: 269 / 269      4: 104 / 106     12: 48 / 74      16: 38 / 87       taken: 38 / 74
+//   700 x 4 x 8 heads of 64       1: 63 / 63        2: 53 / 83       4: 31 / 56       8: 36 / 70        taken: 31 / 56
+//   1999 x 6 x 12 of 48 and 80    1: 171 / 474      2: 197 / 587     3: 186 / 607     4: 212 / 571      taken: 186 / 474
+//   the same, ragged              1: 226 / 423      2: 199 / 518     3: 169 / 531     8: 177 / 530      taken: 171 / 421
 static int lc_segments(int64_t T, int64_t blocks, int resident) {
   const int64_t chunks = ceil_div(T, LC);
   int best = 1;

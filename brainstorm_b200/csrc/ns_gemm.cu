@@ -501,9 +501,17 @@ static int ns_map(const NsMatrix& a, bool mn, int batch, int rows, CUtensorMap* 
   return B200_OK;
 }
 
-// What the truncating accumulation of a chunk takes from a sum of one sign, on the average.  Measured as the factor that
-// makes five Newton-Schulz steps most exact at seven shapes from 64 x 3000 to 4096 x 4096: the error against 64 bits falls
-// from 2.2 - 4.2e-6 to 0.9 - 2.6e-6 (float32 products: 1.5 - 4.8e-6); a sum without a sign does not notice 2^-22.
+// What the truncating accumulation of a chunk takes from a sum of one sign, on the average: without it one Newton-Schulz step
+// makes X too small by 2 to 9e-7 at every shape tried.  Chosen at seven shapes from 64 x 3000 to 4096 x 4096; at others, in all forms of the
+// products, the error against 64 bits of one step / of five, without it and with it:
+//   16 x 65     3.4e-7 / 1.4e-6   1.7e-7 / 1.6e-6        300 x 700              4.5e-7 / 2.0e-6   2.1e-7 / 0.8e-6
+//   64 x 65     6.4e-7 / 4.0e-6   3.1e-7 / 2.0e-6        513 x 640              4.8e-7 / 2.2e-6   2.0e-7 / 0.9e-6
+//   130 x 129   6.0e-7 / 3.9e-6   2.8e-7 / 1.9e-6        30 x 210 x 215         5.7e-7 / 2.0e-6   2.7e-7 / 0.9e-6
+//   128 x 193   5.9e-7 / 3.6e-6   2.8e-7 / 1.6e-6        40 x 165 x 170         7.4e-7 / 3.6e-6   4.1e-7 / 1.9e-6
+//   48 x 200    5.6e-7 / 3.1e-6   2.5e-7 / 1.1e-6        20 x 390 x 395         9.4e-7 / 4.4e-6   6.2e-7 / 2.9e-6
+//   20 x 20     4.9e-7 / 2.0e-6   2.2e-7 / 1.0e-6        2100 x 2100            3.1e-7 / 3.4e-6   2.6e-7 / 1.9e-6
+// A sum of up to 8 products truncates little; there the factor is an error of its own size: 1 x 1 0.9e-7 / 6.1e-7 and 2.6e-7 / 0.8e-7,
+// 3 x 7 2.1e-7 / 2.1e-7 and 2.7e-7 / 7.4e-7, 4 x 4 2.1e-7 / 5.0e-7 and 2.1e-7 / 7.0e-7, 8 x 8 2.4e-7 / 1.2e-6 and 2.3e-7 / 1.3e-6.
 constexpr float NS_GAIN = 1.f + 0x1p-22f;
 
 typedef void (*NsKernel)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, NsOut, int, int, int, int, int, int, int, int*);

@@ -211,8 +211,8 @@ class SequenceOps(object):
                 inputs hold behind the end is not read.
 
         dk, dv: 1 to 128.  A non-finite value of a token spreads to later tokens of its sequence and head, and may
-        spread to up to 15 tokens before it.  Products are as exact as in float32 (22 bits of each operand, sums in float32).
-        From 9 tokens on, a value more than 2^17 below the largest of its row (one token and head of ``q``, ``k``, ``v`` or
+        spread to up to 15 tokens before it.  Up to 8 tokens everything is float32.  From 9 on operands have 22 bits and sums on
+        the tensor core truncate (errors are two to three times those of float32 sums), and a value more than 2^17 below the largest of its row (one token and head of ``q``, ``k``, ``v`` or
         ``dout``, and the state) keeps fewer bits: it is held to 2^-38 of that largest value.  Other tokens do not matter."""
         T, B, H, K, dk, dv = self._attention_shapes(q, k, v, 4)
         _expect(out, (T, B, H, dv), 'out')
@@ -294,7 +294,8 @@ class SequenceOps(object):
                 block), ``gate=None`` the gate.
             w_post, scale, w_pre: vectors of ``width`` values, or None for ones.
             r_post, r_pre: (rows,) receive ``1 / rms`` of ``y`` and ``x_out``, which the backward pass needs.
-            epsilon: added to the mean squares.
+            epsilon: added to the mean squares, which are float32: values from 1.8e19 on leave its range, and a row that holds one
+                has the norm 0.
             activation: 'sigmoid', 'tanh', 'rel', 'el' or 'linear'.
 
         width: up to 16384.  ``x_out`` may be ``x`` and ``h_out`` may be ``y``, the same view; no other output may overlap
