@@ -295,7 +295,7 @@ class SequenceOps(object):
             w_post, scale, w_pre: vectors of ``width`` values, or None for ones.
             r_post, r_pre: (rows,) receive ``1 / rms`` of ``y`` and ``x_out``, which the backward pass needs.
             epsilon: added to the mean squares, which are float32: values from 1.8e19 on leave its range, and a row that holds one
-                has the norm 0.
+                is normalised to zeros.
             activation: 'sigmoid', 'tanh', 'rel', 'el' or 'linear'.
 
         width: up to 16384.  ``x_out`` may be ``x`` and ``h_out`` may be ``y``, the same view; no other output may overlap
