@@ -213,7 +213,8 @@ class SequenceOps(object):
         dk, dv: 1 to 128.  A non-finite value of a token spreads to later tokens of its sequence and head, and may
         spread to up to 15 tokens before it.  Up to 8 tokens everything is float32.  From 9 on operands have 22 bits and sums on
         the tensor core truncate (errors are two to three times those of float32 sums), and a value more than 2^17 below the largest of its row (one token and head of ``q``, ``k``, ``v`` or
-        ``dout``, and the state) keeps fewer bits: it is held to 2^-38 of that largest value.  Other tokens do not matter."""
+        ``dout``, and the state) keeps fewer bits: it is held to 2^-38 of that largest value, and so is a token's part in an output
+        beside the largest part.  Later tokens do not matter."""
         T, B, H, K, dk, dv = self._attention_shapes(q, k, v, 4)
         _expect(out, (T, B, H, dv), 'out')
         strides = 0
