@@ -38,6 +38,7 @@
 
 #include <algorithm>
 
+#include "half_split.cuh"
 #include "linear_attention.cuh"
 
 namespace b200 {
@@ -114,18 +115,6 @@ __device__ __forceinline__ void lc_rows(float (&c)[N][4], const uint32_t (&ah)[4
     }
 }
 __device__ __forceinline__ uint32_t lc_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// two values as (hi, hi) and (lo, lo): lo = fp16(x - hi), the difference in one mixed-precision operation
-__device__ __forceinline__ void lc_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  asm("{\n\t.reg .f32 r0, r1;\n\t.reg .b16 h0, h1, m;\n\t"
-      "cvt.rn.f16x2.f32 %0, %3, %2;\n\t"
-      "mov.b32 {h0, h1}, %0;\n\t"
-      "mov.b16 m, 0xBC00;\n\t"                       // -1
-      "fma.rn.f32.f16 r0, h0, m, %2;\n\t"
-      "fma.rn.f32.f16 r1, h1, m, %3;\n\t"
-      "cvt.rn.f16x2.f32 %1, r1, r0;\n\t}"
-      : "=&r"(hi), "=r"(lo)
-      : "f"(x), "f"(y));
-}
 // (hi + lo) of two values
 __device__ __forceinline__ float2 lc_join(uint32_t hi, uint32_t lo) {
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&hi)), b = __half22float2(*reinterpret_cast<const __half2*>(&lo));
@@ -230,8 +219,8 @@ __device__ __forceinline__ void lc_weights(float& u0, float& u1, float& f0, floa
 }
 __device__ __forceinline__ void lc_put4(uint8_t* hi, uint8_t* lo, int row, int c, int pitch, float4 x, float s) {
   uint32_t h0, l0, h1, l1;
-  lc_split(x.x * s, x.y * s, h0, l0);
-  lc_split(x.z * s, x.w * s, h1, l1);
+  split_halves(x.x * s, x.y * s, h0, l0);
+  split_halves(x.z * s, x.w * s, h1, l1);
   const uint32_t at = lc_at(row, c >> 3, pitch) + ((c & 4) << 1);
   *reinterpret_cast<uint2*>(hi + at) = make_uint2(h0, h1);
   *reinterpret_cast<uint2*>(lo + at) = make_uint2(l0, l1);
@@ -429,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
           uint32_t hi, lo;
-          lc_split(S[m][nt][e] * s_scale, S[m][nt][e + 1] * s_scale, hi, lo);
+          split_halves(S[m][nt][e] * s_scale, S[m][nt][e + 1] * s_scale, hi, lo);
           const uint32_t at = lc_at(row_of(m, e), nt0 + nt, L::VP) + t2 * 2;
           *reinterpret_cast<uint32_t*>(sm + L::S_HI + at) = hi;
           *reinterpret_cast<uint32_t*>(sm + L::S_LO + at) = lo;
@@ -522,10 +511,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
       for (int jt = 0; jt < 4; ++jt)
         if (jt <= r) {
           uint32_t ah[4], al[4];
-          lc_split(P[2 * jt][0] * p_s0, P[2 * jt][1] * p_s0, ah[0], al[0]);
-          lc_split(P[2 * jt][2] * p_s1, P[2 * jt][3] * p_s1, ah[1], al[1]);
-          lc_split(P[2 * jt + 1][0] * p_s0, P[2 * jt + 1][1] * p_s0, ah[2], al[2]);
-          lc_split(P[2 * jt + 1][2] * p_s1, P[2 * jt + 1][3] * p_s1, ah[3], al[3]);
+          split_halves(P[2 * jt][0] * p_s0, P[2 * jt][1] * p_s0, ah[0], al[0]);
+          split_halves(P[2 * jt][2] * p_s1, P[2 * jt][3] * p_s1, ah[1], al[1]);
+          split_halves(P[2 * jt + 1][0] * p_s0, P[2 * jt + 1][1] * p_s0, ah[2], al[2]);
+          split_halves(P[2 * jt + 1][2] * p_s1, P[2 * jt + 1][3] * p_s1, ah[3], al[3]);
           lc_rows(acc_p, ah, al, lc_smem(sm + L::V_HI), lc_smem(sm + L::V_LO), 16 * jt, lane, nt0, nt_n);
         }
       // ---- out
@@ -586,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
 #pragma unroll
                 for (int r = 2 * e; r < 2 * e + 2; ++r) {
                   const float2 y = lc_join(ah[r], al[r]);
-                  lc_split(y.x * w0, y.y * w1, ah[r], al[r]);
+                  split_halves(y.x * w0, y.y * w1, ah[r], al[r]);
                 }
               }
             }

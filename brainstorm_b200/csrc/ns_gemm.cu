@@ -32,6 +32,7 @@
 
 #include <algorithm>
 
+#include "half_split.cuh"
 #include "ns_gemm.cuh"
 #include "tc_ptx.cuh"
 
@@ -106,19 +107,6 @@ static int ns_tiles(int tiles_m, int tiles_n, int bm, int bn, bool symmetric) {
   return n;
 }
 
-// two values as (hi, hi) and (lo, lo): lo = fp16(x - hi), the difference in one mixed-precision operation
-__device__ __forceinline__ void ns_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  asm("{\n\t.reg .f32 r0, r1;\n\t.reg .b16 h0, h1, m;\n\t"
-      "cvt.rn.f16x2.f32 %0, %3, %2;\n\t"
-      "mov.b32 {h0, h1}, %0;\n\t"
-      "mov.b16 m, 0xBC00;\n\t"                       // -1
-      "fma.rn.f32.f16 r0, h0, m, %2;\n\t"
-      "fma.rn.f32.f16 r1, h1, m, %3;\n\t"
-      "cvt.rn.f16x2.f32 %1, r1, r0;\n\t}"
-      : "=&r"(hi), "=r"(lo)
-      : "f"(x), "f"(y));
-}
-
 // W columns (64 or 32) of a warp's 32 rows: from acc (lane: row row0 + lane; columns col ..) to the planes.  Rows go
 // through shared memory (`buf`, this warp's: both planes, 32 rows of W halves and 16 bytes), so that whole rows of a
 // tile meet global memory together: a lane that stored its own row touched 32 lines an instruction, which made the
@@ -137,7 +125,7 @@ __device__ __forceinline__ void ns_store(const float* acc, uint8_t* buf, const N
 #pragma unroll
     for (int u = 0; u < 8; ++u) x[u] = alpha * acc[8 * c8 + u] + (on == 8 * c8 + u ? diagonal : 0.f);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) ns_split(x[2 * u], x[2 * u + 1], hi[u], lo[u]);
+    for (int u = 0; u < 4; ++u) split_halves(x[2 * u], x[2 * u + 1], hi[u], lo[u]);
     *reinterpret_cast<uint4*>(mine + 16 * c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     *reinterpret_cast<uint4*>(mine + PLANE + 16 * c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
