@@ -27,9 +27,9 @@
 //
 // Bound: neither memory nor the tensor pipe (33 and 26 % of the clocks at d = 128 and 64) but the latency between
 // dependent instructions: registers and shared memory let two or three blocks onto an SM, two or three warps a
-// scheduler, which issue in 38 to 46 % of the clocks.  Measured: 8192 x 2 x 16 heads of 128 623 us (state pass 165, handing
-// through 20, outputs 435), HBM time 83; 100 x 128 x 16 heads of 64 with gradients 508 us, HBM time 114; 1999 x 6 x 12 heads
-// of 48 and 80 over 4, ragged, with gradients 605 us, HBM time 39.  (With one scale for all of a chunk's keys, and one for
+// scheduler, which issue in 38 to 46 % of the clocks.  Measured: 8192 x 2 x 16 heads of 128 626 us (state pass 165, handing
+// through 20, outputs 435), HBM time 83; 100 x 128 x 16 heads of 64 with gradients 511 us, HBM time 114; 1999 x 6 x 12 heads
+// of 48 and 80 over 4, ragged, with gradients 596 to 628 us, HBM time 39.  (With one scale for all of a chunk's keys, and one for
 // its values, 598, 454 and 570 us, but a token then lost bits to later ones.)
 //
 // Errors against 64 bits, of |out| and of the gradients together: 4 to 7e-7, two to three times those of sums in float32:
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
       }
       // ---- weights, the scales of q, k and v taken back, and mask, then the scores' own scale for each row.  Element
       // (nt, half, e) is apart by base - 8 (nt - half) - e tokens: the weight of half 1 is the one half 0 had a tile before.
-      // The factors one after the other: two of them together could leave the range of float32.
+      // Those of q and k together are out of the range of float32 only where the score is; the others one after the other.
       const float* pb = pw + (i0 + g - t2);
       const float q_inv0 = lc_inverse(q_scale[i0 + g]), q_inv1 = lc_inverse(q_scale[i0 + g + 8]);
       float m0 = 0.f, m1 = 0.f, b0 = pb[8], b1 = pb[7];
@@ -471,10 +471,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 1 : DK == 64 ? 3 : 2
           const float2 v2 = *reinterpret_cast<const float2*>(v_inv + 8 * nt + t2);
           if (v2.x == 0.f) k2.x = 0.f;                 // a token without a value: its score counts nothing, however large its weight
           if (v2.y == 0.f) k2.y = 0.f;
-          P[nt][0] = P[nt][0] * q_inv0 * k2.x * a0 * v2.x;
-          P[nt][1] = P[nt][1] * q_inv0 * k2.y * a1 * v2.y;
-          P[nt][2] = P[nt][2] * q_inv1 * k2.x * b0 * v2.x;
-          P[nt][3] = P[nt][3] * q_inv1 * k2.y * b1 * v2.y;
+          P[nt][0] = P[nt][0] * (q_inv0 * k2.x) * a0 * v2.x;
+          P[nt][1] = P[nt][1] * (q_inv0 * k2.y) * a1 * v2.y;
+          P[nt][2] = P[nt][2] * (q_inv1 * k2.x) * b0 * v2.x;
+          P[nt][3] = P[nt][3] * (q_inv1 * k2.y) * b1 * v2.y;
           if (nt >= 2 * r) {                            // the tiles on the diagonal
 #pragma unroll
             for (int e = 0; e < 4; ++e)

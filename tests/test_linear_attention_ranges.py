@@ -94,6 +94,18 @@ def test_keys_and_values_whose_product_is_outside_the_range_of_their_scales(hand
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('T', [9, 70, 700])
+def test_queries_near_the_end_of_float32(handler, T):
+    """Queries near 2^112 with keys near 2^-112, and the other way round: the scores are of ordinary size."""
+    d = _case(T, 2, 4, 2, 32, 32, seed=6, decays=DECAYS)
+    for b, power in enumerate((112, -112)):
+        d['q'][:, b] *= np.float32(2.0 ** power)
+        d['k'][:, b] *= np.float32(2.0 ** -power)
+        d['state'][b] *= np.float32(2.0 ** -power)
+    _check_all(handler, d, 1.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('T', [8, 60])
 def test_a_prompt_agrees_with_answering_token_by_token(handler, T):
     """The two forms, on tokens of which the last is by far the largest."""
